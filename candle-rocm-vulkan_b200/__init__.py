@@ -9,6 +9,8 @@ from . import _abi  # noqa: F401
 from . import config  # noqa: F401
 from . import flash_attn  # noqa: F401
 from . import offload  # noqa: F401
+from . import paged  # noqa: F401
 from .offload import CopyEvent, CopyStream, PinnedHostBuffer  # noqa: F401
+from .paged import PagedKvPool, RotaryAxes, rotary_axes  # noqa: F401
 from .turbo_quant import (FlashAttnConfig, KvBlockRef, OutputGather, PackedAttention, PackedBlocksAttention, QuantFormat,  # noqa: F401
                           QuantizedTensor, TurboKvCache, TurboQuantizer, attention_packed, attention_packed_blocks)

@@ -111,6 +111,37 @@ class FaArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class Rotary(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("axis", C.c_void_p), ("pos", C.c_void_p), ("pos_stride", C.c_uint64),
+                ("n_axes", C.c_uint32), ("rot", C.c_uint32), ("interleaved", C.c_uint32), ("inverse", C.c_uint32)]
+
+
+u64x2 = C.c_uint64 * 2
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+                ("q_strides", u64x2), ("k_strides", u64x2), ("q_out_strides", u64x2), ("k_out_strides", u64x2),
+                ("tokens", C.c_uint32), ("hq", C.c_uint32), ("hkv", C.c_uint32), ("d", C.c_uint32), ("dtype", C.c_int32), ("pad", C.c_uint32),
+                ("rotary", Rotary)]
+
+
+class PagedPool(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("k_strides", u64x3), ("v_strides", u64x3),
+                ("n_blocks", C.c_uint32), ("block_rows", C.c_uint32), ("hkv", C.c_uint32), ("d", C.c_uint32), ("dtype", C.c_int32), ("pad", C.c_uint32)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("pool", PagedPool), ("k", C.c_void_p), ("v", C.c_void_p), ("k_strides", u64x2), ("v_strides", u64x2), ("slots", C.c_void_p),
+                ("q", C.c_void_p), ("q_out", C.c_void_p), ("q_strides", u64x2), ("q_out_strides", u64x2), ("tokens", C.c_uint32), ("hq", C.c_uint32),
+                ("src_dtype", C.c_int32), ("pad", C.c_uint32), ("rotary", Rotary), ("status", C.c_void_p)]
+
+
+class PagedUnpackArgs(C.Structure):
+    _fields_ = [("pool", PagedPool), ("table", C.c_void_p), ("table_stride", C.c_uint64), ("cu_k", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("total", C.c_uint64), ("b", C.c_uint32), ("table_cols", C.c_uint32), ("dtype", C.c_int32), ("pad", C.c_uint32), ("status", C.c_void_p)]
+
+
 # every symbol that include/b200attn.h declares
 SYMBOLS = [
     "b200_row_layout", "b200_codebook", "b200_hadamard_signs", "b200_qjl_matrix", "b200_row_group", "b200_split_count_grouped",
@@ -118,6 +149,7 @@ SYMBOLS = [
     "b200_describe", "b200_last_error", "b200_tq_rotate", "b200_tq_quantize", "b200_tq_dequantize", "b200_kv_append", "b200_kv_unpack",
     "b200_tq_attention_workspace_bytes", "b200_tq_attention", "b200_tq_attention_static", "b200_tq_attention_gather",
     "b200_flash_attn_workspace_bytes", "b200_flash_attn_paged_workspace_bytes", "b200_flash_attn_paged",
+    "b200_rotary_axes", "b200_paged_append", "b200_paged_unpack",
     "b200_flash_attn", "b200_fa_prefill_append", "b200_device_wait_status", "b200_device_wait_check",
     "b200_pinned_alloc", "b200_pinned_free", "b200_pinned_len", "b200_pinned_wait_idle", "b200_pinned_ptr",
     "b200_copy_upload", "b200_copy_download", "b200_copy_event_wait_on_compute", "b200_copy_event_synchronize",
@@ -170,6 +202,9 @@ def lib():
         l.b200_flash_attn_paged_workspace_bytes.restype = C.c_size_t
         l.b200_flash_attn_paged.argtypes = [C.POINTER(FaArgs), C.c_void_p, C.c_uint32, C.c_void_p]
         l.b200_fa_prefill_append.argtypes = [C.POINTER(FaArgs), C.POINTER(KvAppendArgs), C.c_void_p]
+        l.b200_rotary_axes.argtypes = [C.c_void_p, C.c_void_p]  # the arguments' bytes, or a structure by reference
+        l.b200_paged_append.argtypes = [C.c_void_p, C.c_void_p]
+        l.b200_paged_unpack.argtypes = [C.c_void_p, C.c_void_p]
         l.b200_device_wait_check.argtypes = [C.c_int]
         l.b200_pinned_alloc.argtypes = [C.c_size_t, C.POINTER(C.c_void_p)]
         l.b200_pinned_free.argtypes = [C.c_void_p]

@@ -1,0 +1,239 @@
+"""A pool of cache pages for serving, and rotary positions with several axes, on top of libb200attn.so.
+
+One pool holds the keys and values of all sequences: equal pages, in the layout of `flash_attn_varlen_paged_windowed`
+((num_blocks, block_size, kv_heads, head_dim), candle-flash-attn/src/lib.rs:341-420), a table row per sequence that lists its
+pages, and one slot (block * block_size + row) per token. `append` turns the new queries and keys by their positions and writes
+keys and values, quantised where the pool holds MXFP8; `keys_values` reads sequences back.
+"""
+import ctypes as C
+import struct
+from typing import Optional, Sequence
+
+import torch
+
+from . import _abi as A
+from .turbo_quant import _dtype_id, _need_cuda, _stream
+
+_E4M3 = getattr(torch, "float8_e4m3fn", None)
+_POOL_DTYPES = {torch.float16: A.F16, torch.bfloat16: A.BF16, _E4M3: A.FP8}
+
+# the argument structures in the order of the header, packed in one go (as in turbo_quant.py)
+_POOL = struct.Struct("@4P3Q3Q4IiI")
+_ROTARY = "3PQ4I"
+_ROTARY_ARGS = struct.Struct("@4P2Q2Q2Q2Q4IiI" + _ROTARY)
+_APPEND_ARGS = struct.Struct("@2P2Q2Q3P2Q2QIIiI" + _ROTARY + "P")   # behind the pool
+_UNPACK_ARGS = struct.Struct("@PQ3PQIIiIP")                         # behind the pool
+assert _POOL.size == C.sizeof(A.PagedPool) and _ROTARY_ARGS.size == C.sizeof(A.RotaryArgs)
+assert _POOL.size + _APPEND_ARGS.size == C.sizeof(A.PagedAppendArgs) and _POOL.size + _UNPACK_ARGS.size == C.sizeof(A.PagedUnpackArgs)
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
+def _call(fn, args: bytes, device):
+    """The library call on the tensors' device and its current stream."""
+    if device.index == _current_device():
+        rc = fn(args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(args, _stream(device))
+    if rc:
+        A.check(rc)
+
+
+def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:
+    """Lengths, slots, positions and tables as the kernels read them: `dtype`, on the device, contiguous along the last axis."""
+    if t.dtype != dtype or t.device != device:
+        if t.dtype.is_floating_point or t.dtype == torch.bool:
+            raise ValueError(f"{what} must be whole numbers, got {t.dtype}")
+        t = t.to(device=device, dtype=dtype)
+    return t if t.stride(-1) == 1 or t.numel() <= 1 else t.contiguous()
+
+
+def _heads(t: torch.Tensor, what: str, tokens: Optional[int] = None, d: Optional[int] = None) -> torch.Tensor:
+    if t.dim() != 3 or (tokens is not None and t.shape[0] != tokens) or (d is not None and t.shape[2] != d):
+        raise ValueError(f"{what} must be ({'tokens' if tokens is None else tokens}, heads, {'head_dim' if d is None else d}), got {tuple(t.shape)}")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+class RotaryAxes:
+    """The frequencies of a rotary position and the axis that each of them goes by.
+
+    `freq`: rot / 2 frequencies (radians per position); a head's first rot elements are turned in pairs, pair f by
+    position[axis of f] * freq[f]. `sections`: how many frequencies, in order, go by axis 0, 1, 2 ... (time, height, width
+    of image and video patches; text has one position on all axes); `axes`: instead, the axis of every frequency. Neither:
+    one axis. `interleaved`: a pair is (2 f, 2 f + 1) instead of (f, f + rot / 2)."""
+
+    def __init__(self, freq, sections: Optional[Sequence[int]] = None, axes: Optional[Sequence[int]] = None, interleaved: bool = False, device="cuda"):
+        if isinstance(freq, torch.Tensor) and freq.is_cuda:
+            device = freq.device
+        self.freq = torch.as_tensor(freq, dtype=torch.float32, device=device).contiguous()
+        if self.freq.dim() != 1 or self.freq.numel() == 0 or self.freq.numel() % 8:
+            raise ValueError(f"rotary: frequencies must be a vector of a multiple of 8, got {tuple(self.freq.shape)}")
+        half = self.freq.numel()
+        self.rot, self.interleaved = 2 * half, bool(interleaved)
+        if sections is not None:
+            if axes is not None:
+                raise ValueError("rotary: sections or axes, not both")
+            sections = [int(n) for n in sections]
+            if min(sections, default=-1) < 0 or sum(sections) != half:
+                raise ValueError(f"rotary: sections {sections} do not add up to {half} frequencies")
+            axes = [a for a, n in enumerate(sections) for _ in range(n)]
+            self.n_axes = len(sections)
+        else:
+            axes = [int(a) for a in axes] if axes is not None else [0] * half
+            self.n_axes = max(axes, default=0) + 1
+        if len(axes) != half or min(axes) < 0 or self.n_axes > 256:
+            raise ValueError(f"rotary: {half} frequencies need an axis from 0 to 255 each")
+        self.axis = torch.tensor(axes, dtype=torch.uint8, device=self.freq.device)
+
+    def fields(self, positions: torch.Tensor, tokens: int, device, inverse: bool):
+        """(the values of a B200Rotary, the positions to keep alive)."""
+        pos = positions if positions.dim() == 2 else positions.reshape(1, -1) if positions.dim() == 1 else None
+        if pos is None or tuple(pos.shape) != (self.n_axes, tokens):
+            raise ValueError(f"rotary: positions must be ({self.n_axes}, {tokens}), got {tuple(positions.shape)}")
+        if self.freq.device != device:
+            raise ValueError("rotary: frequencies live on another device")
+        pos = _ints(pos, torch.int64, device, "rotary: positions")
+        return (self.freq.data_ptr(), self.axis.data_ptr(), pos.data_ptr(), pos.stride(0), self.n_axes, self.rot, int(self.interleaved), int(inverse)), pos
+
+
+_NO_ROTARY = (0, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _out_like(t: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    if out.shape != t.shape or out.dtype != t.dtype or out.device != t.device or out.stride(2) != 1:
+        raise ValueError(f"{what} must be a {t.dtype} {tuple(t.shape)} tensor on {t.device} with a contiguous head dim")
+    return out
+
+
+def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: RotaryAxes, inverse: bool = False,
+                q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """`q` (tokens, q_heads, head_dim) and `k` (tokens, kv_heads, head_dim; or None) turned by the angles of `positions` (axes, tokens),
+    in one launch: (q_out, k_out), new tensors unless given (`q_out=q`: in place). The angles are formed in 64 bits from whole
+    positions; the elements are turned in f32 and rounded once. `inverse=True` turns back: the gradient with respect to q and
+    k of a call's outputs' gradients."""
+    _need_cuda(q, "q")
+    q = _heads(q, "rotary: q")
+    tokens, hq, d = q.shape
+    if rotary.rot > d:
+        raise ValueError(f"rotary: {rotary.rot} turned elements, heads of {d}")
+    qo = _out_like(q, q_out, "rotary: q_out")
+    qs, qos = (q.stride(0), q.stride(1)), (qo.stride(0), qo.stride(1))
+    if k is not None:
+        k = _heads(k, "rotary: k", tokens, d)
+        if k.dtype != q.dtype or k.device != q.device:
+            raise ValueError(f"rotary: q is {q.dtype} on {q.device}, k is {k.dtype} on {k.device}")
+        ko = _out_like(k, k_out, "rotary: k_out")
+        kp, kop, ks, kos, hkv = k.data_ptr(), ko.data_ptr(), (k.stride(0), k.stride(1)), (ko.stride(0), ko.stride(1)), k.shape[1]
+    else:
+        ko, kp, kop, ks, kos, hkv = None, 0, 0, (0, 0), (0, 0), 0
+    fields, pos = rotary.fields(positions, tokens, q.device, inverse)
+    _call(A.lib().b200_rotary_axes, _ROTARY_ARGS.pack(q.data_ptr(), kp, qo.data_ptr(), kop, *qs, *ks, *qos, *kos, tokens, hq, hkv, d, _dtype_id(q), 0, *fields), q.device)
+    return qo, ko
+
+
+class PagedKvPool:
+    """Pages of keys and values: `num_blocks` pages of `block_size` rows of (kv_heads, head_dim). `format`: "bf16" / "f16" (elements as they
+    are), or "mxfp8": E4M3 codes with an E8M0 scale per 32 elements, the codes and scales of `TurboQuantizer`'s MXFP8 rows
+    (0.52 of the bytes of 16 bits) in planes of their own, `k` / `v` (num_blocks, block_size, kv_heads, head_dim) and `k_scale` / `v_scale`
+    (num_blocks, kv_heads, block_size, head_dim / 32)."""
+
+    def __init__(self, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, format: str = "bf16", device="cuda"):
+        kinds = {"bf16": torch.bfloat16, "f16": torch.float16, "mxfp8": _E4M3}
+        if format not in kinds:
+            raise ValueError(f"paged pool: format {format!r} (bf16, f16, mxfp8)")
+        if format == "mxfp8" and head_dim % 32:
+            raise ValueError(f"paged pool: MXFP8 needs head dims that are multiples of 32, got {head_dim}")
+        shape = (num_blocks, block_size, kv_heads, head_dim)
+        plane = lambda: torch.zeros(shape, dtype=torch.uint8 if format == "mxfp8" else kinds[format], device=device).view(kinds[format])
+        scale = lambda: torch.zeros((num_blocks, kv_heads, block_size, head_dim // 32), dtype=torch.uint8, device=device) if format == "mxfp8" else None
+        self._take(plane(), plane(), scale(), scale())
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        """A pool over a program's own tensors (views in other orders too, rows contiguous); nothing is copied."""
+        self = cls.__new__(cls)
+        self._take(k, v, k_scale, v_scale)
+        return self
+
+    def _take(self, k, v, ks, vs):
+        if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError(f"paged pool: k {tuple(k.shape)} {k.dtype} / v {tuple(v.shape)} {v.dtype} must be two (num_blocks, block_size, kv_heads, head_dim) tensors of one type")
+        if k.dtype not in _POOL_DTYPES:
+            raise ValueError(f"paged pool: {k.dtype} (bf16, f16, or float8_e4m3fn with scales)")
+        _need_cuda(k, "paged pool: k")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("paged pool: rows must be contiguous along the head dim")
+        n, rows, h, d = k.shape
+        if k.dtype == _E4M3:
+            for s, what in ((ks, "k_scale"), (vs, "v_scale")):
+                if s is None or tuple(s.shape) != (n, h, rows, d // 32) or s.element_size() != 1 or s.device != k.device or not s.is_contiguous() or d % 32:
+                    raise ValueError(f"paged pool: {what} must be a contiguous one-byte ({n}, {h}, {rows}, {d // 32}) tensor, and the head dim a multiple of 32")
+        elif ks is not None or vs is not None:
+            raise ValueError("paged pool: scales belong to float8_e4m3fn pages")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, ks, vs
+        self.num_blocks, self.block_size, self.kv_heads, self.head_dim = n, rows, h, d
+        self.device = k.device
+        self.dtype = _POOL_DTYPES[k.dtype]
+        self._packed = _POOL.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr() if ks is not None else 0, vs.data_ptr() if vs is not None else 0,
+                                  *k.stride()[:3], *v.stride()[:3], n, rows, h, d, self.dtype, 0)
+
+    def storage_bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rotary: Optional[RotaryAxes] = None, positions: Optional[torch.Tensor] = None,
+               q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+        """Writes `k` / `v` (tokens, kv_heads, head_dim; f32, f16 or bf16) to `slots` (tokens), in one launch. A negative slot's token
+        is not written; a slot past the pool is not either, and sets `status` (an int32 device tensor) to 3. With `rotary` and
+        `positions` (axes, tokens) the keys are turned first, and with `q` (tokens, q_heads, head_dim) the queries
+        beside them: returns them in `q_out` (a new tensor unless given; `q` itself: in place)."""
+        dev = self.device
+        k = _heads(k, "paged append: k", None, self.head_dim)
+        tokens = k.shape[0]
+        v = _heads(v, "paged append: v", tokens, self.head_dim)
+        if k.shape[1] != self.kv_heads or v.shape[1] != self.kv_heads or k.dtype != v.dtype or k.device != dev or v.device != dev:
+            raise ValueError(f"paged append: k {tuple(k.shape)} {k.dtype} / v {tuple(v.shape)} {v.dtype} do not match {self.kv_heads} kv heads on {dev}")
+        slots = _ints(slots, torch.int64, dev, "paged append: slots")
+        if slots.dim() != 1 or slots.shape[0] != tokens:
+            raise ValueError(f"paged append: {tokens} tokens need as many slots, got {tuple(slots.shape)}")
+        if (rotary is None) != (positions is None):
+            raise ValueError("paged append: rotary and positions come together")
+        fields, pos = rotary.fields(positions, tokens, dev, False) if rotary is not None else (_NO_ROTARY, None)
+        if rotary is not None and rotary.rot > self.head_dim:
+            raise ValueError(f"rotary: {rotary.rot} turned elements, heads of {self.head_dim}")
+        qo, qp, qop, qs, qos, hq = None, 0, 0, (0, 0), (0, 0), 0
+        if q is not None:
+            if rotary is None:
+                raise ValueError("paged append: queries are turned; without rotary there is nothing to do with them")
+            q = _heads(q, "paged append: q", tokens, self.head_dim)
+            if q.dtype != k.dtype or q.device != dev:
+                raise ValueError(f"paged append: q is {q.dtype} on {q.device}, k {k.dtype} on {dev}")
+            qo = _out_like(q, q_out, "paged append: q_out")
+            qp, qop, qs, qos, hq = q.data_ptr(), qo.data_ptr(), (q.stride(0), q.stride(1)), (qo.stride(0), qo.stride(1)), q.shape[1]
+        _call(A.lib().b200_paged_append, self._packed + _APPEND_ARGS.pack(
+            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), qp, qop, *qs, *qos, tokens, hq, _dtype_id(k), 0,
+            *fields, status.data_ptr() if status is not None else 0), dev)
+        return qo
+
+    def _table(self, table: torch.Tensor, b: int, what: str) -> torch.Tensor:
+        if table.dim() != 2 or table.shape[0] != b:
+            raise ValueError(f"{what}: block_table must have a row for each of {b} sequences, got {tuple(table.shape)}")
+        return _ints(table, torch.int32, self.device, f"{what}: block_table")
+
+    def keys_values(self, block_table: torch.Tensor, seqlens_k: torch.Tensor, total: int, dtype: Optional[torch.dtype] = None,
+                    status: Optional[torch.Tensor] = None):
+        """The rows of sequences, packed one behind the other: contiguous (total, kv_heads, head_dim) keys and values in `dtype` (the
+        pool's own, bf16 for MXFP8). `seqlens_k`: cumulative lengths (sequences + 1, on the device, as for the varlen calls); `total`:
+        their last (rows behind it are left as allocated). Page numbers outside the pool read as zeros and set `status` to 3."""
+        b = seqlens_k.numel() - 1
+        table = self._table(block_table, b, "paged keys_values")
+        cu = _ints(seqlens_k, torch.int32, self.device, "paged keys_values: seqlens_k")
+        dtype = dtype or (torch.bfloat16 if self.dtype == A.FP8 else self.k.dtype)
+        k = torch.empty((int(total), self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        _call(A.lib().b200_paged_unpack, self._packed + _UNPACK_ARGS.pack(
+            table.data_ptr(), table.stride(0), cu.data_ptr(), k.data_ptr(), v.data_ptr(), k.shape[0], b, table.shape[1], _dtype_id(k), 0,
+            status.data_ptr() if status is not None else 0), self.device)
+        return k, v

@@ -473,6 +473,90 @@ int b200_flash_attn_paged(const B200FaArgs *args, const B200Page *pages, uint32_
  * pointers and strides must describe the same tensors viewed as (b, hkv, t, d). */
 int b200_fa_prefill_append(const B200FaArgs *fa, const B200KvAppendArgs *append, b200_stream_t stream);
 
+/* ---- rotary positions with several axes ------------------------------------------------------------------------------- */
+/* The angles of a call: frequency f (of rot / 2) turns a pair of elements by pos[axis[f]][token] * freq[f]. The product is
+ * formed in 64 bits and reduced there, so positions of millions keep their angles; sines and cosines are f32. The pair is
+ * (f, f + rot / 2) of every head, or with `interleaved` (2 f, 2 f + 1); elements from rot on stay as they are. `inverse`
+ * turns the other way: the gradient of the call, or a cached key taken back to position 0. */
+typedef struct B200Rotary {
+    const float *freq;   /* device, rot / 2 */
+    const uint8_t *axis; /* device, rot / 2: the axis each frequency goes by; NULL: axis 0 */
+    const int64_t *pos;  /* device: the position of token t on axis a at pos[a * pos_stride + t] */
+    uint64_t pos_stride;
+    uint32_t n_axes, rot;
+    uint32_t interleaved, inverse;
+} B200Rotary;
+
+/* q (tokens, hq, d) and k (tokens, hkv, d) -> q_out, k_out, all of `dtype` with (token, head) element strides and contiguous
+ * head dim. In place allowed (the same pointers and strides); otherwise outputs must not overlap inputs. k = NULL (hkv = 0): only
+ * q. Head dims: multiples of 8 up to 256; rot: a multiple of 16 up to d. */
+typedef struct B200RotaryArgs {
+    const void *q, *k;
+    void *q_out, *k_out;
+    uint64_t q_strides[2], k_strides[2], q_out_strides[2], k_out_strides[2]; /* (token, head) in elements */
+    uint32_t tokens, hq, hkv, d;
+    int32_t dtype; /* B200_F32 / B200_F16 / B200_BF16 */
+    uint32_t pad;
+    B200Rotary rotary;
+} B200RotaryArgs;
+int b200_rotary_axes(const B200RotaryArgs *args, b200_stream_t stream);
+
+/* ---- a pool of cache pages ---------------------------------------------------------------------------------------------- */
+/* Keys and values of all sequences of a serving program: n_blocks pages of block_rows rows, (block, row, kv head, d) with
+ * (block, row, head) element strides and contiguous head dim, the layout of flash_attn_varlen_paged_windowed
+ * (candle-flash-attn/src/lib.rs:341-420). dtype B200_F16 / B200_BF16: elements as they are. B200_FP8: MXFP8, the codes and
+ * scales of b200_tq_quantize's rows in planes of their own: E4M3 codes, and one E8M0 byte per 32 elements of a row in
+ * k_scale / v_scale, (block, kv head, row, d / 32) contiguous (d a multiple of 32). All bases and row, head and block
+ * strides are multiples of 16 bytes. Head dims: multiples of 8 up to 256.
+ * A sequence's pages are a row of a block table: its key j is row j % block_rows of page table[j / block_rows]. Entries that no key
+ * needs are not read. An entry outside [0, n_blocks) that one needs holds zeros, and sets `status` (where the call has one) to 3. */
+typedef struct B200PagedPool {
+    void *k, *v;
+    uint8_t *k_scale, *v_scale;
+    uint64_t k_strides[3], v_strides[3]; /* (block, row, head) in elements */
+    uint32_t n_blocks, block_rows, hkv, d;
+    int32_t dtype;
+    uint32_t pad;
+} B200PagedPool;
+
+/* New tokens' keys and values into the pool, quantised as they are written where it holds MXFP8: token t goes to slot
+ * slots[t] = block * block_rows + row. A negative slot: the token is not written (padding); one past the pool: not written, and
+ * `status` becomes 3. Where two tokens name one slot, it holds pieces of either. With rotary.freq the keys are turned first (in f32, rounded once, to
+ * what the pool holds), and with q the queries beside them (q -> q_out, in place allowed), all in one launch. k, v (tokens,
+ * hkv, d) and q (tokens, hq, d) of src_dtype, (token, head) element strides. */
+typedef struct B200PagedAppendArgs {
+    B200PagedPool pool;
+    const void *k, *v;
+    uint64_t k_strides[2], v_strides[2];
+    const int64_t *slots; /* device, one per token */
+    const void *q;        /* NULL: no queries */
+    void *q_out;
+    uint64_t q_strides[2], q_out_strides[2];
+    uint32_t tokens, hq;
+    int32_t src_dtype;
+    uint32_t pad;
+    B200Rotary rotary; /* freq NULL: nothing is turned */
+    int32_t *status;   /* optional device word */
+} B200PagedAppendArgs;
+int b200_paged_append(const B200PagedAppendArgs *args, b200_stream_t stream);
+
+/* The way back: the keys and values of b sequences, packed one behind the other, as contiguous (total, hkv, d) tensors of `dtype`
+ * (f32, f16 or bf16; each value rounded once). Sequence i has the rows cu_k[i] .. cu_k[i + 1] - 1; rows of the outputs behind
+ * cu_k[b] are left as they were. v = NULL: only keys. Keys beyond table_cols pages read as zeros (status 3). */
+typedef struct B200PagedUnpackArgs {
+    B200PagedPool pool;
+    const int32_t *table; /* device, (b, table_cols) with row stride table_stride */
+    uint64_t table_stride;
+    const uint32_t *cu_k; /* device, b + 1 */
+    void *k, *v;
+    uint64_t total;
+    uint32_t b, table_cols;
+    int32_t dtype;
+    uint32_t pad;
+    int32_t *status;
+} B200PagedUnpackArgs;
+int b200_paged_unpack(const B200PagedUnpackArgs *args, b200_stream_t stream);
+
 /* Health check: 1 when a bounded device-side wait of the attention kernels (an mbarrier that a copy or
  * a tensor core commit should have completed, the flag of another rank in the gathered attention) has run out
  * on the current device since the library was loaded or the flag was last cleared, 0 otherwise, -1 when the

@@ -269,6 +269,91 @@ pub struct B200CopyEvent {
     _private: [u8; 0],
 }
 
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct B200Rotary {
+    pub freq: *const f32,
+    pub axis: *const u8,
+    pub pos: *const i64,
+    pub pos_stride: u64,
+    pub n_axes: u32,
+    pub rot: u32,
+    pub interleaved: u32,
+    pub inverse: u32,
+}
+
+#[repr(C)]
+pub struct B200RotaryArgs {
+    pub q: *const c_void,
+    pub k: *const c_void,
+    pub q_out: *mut c_void,
+    pub k_out: *mut c_void,
+    pub q_strides: [u64; 2],
+    pub k_strides: [u64; 2],
+    pub q_out_strides: [u64; 2],
+    pub k_out_strides: [u64; 2],
+    pub tokens: u32,
+    pub hq: u32,
+    pub hkv: u32,
+    pub d: u32,
+    pub dtype: i32,
+    pub pad: u32,
+    pub rotary: B200Rotary,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct B200PagedPool {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut u8,
+    pub v_scale: *mut u8,
+    pub k_strides: [u64; 3],
+    pub v_strides: [u64; 3],
+    pub n_blocks: u32,
+    pub block_rows: u32,
+    pub hkv: u32,
+    pub d: u32,
+    pub dtype: i32,
+    pub pad: u32,
+}
+
+#[repr(C)]
+pub struct B200PagedAppendArgs {
+    pub pool: B200PagedPool,
+    pub k: *const c_void,
+    pub v: *const c_void,
+    pub k_strides: [u64; 2],
+    pub v_strides: [u64; 2],
+    pub slots: *const i64,
+    pub q: *const c_void,
+    pub q_out: *mut c_void,
+    pub q_strides: [u64; 2],
+    pub q_out_strides: [u64; 2],
+    pub tokens: u32,
+    pub hq: u32,
+    pub src_dtype: i32,
+    pub pad: u32,
+    pub rotary: B200Rotary,
+    pub status: *mut i32,
+}
+
+#[repr(C)]
+pub struct B200PagedUnpackArgs {
+    pub pool: B200PagedPool,
+    pub table: *const i32,
+    pub table_stride: u64,
+    pub cu_k: *const u32,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub total: u64,
+    pub b: u32,
+    pub table_cols: u32,
+    pub dtype: i32,
+    pub pad: u32,
+    pub status: *mut i32,
+}
+
 #[link(name = "b200attn")]
 extern "C" {
     // host-side tables and plans (candle-core/src/accel/{formats,turbo,attention}.rs)
@@ -306,6 +391,11 @@ extern "C" {
     pub fn b200_flash_attn_paged_workspace_bytes(args: *const B200FaArgs, n_pages: u32) -> usize;
     pub fn b200_flash_attn_paged(args: *const B200FaArgs, pages: *const B200Page, n_pages: u32, stream: b200_stream_t) -> c_int;
     pub fn b200_fa_prefill_append(fa: *const B200FaArgs, append: *const B200KvAppendArgs, stream: b200_stream_t) -> c_int;
+
+    // a pool of cache pages: rotary positions, rows in and out
+    pub fn b200_rotary_axes(args: *const B200RotaryArgs, stream: b200_stream_t) -> c_int;
+    pub fn b200_paged_append(args: *const B200PagedAppendArgs, stream: b200_stream_t) -> c_int;
+    pub fn b200_paged_unpack(args: *const B200PagedUnpackArgs, stream: b200_stream_t) -> c_int;
 
     // health of the bounded device waits
     pub fn b200_device_wait_status() -> c_int;

@@ -142,6 +142,14 @@ class PagedUnpackArgs(C.Structure):
                 ("total", C.c_uint64), ("b", C.c_uint32), ("table_cols", C.c_uint32), ("dtype", C.c_int32), ("pad", C.c_uint32), ("status", C.c_void_p)]
 
 
+class PagedAttnArgs(C.Structure):
+    _fields_ = [("pool", PagedPool), ("q", C.c_void_p), ("out", C.c_void_p), ("q_strides", u64x2), ("out_strides", u64x2), ("cu_q", C.c_void_p),
+                ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_uint64), ("b", C.c_uint32), ("total_q", C.c_uint32), ("max_q", C.c_uint32),
+                ("max_k", C.c_uint32), ("hq", C.c_uint32), ("table_cols", C.c_uint32), ("q_dtype", C.c_int32), ("scale", C.c_float), ("softcap", C.c_float),
+                ("wl", C.c_int32), ("wr", C.c_int32), ("alibi", C.c_void_p), ("alibi_bstride", C.c_uint32), ("pad", C.c_uint32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("status", C.c_void_p)]
+
+
 # every symbol that include/b200attn.h declares
 SYMBOLS = [
     "b200_row_layout", "b200_codebook", "b200_hadamard_signs", "b200_qjl_matrix", "b200_row_group", "b200_split_count_grouped",
@@ -149,7 +157,7 @@ SYMBOLS = [
     "b200_describe", "b200_last_error", "b200_tq_rotate", "b200_tq_quantize", "b200_tq_dequantize", "b200_kv_append", "b200_kv_unpack",
     "b200_tq_attention_workspace_bytes", "b200_tq_attention", "b200_tq_attention_static", "b200_tq_attention_gather",
     "b200_flash_attn_workspace_bytes", "b200_flash_attn_paged_workspace_bytes", "b200_flash_attn_paged",
-    "b200_rotary_axes", "b200_paged_append", "b200_paged_unpack",
+    "b200_rotary_axes", "b200_paged_append", "b200_paged_unpack", "b200_paged_attention_workspace_bytes", "b200_paged_attention",
     "b200_flash_attn", "b200_fa_prefill_append", "b200_device_wait_status", "b200_device_wait_check",
     "b200_pinned_alloc", "b200_pinned_free", "b200_pinned_len", "b200_pinned_wait_idle", "b200_pinned_ptr",
     "b200_copy_upload", "b200_copy_download", "b200_copy_event_wait_on_compute", "b200_copy_event_synchronize",
@@ -205,6 +213,9 @@ def lib():
         l.b200_rotary_axes.argtypes = [C.c_void_p, C.c_void_p]  # the arguments' bytes, or a structure by reference
         l.b200_paged_append.argtypes = [C.c_void_p, C.c_void_p]
         l.b200_paged_unpack.argtypes = [C.c_void_p, C.c_void_p]
+        l.b200_paged_attention_workspace_bytes.argtypes = [C.c_void_p]
+        l.b200_paged_attention_workspace_bytes.restype = C.c_size_t
+        l.b200_paged_attention.argtypes = [C.c_void_p, C.c_void_p]
         l.b200_device_wait_check.argtypes = [C.c_int]
         l.b200_pinned_alloc.argtypes = [C.c_size_t, C.POINTER(C.c_void_p)]
         l.b200_pinned_free.argtypes = [C.c_void_p]

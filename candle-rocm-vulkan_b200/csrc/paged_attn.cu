@@ -1,0 +1,788 @@
+// Attention of a ragged batch's new tokens over a pool of cache pages: b200_paged_attention, and its kernel for sequences with few
+// new tokens. Per query head, o_t = sum_j w_tj v_j / sum_j w_tj with w_tj = exp(scale q_t . k_j (soft cap, ALiBi)) over the keys j that
+// token t sees, in one pass with a running maximum and sum.
+//
+// Sequences with few packed query rows (token x head of the group) are bound by memory: every key and value is read once for at
+// most 16 rows. The batch is ragged and only the device knows its lengths, so the work is divided there: a column is 16 rows of
+// one kv head, a unit is what a block's four warps score at a time (64 or 128 keys), and the units of all columns, one behind the other,
+// are cut into equal shares, one per block (two blocks per SM). A block that holds all of a column writes its rows; parts of
+// columns go to the workspace, two at most per block (where its share begins and where it ends), and a second grid joins
+// them: it has a block per border between shares, and the first border inside a column belongs to that column.
+// In a block each warp has keys of its own, K and V in a ring of stages that it fills ahead of the column it is working on,
+// across columns too; scores and sums run on mma.sync m16n8k16, and the warps' partial results meet in shared memory at a
+// column's end.
+//
+// MXFP8 keys and values stay codes up to the registers. Scores: the codes are exact in f16; q is taken to f16 behind a power of
+// two per row (a bf16 element keeps its eight bits unless it is 2^28 below the row's largest), and a block of 32 elements adds its
+// sum times its scale in f32. Values: the codes times their power of two in q's type, which holds the product exactly unless it leaves
+// that type's range; weights are rounded to q's type, as for 16-bit pools (2^-9 or 2^-12 each, and they average out).
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace b200 {
+
+constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32, PA_ROWS = 16;
+constexpr float PA_LOG2E = 1.4426950408889634f;
+
+struct PaParams {
+    const char *q;
+    char *out;
+    uint64_t q_st, q_sh, o_st, o_sh;  // bytes
+    const uint32_t *cu_q;
+    const int32_t *kv_len, *table;
+    uint64_t table_stride;
+    PoolParams pool;
+    const float *alibi;
+    int32_t *status;
+    float *part_o;    // [2 x blocks][16][d]
+    float2 *part_ml;  // [2 x blocks][16]: maximum (log 2), sum
+    uint32_t b, hq, hkv, group, d, total_q, max_q, max_k, table_cols, alibi_bs;
+    float scale, softcap;
+    int32_t wl, wr;
+    uint32_t blocks, min_units;
+};
+
+// KIND: 0 f16, 1 bf16, 2 MXFP8 under f16 queries, 3 MXFP8 under bf16 queries
+template <int HD, int KIND>
+struct PA {
+    static constexpr bool MX = KIND >= 2, BF16 = KIND & 1;
+    static constexpr int ES = MX ? 1 : 2, RB = HD * ES;                   // bytes of a row
+    static constexpr int KEYS = HD == 64 || (HD == 128 && MX) ? 32 : 16;  // of a warp's tile
+    static constexpr int UNIT = KEYS * PA_WARPS, CPR = RB / 16, NB = HD / 32;
+    static constexpr uint32_t TILE = KEYS * RB, STAGE = 2 * TILE;        // K, V
+    static constexpr uint32_t SC = MX ? 2 * KEYS * NB : 0;               // scales of a stage
+    static constexpr int NS = HD == 256 && !MX ? 2 : 3;
+    static constexpr int MROW = HD / 2 + 2;                              // floats per row of the merge: half a row, maximum, sum
+    static constexpr uint32_t SM_SC = PA_WARPS * NS * STAGE, SM_MERGE = SM_SC + PA_WARPS * NS * SC, SMEM = SM_MERGE + PA_WARPS * PA_ROWS * MROW * 4;
+    // 16-byte chunk ch of row r of a tile, in 128-byte columns (64 where a row is no longer), swizzled
+    __device__ static __forceinline__ uint32_t at(int r, int ch) {
+        if (RB == 64) return r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
+        return (ch >> 3) * (KEYS * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+    }
+};
+
+struct PaSeq {
+    uint32_t q0, rows, packs;  // first token; packed rows; groups of 16 of them
+    int lq, lk, ulo, uhi;      // units that some row sees
+};
+// keys [lo, hi) that packed row r sees
+__device__ __forceinline__ void pa_range(const PaParams &p, const PaSeq &s, uint32_t r, int &lo, int &hi) {
+    const int pos = (int)(r / p.group) + s.lk - s.lq;
+    lo = p.wl >= 0 && pos > p.wl ? min(pos - p.wl, s.lk) : 0;
+    hi = p.wr >= 0 && pos < s.lk - p.wr - 1 ? pos + p.wr + 1 : s.lk;
+    hi = max(hi, lo);
+}
+// the sequence's units
+__device__ __forceinline__ uint64_t pa_seq(const PaParams &p, uint32_t b, int unit, PaSeq &s) {
+    s.q0 = min(p.cu_q[b], p.total_q);
+    const uint32_t end = min(p.cu_q[b + 1], p.total_q);
+    s.lq = end > s.q0 ? (int)min(end - s.q0, p.max_q) : 0;
+    s.lk = max(0, min(p.kv_len[b], (int)p.max_k));
+    s.rows = (uint32_t)s.lq * p.group;
+    s.packs = (s.rows + PA_ROWS - 1) / PA_ROWS;
+    s.ulo = s.uhi = 0;
+    if (s.rows == 0) return 0;
+    int lo, hi, x;
+    pa_range(p, s, 0, lo, x);
+    pa_range(p, s, s.rows - 1, x, hi);
+    s.ulo = lo / unit;
+    s.uhi = hi > lo ? (hi + unit - 1) / unit : s.ulo + 1;  // rows that see nothing still have zeros to write
+    return (uint64_t)(uint32_t)(s.uhi - s.ulo) * s.packs * p.hkv;
+}
+
+// Where the block (all of its threads; a multiple of 32, 256 at most) finds unit `target(total)` of all: the sequence and the unit
+// within it. Every thread sums a run of sequences. `scratch`: ten words of shared memory.
+struct PaPlace {
+    uint64_t total, per, off;
+    uint32_t seq;
+};
+template <typename F>
+__device__ __forceinline__ PaPlace pa_place(const PaParams &p, int unit, uint64_t *scratch, F target) {
+    uint64_t *const s_sum = scratch, *const s_at = scratch + 8;
+    const uint32_t n = (p.b + blockDim.x - 1) / blockDim.x, first = min(threadIdx.x * n, p.b), last = min(first + n, p.b);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    uint64_t sum = 0;
+    PaSeq s;
+    for (uint32_t i = first; i < last; ++i) sum += pa_seq(p, i, unit, s);
+    uint64_t upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_sum[warp] = upto;
+    __syncthreads();
+    PaPlace at;
+    at.total = 0;
+    uint64_t before = upto - sum;
+    for (int w = 0; w < warps; ++w) {
+        if (w < warp) before += s_sum[w];
+        at.total += s_sum[w];
+    }
+    at.per = max((at.total + p.blocks - 1) / p.blocks, (uint64_t)p.min_units);
+    const uint64_t want = target(at.per);
+    if (want >= before && want < before + sum) {
+        uint64_t rest = want - before;
+        for (uint32_t i = first; i < last; ++i) {
+            const uint64_t u = pa_seq(p, i, unit, s);
+            if (rest < u) {
+                s_at[0] = i;
+                s_at[1] = rest;
+                break;
+            }
+            rest -= u;
+        }
+    }
+    __syncthreads();
+    at.seq = (uint32_t)s_at[0];
+    at.off = s_at[1];
+    return at;
+}
+
+// a unit of a column of a sequence, and the way to the next one
+struct PaCursor {
+    PaSeq s;
+    uint32_t seq, col;  // col = head x packs + pack
+    int u;
+    __device__ __forceinline__ void start(const PaParams &p, int unit, uint32_t seq_, uint64_t off) {
+        seq = seq_;
+        pa_seq(p, seq, unit, s);
+        const uint32_t n = (uint32_t)(s.uhi - s.ulo);
+        col = (uint32_t)(off / n);
+        u = s.ulo + (int)(off - (uint64_t)col * n);
+    }
+    __device__ __forceinline__ void next(const PaParams &p, int unit) {
+        if (++u < s.uhi) return;
+        if (++col == s.packs * p.hkv) {
+            col = 0;
+            while (++seq < p.b && pa_seq(p, seq, unit, s) == 0) {}
+        }
+        u = s.ulo;
+    }
+};
+
+__device__ __forceinline__ void pa_ldsm(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+__device__ __forceinline__ void pa_ldsm_trans(uint32_t addr, uint32_t &r0, uint32_t &r1, uint32_t &r2, uint32_t &r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+__device__ __forceinline__ uint2 pa_lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t pa_lds8(uint32_t addr) {
+    uint32_t v;
+    asm volatile("{\n .reg .u16 t;\n ld.shared.u8 t, [%1];\n cvt.u32.u16 %0, t;\n}" : "=r"(v) : "r"(addr));
+    return v;
+}
+template <bool BF16>
+__device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        mma_f16_16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pa_pack2(float lo, float hi) {
+    uint32_t d;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pa_mul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// the E4M3 codes of byte i of two words as a pair of values: f16, or bf16 times 2^-120 (a code's exponent and mantissa in the places
+// of a bf16's, its subnormals among that type's)
+template <bool BF16, int I>
+__device__ __forceinline__ uint32_t pa_codes(uint32_t lo, uint32_t hi) {
+    if (BF16) {
+        const uint32_t t = __byte_perm(lo, hi, (4u + I) << 12 | I << 4);
+        return (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+    }
+    return cvt_e4m3x2_f16x2(__byte_perm(lo, hi, (4u + I) << 4 | I));
+}
+// The multiplier that takes such a pair to its values, for the scales e0 and e1: f16 2^(e - 127), bf16 2^(e - 127 + 120). Scales outside the
+// type's range (f16 e < 103, bf16 e > 134) go in two steps: `rest` is the second.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pa_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
+    if (BF16) {
+        const uint32_t m0 = min(e0, 134u), m1 = min(e1, 134u);
+        rest = (e0 - m0 + 127u) << 7 | (e1 - m1 + 127u) << 23;
+        return (m0 + 120u) << 7 | (m1 + 120u) << 23;
+    }
+    const uint32_t m0 = max(e0, 103u), m1 = max(e1, 103u);
+    rest = pack_f16x2(e8m0_to_f(e0 + 127u - m0), e8m0_to_f(e1 + 127u - m1));
+    return pack_f16x2(e8m0_to_f(m0), e8m0_to_f(m1));
+}
+
+template <int HD, int KIND>
+__global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_kernel(const PaParams p) {
+    using C = PA<HD, KIND>;
+    constexpr bool MX = C::MX, BF16 = C::BF16;
+    constexpr int KSTEPS = HD / 16, NT = HD / 8, KEYS = C::KEYS, KG = KEYS / 16, UNIT = C::UNIT;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const uint32_t ring = smem_u32(smem) + warp * C::NS * C::STAGE, scales = smem_u32(smem) + C::SM_SC + warp * C::NS * C::SC;
+    float *const mg = reinterpret_cast<float *>(smem + C::SM_MERGE);
+    if (p.blocks > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining grid may get ready
+    const PoolParams &pl = p.pool;
+
+    const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return blockIdx.x * per; });
+    const uint64_t u0 = blockIdx.x * place.per;
+    if (u0 >= place.total) return;
+    const int nu = (int)min(place.per, place.total - u0);
+    PaCursor cur, lead;  // the unit being worked on, and the one to be asked for next
+    cur.start(p, UNIT, place.seq, place.off);
+    lead = cur;
+
+    // A warp's keys of the lead's unit into stage st: lane i finds key i's row, then C::CPR lanes copy a row. What no row of the column
+    // sees, and what a page outside the pool would hold, is zeros.
+    auto request = [&](int st) {
+        const uint32_t hk = lead.col / lead.s.packs, pack = lead.col - hk * lead.s.packs, r0 = pack * PA_ROWS;
+        int lo, hi, x;
+        pa_range(p, lead.s, r0, lo, x);
+        pa_range(p, lead.s, min(r0 + PA_ROWS, lead.s.rows) - 1, x, hi);
+        const int j = lead.u * UNIT + warp * KEYS + lane;
+        const char *kr = nullptr, *vr = nullptr;
+        uint64_t srow = 0;
+        if (lane < KEYS && j >= lo && j < hi) {
+            const uint32_t page = pool_div((uint32_t)j, pl.div_mul, pl.div_shr), row = (uint32_t)j - page * pl.block_rows;
+            const int id = page < p.table_cols ? p.table[lead.seq * p.table_stride + page] : -1;
+            if (id >= 0 && (uint32_t)id < pl.n_blocks) {
+                kr = pl.k + (uint64_t)id * pl.k_sb + row * pl.k_sr + hk * pl.k_sh;
+                vr = pl.v + (uint64_t)id * pl.v_sb + row * pl.v_sr + hk * pl.v_sh;
+                srow = (((uint64_t)id * pl.hkv + hk) * pl.block_rows + row) * (p.d / 32);
+            } else if (p.status) {
+                atomicExch(p.status, 3);
+            }
+        }
+        const uint32_t dst = ring + st * C::STAGE, ch = lane % C::CPR;
+#pragma unroll
+        for (int i = 0; i < KEYS * C::CPR / 32; ++i) {
+            const int row = i * (32 / C::CPR) + lane / C::CPR;
+            const char *ks = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(kr), row));
+            const char *vs = reinterpret_cast<const char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vr), row));
+            const bool in = ks != nullptr && ch * 16 < p.d * C::ES;
+            const uint32_t at = dst + C::at(row, ch);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(in ? ks + ch * 16 : pl.k), "r"(in ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + C::TILE), "l"(in ? vs + ch * 16 : pl.v), "r"(in ? 16 : 0) : "memory");
+        }
+        if (MX && lane < KEYS) {
+            const uint32_t nb = p.d / 32, at = scales + st * C::SC + lane * C::NB;
+#pragma unroll
+            for (int i = 0; i < C::NB; ++i) {
+                const bool in = kr != nullptr && (uint32_t)i < nb;
+                const uint32_t ke = in ? pl.ks[srow + i] : 127u, ve = in ? pl.vs[srow + i] : 127u;
+                asm volatile("st.shared.u8 [%0], %1;" ::"r"(at + i), "r"(ke) : "memory");
+                asm volatile("st.shared.u8 [%0], %1;" ::"r"(at + KEYS * C::NB + i), "r"(ve) : "memory");
+            }
+        }
+    };
+    for (int t = 0; t < C::NS; ++t) {
+        if (t < nu) {
+            request(t);
+            lead.next(p, UNIT);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    uint32_t qa[KSTEPS][4];
+    float m[2], l[2], oacc[NT][4], sc[2], slope[2];
+    int r_lo[2], r_hi[2], r_pos[2], lomax = 0, himin = 0;
+    const bool plain = p.softcap <= 0.0f && p.alibi == nullptr;
+    bool begin = true;
+    int seg_u = 0;
+    uint32_t seg = 0;  // the block's segments so far
+    for (int t = 0; t < nu; ++t) {
+        const uint32_t hk = cur.col / cur.s.packs, pack = cur.col - hk * cur.s.packs, row0 = pack * PA_ROWS;
+        if (begin) {
+            // ---- a column: its rows of q as A fragments, their keys and scales
+            begin = false;
+            seg_u = cur.u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t r = row0 + g + 8 * e;
+                m[e] = -INFINITY, l[e] = 0.0f, slope[e] = 0.0f, sc[e] = p.scale;
+                r_lo[e] = 0, r_hi[e] = cur.s.lk, r_pos[e] = 0;  // rows that do not exist see every key and are never stored
+                const bool there = r < cur.s.rows;
+                const uint32_t tok = there ? r / p.group : 0, h = hk * p.group + (there ? r - tok * p.group : 0);
+                const char *src = p.q + (cur.s.q0 + tok) * p.q_st + h * p.q_sh;
+                if (there) {
+                    pa_range(p, cur.s, r, r_lo[e], r_hi[e]);
+                    r_pos[e] = (int)tok + cur.s.lk - cur.s.lq;
+                    if (p.alibi) slope[e] = p.alibi[(size_t)cur.seq * p.alibi_bs + h];
+                }
+                if (!MX) {
+#pragma unroll
+                    for (int ks = 0; ks < KSTEPS; ++ks) {
+                        const uint32_t at = ks * 16 + 2 * c;
+                        qa[ks][e] = there && at < p.d ? *reinterpret_cast<const uint32_t *>(src + at * 2) : 0u;
+                        qa[ks][2 + e] = there && at + 8 < p.d ? *reinterpret_cast<const uint32_t *>(src + (at + 8) * 2) : 0u;
+                    }
+                } else {
+                    // a block of 32 elements is two steps: lane c has its elements 8 c .. 8 c + 7, four a step
+                    uint4 w[C::NB];
+                    float top = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < C::NB; ++i) {
+                        const uint32_t at = i * 32 + 8 * c;
+                        w[i] = there && at < p.d ? *reinterpret_cast<const uint4 *>(src + at * 2) : make_uint4(0u, 0u, 0u, 0u);
+                        if (BF16) {
+                            const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(u2f(a[k] << 16)), fabsf(u2f(a[k] & 0xffff0000u))));
+                        }
+                    }
+                    float f = 1.0f;
+                    if (BF16) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const int ex = (int)((f2u(top) >> 23) & 0xffu);  // the row's largest lands in [2^14, 2^15)
+                        const int fe = min(max(127 + 14 + 127 - ex, 27), 227);
+                        f = u2f((uint32_t)fe << 23);
+                        sc[e] = p.scale * u2f((uint32_t)(254 - fe) << 23);
+                    }
+#pragma unroll
+                    for (int i = 0; i < C::NB; ++i) {
+                        uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                        if (BF16)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) a[k] = pack_f16x2(u2f(a[k] << 16) * f, u2f(a[k] & 0xffff0000u) * f);
+                        qa[2 * i][e] = a[0], qa[2 * i][2 + e] = a[1], qa[2 * i + 1][e] = a[2], qa[2 * i + 1][2 + e] = a[3];
+                    }
+                }
+            }
+            int x;
+            pa_range(p, cur.s, min(row0 + PA_ROWS, cur.s.rows) - 1, lomax, x);
+            pa_range(p, cur.s, row0, x, himin);
+        }
+        const int j0 = cur.u * UNIT + warp * KEYS, st = t % C::NS;
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::NS - 1) : "memory");
+        __syncwarp();
+        const uint32_t tk = ring + st * C::STAGE, tv = tk + C::TILE, tsc = scales + st * C::SC;
+
+        // ---- scores
+        float s[2 * KG][4];
+#pragma unroll
+        for (int n = 0; n < 2 * KG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        if (!MX) {
+            const uint32_t kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+                for (int np = 0; np < KG; ++np) {
+                    uint32_t b0, b1, b2, b3;
+                    pa_ldsm(tk + C::at(np * 16 + kr, ks * 2 + kc), b0, b1, b2, b3);
+                    pa_mma<BF16>(s[2 * np], qa[ks], b0, b1);
+                    pa_mma<BF16>(s[2 * np + 1], qa[ks], b2, b3);
+                }
+        } else {
+            const uint32_t nb = p.d / 32;
+#pragma unroll
+            for (int n = 0; n < 2 * KG; ++n)
+#pragma unroll
+                for (int i = 0; i < C::NB; ++i) {
+                    if ((uint32_t)i >= nb) break;
+                    const uint2 w = pa_lds64(tk + C::at(8 * n + g, 2 * i + (c >> 1)) + (c & 1) * 8);
+                    float z[4];
+                    const uint32_t(&q0)[4] = qa[2 * i], (&q1)[4] = qa[2 * i + 1];
+                    mma_f16_16816_z(z, q0[0], q0[1], q0[2], q0[3], cvt_e4m3x2_f16x2(w.x), cvt_e4m3x2_hi_f16x2(w.x));
+                    mma_f16_16816(z, q1[0], q1[1], q1[2], q1[3], cvt_e4m3x2_f16x2(w.y), cvt_e4m3x2_hi_f16x2(w.y));
+                    const float s0 = e8m0_to_f(pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i)), s1 = e8m0_to_f(pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i));
+                    s[n][0] = fmaf(z[0], s0, s[n][0]);
+                    s[n][1] = fmaf(z[1], s1, s[n][1]);
+                    s[n][2] = fmaf(z[2], s0, s[n][2]);
+                    s[n][3] = fmaf(z[3], s1, s[n][3]);
+                }
+        }
+        const bool full = plain && j0 >= lomax && j0 + KEYS <= himin;
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2 * KG; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = i >> 1;
+                float x = s[n][i] * (sc[e] * PA_LOG2E);
+                if (!full) {
+                    const int j = j0 + 8 * n + 2 * c + (i & 1);
+                    if (!plain) {
+                        x = s[n][i] * sc[e];
+                        if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
+                        if (slope[e] != 0.0f) x -= slope[e] * fabsf((float)(r_pos[e] - j));
+                        x *= PA_LOG2E;
+                    }
+                    if (!(j >= r_lo[e] && j < r_hi[e])) x = -INFINITY;
+                }
+                s[n][i] = x;
+                mx[e] = fmaxf(mx[e], x);
+            }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float mn = fmaxf(m[e], mx[e]), f = m[e] == -INFINITY ? 0.0f : fast_exp2(m[e] - mn);
+                m[e] = mn;
+                l[e] *= f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) oacc[n][2 * e] *= f, oacc[n][2 * e + 1] *= f;
+            }
+        }
+        const float ms0 = m[0] == -INFINITY ? 0.0f : m[0], ms1 = m[1] == -INFINITY ? 0.0f : m[1];
+        uint32_t pa[KG][4];
+#pragma unroll
+        for (int n = 0; n < 2 * KG; ++n) {
+            const float p0 = fast_exp2(s[n][0] - ms0), p1 = fast_exp2(s[n][1] - ms0), p2 = fast_exp2(s[n][2] - ms1), p3 = fast_exp2(s[n][3] - ms1);
+            l[0] += p0 + p1;
+            l[1] += p2 + p3;
+            pa[n >> 1][(n & 1) * 2] = pa_pack2<BF16>(p0, p1);
+            pa[n >> 1][(n & 1) * 2 + 1] = pa_pack2<BF16>(p2, p3);
+        }
+        // ---- O += P V
+        if (!MX) {
+            const uint32_t vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = lane >> 4;
+#pragma unroll
+            for (int kk = 0; kk < KG; ++kk)
+#pragma unroll
+                for (int np = 0; np < NT / 2; ++np) {
+                    uint32_t b0, b1, b2, b3;
+                    pa_ldsm_trans(tv + C::at(kk * 16 + vr, np * 2 + vc), b0, b1, b2, b3);
+                    pa_mma<BF16>(oacc[2 * np], pa[kk], b0, b1);
+                    pa_mma<BF16>(oacc[2 * np + 1], pa[kk], b2, b3);
+                }
+        } else {
+            // column n = g of the products' tile i is element g HD / 8 + i: a lane reads the same bytes of its four keys
+            constexpr int W = HD / 32;  // words of a lane's elements
+            const uint32_t blk = g * (HD / 8) / 32, vsc = tsc + KEYS * C::NB + blk;
+#pragma unroll
+            for (int kk = 0; kk < KG; ++kk) {
+                uint32_t e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = pa_lds8(vsc + (kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8) * C::NB);
+                uint32_t rest0, rest1;
+                const uint32_t f0 = pa_scale2<BF16>(e[0], e[1], rest0), f1 = pa_scale2<BF16>(e[2], e[3], rest1);
+                const uint32_t top = max(max(e[0], e[1]), max(e[2], e[3])), low = min(min(e[0], e[1]), min(e[2], e[3]));
+                const bool far = __any_sync(0xffffffffu, BF16 ? top > 134u : low < 103u);
+#pragma unroll
+                for (int i = 0; i < W; i += 2) {
+                    uint32_t w[4][2];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint2 v = pa_lds64(tv + C::at(kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8, (g * W + i) >> 2) + ((g * W + i) & 3) * 4);
+                        w[k][0] = v.x, w[k][1] = v.y;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t b0[4] = {pa_codes<BF16, 0>(w[0][x], w[1][x]), pa_codes<BF16, 1>(w[0][x], w[1][x]), pa_codes<BF16, 2>(w[0][x], w[1][x]),
+                                          pa_codes<BF16, 3>(w[0][x], w[1][x])};
+                        uint32_t b1[4] = {pa_codes<BF16, 0>(w[2][x], w[3][x]), pa_codes<BF16, 1>(w[2][x], w[3][x]), pa_codes<BF16, 2>(w[2][x], w[3][x]),
+                                          pa_codes<BF16, 3>(w[2][x], w[3][x])};
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            b0[y] = pa_mul2<BF16>(b0[y], f0);
+                            b1[y] = pa_mul2<BF16>(b1[y], f1);
+                            if (far) b0[y] = pa_mul2<BF16>(b0[y], rest0), b1[y] = pa_mul2<BF16>(b1[y], rest1);
+                            pa_mma<BF16>(oacc[(i + x) * 4 + y], pa[kk], b0[y], b1[y]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();  // the stage has been read
+        if (t + C::NS < nu) {
+            request(st);
+            lead.next(p, UNIT);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+
+        // ---- the end of the column, or of the block's share
+        const PaCursor done = cur;
+        cur.next(p, UNIT);
+        begin = t + 1 == nu || cur.col != done.col || cur.seq != done.seq;
+        if (!begin) continue;
+        const bool whole = seg_u == done.s.ulo && done.u == done.s.uhi - 1;
+        const uint64_t slot = 2ull * blockIdx.x + (seg ? 1 : 0);
+        ++seg;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        }
+        const int row = tid >> 3, ch = tid & 7;
+        const uint32_t r = row0 + row, tok = r / p.group;
+        const bool there = r < done.s.rows;
+        char *const orow = p.out + (done.s.q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
+        // half of the elements at a time: the warps' sums (and their maxima and weights), then eight threads per row
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float *dst = mg + (warp * PA_ROWS + g + 8 * e) * C::MROW;
+#pragma unroll
+                for (int n = 0; n < NT / 2; ++n) {
+                    const float x0 = oacc[hf * (NT / 2) + n][2 * e], x1 = oacc[hf * (NT / 2) + n][2 * e + 1];
+                    if (MX) dst[2 * c * (NT / 2) + n] = x0, dst[(2 * c + 1) * (NT / 2) + n] = x1;
+                    else *reinterpret_cast<float2 *>(dst + 8 * n + 2 * c) = make_float2(x0, x1);
+                }
+                if (c == 0) dst[HD / 2] = m[e], dst[HD / 2 + 1] = l[e];
+            }
+            __syncthreads();
+            if (!there) continue;
+            float f[PA_WARPS], M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, mg[(w * PA_ROWS + row) * C::MROW + HD / 2]);
+            const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) {
+                f[w] = fast_exp2(mg[(w * PA_ROWS + row) * C::MROW + HD / 2] - ms);
+                L += f[w] * mg[(w * PA_ROWS + row) * C::MROW + HD / 2 + 1];
+            }
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll 4
+            for (int x = 2 * ch; x < HD / 2; x += 16) {
+                // the elements that stand at x: MX has HD / 16 neighbours of every group of HD / 8
+                const uint32_t dd = MX ? (x / (HD / 16)) * (HD / 8) + hf * (HD / 16) + x % (HD / 16) : hf * (HD / 2) + x;
+                if (dd >= p.d) continue;
+                float o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const float2 v = *reinterpret_cast<const float2 *>(mg + (w * PA_ROWS + row) * C::MROW + x);
+                    o0 = fmaf(f[w], v.x, o0);
+                    o1 = fmaf(f[w], v.y, o1);
+                }
+                if (whole) *reinterpret_cast<uint32_t *>(orow + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
+                else *reinterpret_cast<float2 *>(p.part_o + (slot * PA_ROWS + row) * p.d + dd) = make_float2(o0, o1);
+            }
+            if (!whole && hf == 0 && ch == 0) p.part_ml[slot * PA_ROWS + row] = make_float2(M, L);
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Joins the parts of columns that lie in several shares. Block i stands at the border in front of share i + 1; the first border inside a
+// column is the one that joins it. Its eight warps take rows and parts; a row's parts meet in shared memory.
+template <bool BF16>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const int unit) {
+    __shared__ float s_o[8][256];
+    __shared__ float s_l[8], s_m[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ uint64_t s_place[10];
+    uint64_t border = 0;
+    const PaPlace place = pa_place(p, unit, s_place, [&](uint64_t per) { return border = (blockIdx.x + 1) * per; });
+    PaCursor at;
+    uint64_t first = border, last = border;
+    if (border < place.total) {
+        at.start(p, unit, place.seq, place.off);
+        first = border - (uint64_t)(at.u - at.s.ulo), last = first + (uint64_t)(at.s.uhi - at.s.ulo) - 1;
+    }
+    if (first == border || blockIdx.x * place.per > first) {  // behind the last unit, between two columns, or not the column's first
+        if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid does not end before the one it follows
+        return;
+    }
+    const uint32_t b0 = blockIdx.x, parts = (uint32_t)(last / place.per) - b0 + 1;
+    const uint32_t hk = at.col / at.s.packs, row0 = (at.col - hk * at.s.packs) * PA_ROWS, rows = min((uint32_t)PA_ROWS, at.s.rows - row0);
+    // warps per row, a power of two
+    const uint32_t per_row = rows > 4 ? 1 : (rows > 2 ? 2 : (rows > 1 ? 4 : 8)), step = 8 / per_row;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t base = 0; base < rows; base += step) {
+        const uint32_t row = base + warp / per_row, sub = warp % per_row;
+        float M = -INFINITY, L = 0.0f, o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+        if (row < rows)
+            for (uint32_t k0 = sub; k0 < parts; k0 += 4 * per_row) {
+                float2 ml[4];
+                float4 v[4][2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t part = k0 + k * per_row;
+                    // a share's first segment is in its first slot; the column's first part is that only where column and share begin alike
+                    const uint64_t slot = 2ull * (b0 + part) + (part == 0 && first != b0 * place.per ? 1 : 0);
+                    const bool in = part < parts;
+                    ml[k] = in ? p.part_ml[slot * PA_ROWS + row] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint32_t d0 = hf * 128 + 4 * lane;
+                        v[k][hf] = in && d0 < p.d ? *reinterpret_cast<const float4 *>(p.part_o + (slot * PA_ROWS + row) * p.d + d0) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+                }
+                const float mn = fmaxf(fmaxf(fmaxf(M, ml[0].x), fmaxf(ml[1].x, ml[2].x)), ml[3].x), ms = mn == -INFINITY ? 0.0f : mn;
+                const float f = fast_exp2(M - ms);
+                M = mn;
+                L *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float w = fast_exp2(ml[k].x - ms);
+                    L = fmaf(w, ml[k].y, L);
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        o[4 * hf] = fmaf(w, v[k][hf].x, o[4 * hf]);
+                        o[4 * hf + 1] = fmaf(w, v[k][hf].y, o[4 * hf + 1]);
+                        o[4 * hf + 2] = fmaf(w, v[k][hf].z, o[4 * hf + 2]);
+                        o[4 * hf + 3] = fmaf(w, v[k][hf].w, o[4 * hf + 3]);
+                    }
+                }
+            }
+        if (per_row > 1) {
+            if (lane == 0) s_m[warp] = M, s_l[warp] = L;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) *reinterpret_cast<float4 *>(&s_o[warp][hf * 128 + 4 * lane]) = make_float4(o[4 * hf], o[4 * hf + 1], o[4 * hf + 2], o[4 * hf + 3]);
+            __syncthreads();
+            if (sub == 0 && row < rows) {
+                float mn = M;
+                for (uint32_t w = 1; w < per_row; ++w) mn = fmaxf(mn, s_m[warp + w]);
+                const float ms = mn == -INFINITY ? 0.0f : mn, f = fast_exp2(M - ms);
+                L *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= f;
+                for (uint32_t w = 1; w < per_row; ++w) {
+                    const float g = fast_exp2(s_m[warp + w] - ms);
+                    L = fmaf(g, s_l[warp + w], L);
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[4 * hf + i] = fmaf(g, s_o[warp + w][hf * 128 + 4 * lane + i], o[4 * hf + i]);
+                }
+            }
+            __syncthreads();
+        }
+        if (sub == 0 && row < rows) {
+            const uint32_t r = row0 + row, tok = r / p.group;
+            char *const orow = p.out + (at.s.q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const uint32_t d0 = hf * 128 + 4 * lane;
+                if (d0 < p.d)
+                    *reinterpret_cast<uint2 *>(orow + d0 * 2) = make_uint2(pa_pack2<BF16>(o[4 * hf] * inv, o[4 * hf + 1] * inv), pa_pack2<BF16>(o[4 * hf + 2] * inv, o[4 * hf + 3] * inv));
+            }
+        }
+    }
+}
+
+struct PaPlan {
+    PaParams p;
+    int hd, kind, unit;
+    size_t ws_bytes, off_ml;
+};
+
+static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl) {
+    const char *what = "paged_attention";
+    if (!a) return set_error(B200_ERR_BAD_ARG, "%s: null args", what);
+    PaParams &p = pl.p;
+    memset(&p, 0, sizeof(p));
+    const int rc = pool_params(a->pool, what, &p.pool);
+    if (rc) return rc;
+    if (a->q_dtype != B200_F16 && a->q_dtype != B200_BF16) return set_error(B200_ERR_BAD_ARG, "%s: query dtype %d (f16, bf16)", what, a->q_dtype);
+    if (a->pool.dtype != B200_FP8 && a->pool.dtype != a->q_dtype) return set_error(B200_ERR_BAD_ARG, "%s: a pool of dtype %d under queries of dtype %d", what, a->pool.dtype, a->q_dtype);
+    if (a->hq == 0 || a->hq % a->pool.hkv) return set_error(B200_ERR_BAD_ARG, "%s: %u query heads are not a multiple of %u kv heads", what, a->hq, a->pool.hkv);
+    if (a->max_k >= (1u << 30) || a->total_q >= (1u << 30)) return set_error(B200_ERR_UNSUPPORTED_SHAPE, "%s: %u tokens over %u keys", what, a->total_q, a->max_k);
+    if ((uint64_t)a->max_q * (a->hq / a->pool.hkv) >= (1ull << 31)) return set_error(B200_ERR_UNSUPPORTED_SHAPE, "%s: %u tokens of a sequence", what, a->max_q);
+    uint64_t low = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out);
+    for (int i = 0; i < 2; ++i) low |= (a->q_strides[i] | a->out_strides[i]) * 2;
+    if (low & 15) return set_error(B200_ERR_UNSUPPORTED_SHAPE, "%s: the rows of q and out must start at multiples of 16 bytes", what);
+    p.q = static_cast<const char *>(a->q), p.out = static_cast<char *>(a->out);
+    p.q_st = a->q_strides[0] * 2, p.q_sh = a->q_strides[1] * 2, p.o_st = a->out_strides[0] * 2, p.o_sh = a->out_strides[1] * 2;
+    p.cu_q = a->cu_q, p.kv_len = a->kv_len, p.table = a->table, p.table_stride = a->table_stride;
+    p.alibi = a->alibi, p.alibi_bs = a->alibi_bstride, p.status = a->status;
+    p.b = a->b, p.hq = a->hq, p.hkv = a->pool.hkv, p.group = a->hq / a->pool.hkv, p.d = a->pool.d;
+    p.total_q = a->total_q, p.max_q = a->max_q, p.max_k = (uint32_t)std::min<uint64_t>(a->max_k, (uint64_t)a->table_cols * a->pool.block_rows), p.table_cols = a->table_cols;
+    p.scale = a->scale, p.softcap = a->softcap, p.wl = a->wl, p.wr = a->wr;
+    pl.hd = p.d <= 64 ? 64 : (p.d <= 128 ? 128 : 256);
+    const bool mx = a->pool.dtype == B200_FP8;
+    pl.kind = (mx ? 2 : 0) + (a->q_dtype == B200_BF16 ? 1 : 0);
+    pl.unit = PA_WARPS * (pl.hd == 64 || (pl.hd == 128 && mx) ? 32 : 16);
+    int sms = 148, dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    // no more blocks than there can be units
+    const uint64_t rows = (uint64_t)a->max_q * p.group, packs = (rows + PA_ROWS - 1) / PA_ROWS;
+    const uint64_t most = std::max<uint64_t>((uint64_t)a->b * p.hkv * packs * ((p.max_k + pl.unit - 1) / pl.unit + 1), 1);
+    p.blocks = (uint32_t)std::min<uint64_t>((uint64_t)sms * (pl.hd == 256 ? 1 : 2), most);
+    p.min_units = 1;
+    const size_t part_o = (size_t)2 * p.blocks * PA_ROWS * p.d * 4;
+    pl.off_ml = (part_o + 255) / 256 * 256;
+    pl.ws_bytes = p.blocks > 1 ? pl.off_ml + (size_t)2 * p.blocks * PA_ROWS * 8 : 0;
+    return B200_OK;
+}
+
+template <int HD, int KIND>
+static int pa_launch(const PaPlan &pl, cudaStream_t stream) {
+    static thread_local bool done[16] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 16 || !done[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA<HD, KIND>::SMEM);
+        if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention: shared memory opt-in: %s", cudaGetErrorString(e));
+        if (dev >= 0 && dev < 16) done[dev] = true;
+    }
+    paged_decode_kernel<HD, KIND><<<pl.p.blocks, PA_THREADS, PA<HD, KIND>::SMEM, stream>>>(pl.p);
+    const int rc = check_launch("paged_attention");
+    if (rc || pl.p.blocks == 1) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pl.p.blocks - 1);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<PA<HD, KIND>::BF16>, pl.p, PA<HD, KIND>::UNIT);
+    if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention (join): %s", cudaGetErrorString(e));
+    return check_launch("paged_attention (join)");
+}
+template <int HD>
+static int pa_kind(const PaPlan &pl, cudaStream_t stream) {
+    switch (pl.kind) {
+    case 0: return pa_launch<HD, 0>(pl, stream);
+    case 1: return pa_launch<HD, 1>(pl, stream);
+    case 2: return pa_launch<HD, 2>(pl, stream);
+    default: return pa_launch<HD, 3>(pl, stream);
+    }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" size_t b200_paged_attention_workspace_bytes(const B200PagedAttnArgs *a) {
+    PaPlan pl;
+    return pa_plan(a, pl) ? 0 : pl.ws_bytes;
+}
+
+extern "C" int b200_paged_attention(const B200PagedAttnArgs *a, b200_stream_t stream_) {
+    PaPlan pl;
+    const int rc = pa_plan(a, pl);
+    if (rc) return rc;
+    if (a->b == 0 || a->total_q == 0 || a->max_q == 0) return B200_OK;
+    if (!a->q || !a->out || !a->cu_q || !a->kv_len || !a->table) return set_error(B200_ERR_BAD_ARG, "paged_attention: null pointer");
+    if (pl.ws_bytes) {
+        if (!a->workspace || a->workspace_bytes < pl.ws_bytes)
+            return set_error(B200_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes needed, %zu given", pl.ws_bytes, a->workspace ? a->workspace_bytes : (size_t)0);
+        if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return set_error(B200_ERR_BAD_ARG, "paged_attention: workspace must be 16-byte aligned");
+        pl.p.part_o = static_cast<float *>(a->workspace);
+        pl.p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(a->workspace) + pl.off_ml);
+    }
+    cudaStream_t stream = (cudaStream_t)stream_;
+    if (pl.hd == 64) return pa_kind<64>(pl, stream);
+    if (pl.hd == 128) return pa_kind<128>(pl, stream);
+    return pa_kind<256>(pl, stream);
+}

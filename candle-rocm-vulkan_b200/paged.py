@@ -2,8 +2,9 @@
 
 One pool holds the keys and values of all sequences: equal pages, in the layout of `flash_attn_varlen_paged_windowed`
 ((num_blocks, block_size, kv_heads, head_dim), candle-flash-attn/src/lib.rs:341-420), a table row per sequence that lists its
-pages, and one slot (block * block_size + row) per token. `append` turns the new queries and keys by their positions and writes
-keys and values, quantised where the pool holds MXFP8; `keys_values` reads sequences back.
+pages, and one slot (block * block_size + row) per token. A serving step of one layer is two calls that launch and return, with
+all lengths on the device: `append` (turns the new queries and keys by their positions and writes keys and values, quantised
+where the pool holds MXFP8) and `attention` (every sequence's new tokens over its pages). Both can be captured in a CUDA graph.
 """
 import ctypes as C
 import struct
@@ -12,7 +13,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _abi as A
-from .turbo_quant import _dtype_id, _need_cuda, _stream
+from .turbo_quant import FlashAttnConfig, _call_workspace, _dtype_id, _need_cuda, _stream
 
 _E4M3 = getattr(torch, "float8_e4m3fn", None)
 _POOL_DTYPES = {torch.float16: A.F16, torch.bfloat16: A.BF16, _E4M3: A.FP8}
@@ -23,8 +24,10 @@ _ROTARY = "3PQ4I"
 _ROTARY_ARGS = struct.Struct("@4P2Q2Q2Q2Q4IiI" + _ROTARY)
 _APPEND_ARGS = struct.Struct("@2P2Q2Q3P2Q2QIIiI" + _ROTARY + "P")   # behind the pool
 _UNPACK_ARGS = struct.Struct("@PQ3PQIIiIP")                         # behind the pool
+_ATTN_ARGS = struct.Struct("@2P2Q2Q3PQ6IiffiiPIIPNP")              # behind the pool
 assert _POOL.size == C.sizeof(A.PagedPool) and _ROTARY_ARGS.size == C.sizeof(A.RotaryArgs)
 assert _POOL.size + _APPEND_ARGS.size == C.sizeof(A.PagedAppendArgs) and _POOL.size + _UNPACK_ARGS.size == C.sizeof(A.PagedUnpackArgs)
+assert _POOL.size + _ATTN_ARGS.size == C.sizeof(A.PagedAttnArgs)
 
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
@@ -237,3 +240,44 @@ class PagedKvPool:
             table.data_ptr(), table.stride(0), cu.data_ptr(), k.data_ptr(), v.data_ptr(), k.shape[0], b, table.shape[1], _dtype_id(k), 0,
             status.data_ptr() if status is not None else 0), self.device)
         return k, v
+
+    def attention(self, q: torch.Tensor, seqlens_q: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+                  cfg: FlashAttnConfig, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of every sequence's new tokens over its pages, read where they are. `q` (total, q_heads, head_dim; f16 or bf16, a 16-bit
+        pool's own type), sequence i's tokens at rows seqlens_q[i] .. seqlens_q[i + 1] - 1: none, one, a few drafted ones or a
+        chunk of a prompt; its keys are the first kv_len[i] of its pages, the new tokens' (written before) among them. Masks are
+        bottom-right aligned as for `flash_attn_varlen`; rows without a visible key give zeros. The lengths are read on the device;
+        `max_seqlen_q` and `max_seqlen_k` bound them (longer ones are cut). Rows of `out` (a new tensor unless given) behind the last
+        sequence are left as they were. Page numbers outside the pool hold zeros and set `status` (an int32 device tensor) to 3."""
+        dev = self.device
+        q = _heads(q, "paged attention: q", None, self.head_dim)
+        total, hq, d = q.shape
+        if q.device != dev:
+            raise ValueError(f"paged attention: q is on {q.device}, the pool on {dev}")
+        if cfg.softcap is not None and not cfg.softcap > 0.0:
+            raise ValueError("flash-attn: softcap must be > 0")
+        if cfg.k_descale != 1.0 or cfg.v_descale != 1.0:
+            raise ValueError("paged attention: a pool's scales are its own; k_descale and v_descale must be 1")
+        b = seqlens_q.numel() - 1
+        if b < 0 or kv_len.numel() != b:
+            raise ValueError(f"paged attention: {seqlens_q.numel()} cumulative lengths do not go with {kv_len.numel()} sequences")
+        out = _out_like(q, out, "paged attention: out")
+        table = self._table(block_table, b, "paged attention")
+        cu = _ints(seqlens_q, torch.int32, dev, "paged attention: seqlens_q")
+        lens = _ints(kv_len, torch.int32, dev, "paged attention: kv_len")
+        alibi, abs_ = None, 0
+        if cfg.alibi_slopes is not None:
+            alibi = cfg.alibi_slopes.to(device=dev, dtype=torch.float32).contiguous()
+            if alibi.shape not in ((hq,), (b, hq)):
+                raise ValueError(f"flash-attn: alibi slopes must be ({hq}) or ({b}, {hq}), got {tuple(alibi.shape)}")
+            abs_ = hq if alibi.dim() == 2 else 0
+        wl, wr = cfg.window_i32()
+        fields = (q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0),
+                  b, total, int(max_seqlen_q), int(max_seqlen_k), hq, table.shape[1], _dtype_id(q), cfg.softmax_scale, cfg.softcap or 0.0, wl, wr,
+                  alibi.data_ptr() if alibi is not None else 0, abs_, 0)
+        st = status.data_ptr() if status is not None else 0
+        lib = A.lib()
+        nbytes = lib.b200_paged_attention_workspace_bytes(self._packed + _ATTN_ARGS.pack(*fields, 0, 0, st))
+        ws = _call_workspace(dev, nbytes) if nbytes else None
+        _call(lib.b200_paged_attention, self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr() if ws is not None else 0, nbytes, st), dev)
+        return out

@@ -557,6 +557,37 @@ typedef struct B200PagedUnpackArgs {
 } B200PagedUnpackArgs;
 int b200_paged_unpack(const B200PagedUnpackArgs *args, b200_stream_t stream);
 
+/* Attention of a ragged batch's new tokens over the pool: q (total_q, hq, d), sequence i's tokens at cu_q[i] .. cu_q[i + 1] - 1 (none,
+ * one, a few drafted ones or a chunk of a prompt), its keys the first kv_len[i] of its pages, the new tokens' among them.
+ * Masks are aligned to the bottom right (token t of lq sits at position kv_len - lq + t) as for b200_tq_attention, and rows
+ * without a visible key give zeros; scores scale * q . k, then softcap (> 0) and ALiBi. All lengths are read on the
+ * device: nothing synchronises, and a captured call follows them. max_q, max_k and the table's columns bound the lengths (longer
+ * ones are cut) and size the launches; total_q bounds cu_q[b], and rows of `out` behind cu_q[b] are left as they were. q and out of q_dtype
+ * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows.
+ * The reference gathers the pages on the host (candle-flash-attn/src/lib.rs:341-420). */
+typedef struct B200PagedAttnArgs {
+    B200PagedPool pool;
+    const void *q;
+    void *out;
+    uint64_t q_strides[2], out_strides[2];
+    const uint32_t *cu_q;  /* device, b + 1 */
+    const int32_t *kv_len; /* device, b */
+    const int32_t *table;  /* device, (b, table_cols) with row stride table_stride */
+    uint64_t table_stride;
+    uint32_t b, total_q, max_q, max_k, hq, table_cols;
+    int32_t q_dtype;
+    float scale, softcap;
+    int32_t wl, wr;
+    const float *alibi;    /* device f32 slopes or NULL */
+    uint32_t alibi_bstride; /* 0 or hq */
+    uint32_t pad;
+    void *workspace;       /* device, 16-byte aligned, b200_paged_attention_workspace_bytes() */
+    size_t workspace_bytes;
+    int32_t *status;       /* optional device word */
+} B200PagedAttnArgs;
+size_t b200_paged_attention_workspace_bytes(const B200PagedAttnArgs *args);
+int b200_paged_attention(const B200PagedAttnArgs *args, b200_stream_t stream);
+
 /* Health check: 1 when a bounded device-side wait of the attention kernels (an mbarrier that a copy or
  * a tensor core commit should have completed, the flag of another rank in the gathered attention) has run out
  * on the current device since the library was loaded or the flag was last cleared, 0 otherwise, -1 when the

@@ -354,6 +354,36 @@ pub struct B200PagedUnpackArgs {
     pub status: *mut i32,
 }
 
+#[repr(C)]
+pub struct B200PagedAttnArgs {
+    pub pool: B200PagedPool,
+    pub q: *const c_void,
+    pub out: *mut c_void,
+    pub q_strides: [u64; 2],
+    pub out_strides: [u64; 2],
+    pub cu_q: *const u32,
+    pub kv_len: *const i32,
+    pub table: *const i32,
+    pub table_stride: u64,
+    pub b: u32,
+    pub total_q: u32,
+    pub max_q: u32,
+    pub max_k: u32,
+    pub hq: u32,
+    pub table_cols: u32,
+    pub q_dtype: i32,
+    pub scale: f32,
+    pub softcap: f32,
+    pub wl: i32,
+    pub wr: i32,
+    pub alibi: *const f32,
+    pub alibi_bstride: u32,
+    pub pad: u32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: usize,
+    pub status: *mut i32,
+}
+
 #[link(name = "b200attn")]
 extern "C" {
     // host-side tables and plans (candle-core/src/accel/{formats,turbo,attention}.rs)
@@ -392,10 +422,12 @@ extern "C" {
     pub fn b200_flash_attn_paged(args: *const B200FaArgs, pages: *const B200Page, n_pages: u32, stream: b200_stream_t) -> c_int;
     pub fn b200_fa_prefill_append(fa: *const B200FaArgs, append: *const B200KvAppendArgs, stream: b200_stream_t) -> c_int;
 
-    // a pool of cache pages: rotary positions, rows in and out
+    // a pool of cache pages: rotary positions, rows in and out, attention
     pub fn b200_rotary_axes(args: *const B200RotaryArgs, stream: b200_stream_t) -> c_int;
     pub fn b200_paged_append(args: *const B200PagedAppendArgs, stream: b200_stream_t) -> c_int;
     pub fn b200_paged_unpack(args: *const B200PagedUnpackArgs, stream: b200_stream_t) -> c_int;
+    pub fn b200_paged_attention_workspace_bytes(args: *const B200PagedAttnArgs) -> usize;
+    pub fn b200_paged_attention(args: *const B200PagedAttnArgs, stream: b200_stream_t) -> c_int;
 
     // health of the bounded device waits
     pub fn b200_device_wait_status() -> c_int;

@@ -1,0 +1,396 @@
+"""Attention of a ragged batch's new tokens over a pool of cache pages, against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from gpu_util import pkg
+
+pytestmark = pytest.mark.gpu
+DT = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def P():
+    return pkg()
+
+
+class Batch:
+    """A pool full of values, sequences of `lq` new tokens over `lk` keys each on pages in random order, and their queries."""
+
+    def __init__(self, P, lq, lk, hq=8, hkv=2, d=128, page=16, dt="bf16", form=None, seed=0, pad=0, spare=2, hot=1.0, order="rows"):
+        g = self.g = torch.Generator(device="cuda").manual_seed(seed)
+        self.lq, self.lk, self.hq, self.hkv, self.d, self.page, self.P = lq, lk, hq, hkv, d, page, P
+        need = [-(-n // page) for n in lk]
+        blocks = sum(need) + spare
+        form = form or dt
+        x = [torch.randn((blocks, page, hkv, d), generator=g, device="cuda") * hot for _ in range(2)]
+        if form == "mxfp8":
+            self.pool = P.PagedKvPool(blocks, page, hkv, d, form)
+            flat = [t.flatten(0, 1) for t in x]
+            self.pool.append(flat[0], flat[1], torch.arange(blocks * page, device="cuda"))
+        elif order == "heads":
+            self.pool = P.PagedKvPool.from_tensors(*(t.to(DT[dt]).transpose(1, 2).contiguous().transpose(1, 2) for t in x))
+        else:
+            self.pool = P.PagedKvPool.from_tensors(*(t.to(DT[dt]) for t in x))
+        ids = torch.randperm(blocks, generator=g, device="cuda").int()
+        self.table = torch.full((len(lk), max(max(need, default=0), 1)), -1, dtype=torch.int32, device="cuda")
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = ids[at:at + n]
+            at += n
+        cu = [0]
+        for n in lq:
+            cu.append(cu[-1] + n)
+        self.cu = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        self.kv_len = torch.tensor(lk, dtype=torch.int32, device="cuda")
+        self.q = torch.randn((cu[-1] + pad, hq, d), generator=g, device="cuda").to(DT[dt])
+
+    def run(self, cfg, **more):
+        return self.pool.attention(self.q, self.cu, self.table, self.kv_len, max(self.lq), max(max(self.lk), 1), cfg, **more)
+
+    def rows(self, which, i):
+        t, s = getattr(self.pool, which), getattr(self.pool, which + "_scale")
+        n = -(-self.lk[i] // self.page)
+        x = t[self.table[i, :n].long()].double()
+        if s is not None:
+            x = x * torch.exp2(s[self.table[i, :n].long()].double() - 127).transpose(1, 2).repeat_interleave(32, -1)
+        return x.flatten(0, 1)[: self.lk[i]]
+
+    def check(self, got, cfg):
+        eps = torch.finfo(self.q.dtype).eps / 2
+        gq, at = self.hq // self.hkv, 0
+        wl, wr = cfg.window_i32()
+        for i, (nq, nk) in enumerate(zip(self.lq, self.lk)):
+            q, o = self.q[at:at + nq].double(), got[at:at + nq].double()
+            at += nq
+            if nq == 0:
+                continue
+            if nk == 0:
+                assert bool((o == 0).all()), i
+                continue
+            k, v = self.rows("k", i), self.rows("v", i)
+            pos = torch.arange(nq, device="cuda")[:, None] + nk - nq
+            j = torch.arange(nk, device="cuda")
+            seen = torch.ones((nq, nk), dtype=torch.bool, device="cuda")
+            if wl >= 0:
+                seen &= j >= pos - wl
+            if wr >= 0:
+                seen &= j <= pos + wr
+            for h in range(self.hq):
+                kk, vv = k[:, h // gq], v[:, h // gq]
+                s = q[:, h] @ kk.t() * cfg.softmax_scale
+                if cfg.softcap:
+                    s = cfg.softcap * torch.tanh(s / cfg.softcap)
+                if cfg.alibi_slopes is not None:
+                    sl = cfg.alibi_slopes if cfg.alibi_slopes.dim() == 1 else cfg.alibi_slopes[i]
+                    s = s - float(sl[h]) * (pos - j).abs()
+                s = s.masked_fill(~seen, -math.inf)
+                p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+                want = p @ vv
+                # scores: f32 sums of d products (truncating: 2^-23 a step), q behind a power of two (2^-25 of its largest), two roundings of
+                # the scaled score, the soft cap's tanh (2^-21 of the cap), and 2^-22 for the exponential
+                ds = (q[:, h].abs() @ kk.abs().t()) * abs(cfg.softmax_scale) * (self.d + 4) * 2.0 ** -23
+                ds = ds + q[:, h].abs().amax(-1, keepdim=True) * kk.abs().sum(-1) * abs(cfg.softmax_scale) * 2.0 ** -25
+                ds = (ds + torch.nan_to_num(s, neginf=0.0).abs() * 2.0 ** -22 + (cfg.softcap or 0.0) * 2.0 ** -21).masked_fill(~seen, 0).amax(-1, keepdim=True)
+                # weights: one rounding to 16 bits, the score's error (on the weight and on the sum), f32 sums
+                mag = p @ vv.abs()
+                tiny = 2.0 ** -24 if self.q.dtype == torch.float16 else 0.0  # an f16 weight or value below the normal ones
+                tol = mag * (eps + 2 * ds + 2.0 ** -18) + want.abs() * eps + tiny * (1 + mag + p.sum(-1, keepdim=True))
+                err = (o[:, h] - want).abs()
+                assert bool((err <= tol).all()), (i, h, float((err / tol).max()))
+        return got
+
+
+def cfg(P, d, **k):
+    c = P.FlashAttnConfig(d ** -0.5, softcap=k.get("softcap"), alibi_slopes=k.get("alibi"))
+    return c.window(k.get("wl"), k.get("wr", 0))
+
+
+RAGGED = ([1, 1, 1, 1, 1], [1, 17, 300, 64, 1000])
+
+
+@pytest.mark.parametrize("dt,form", [("bf16", None), ("f16", None), ("bf16", "mxfp8"), ("f16", "mxfp8")])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 48, 64, 256])
+def test_steps_over_ragged_lengths(P, dt, form, d, page):
+    b = Batch(P, *RAGGED, d=d, page=page, dt=dt, form=form, seed=d + page)
+    c = cfg(P, d)
+    b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("d,form", [(8, None), (40, None), (72, None), (80, None), (96, None), (32, "mxfp8"), (96, "mxfp8"), (160, "mxfp8"), (200, None)])
+def test_other_head_dims(P, d, form):
+    b = Batch(P, [1, 3, 40], [50, 700, 90], d=d, form=form, dt="f16", seed=d)
+    c = cfg(P, d)
+    b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (32, 8), (64, 8), (16, 16), (40, 8), (12, 4), (7, 1), (48, 2)])
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+def test_groups(P, hq, hkv, form):
+    b = Batch(P, [1, 2, 5, 1], [200, 33, 512, 129], hq=hq, hkv=hkv, form=form, seed=hq)
+    c = cfg(P, 128)
+    b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+@pytest.mark.parametrize("opt", [dict(wl=100), dict(wl=0), dict(wr=None), dict(wl=30, wr=20), dict(wr=5), dict(softcap=5.0), dict(softcap=0.5, wl=64), dict(alibi=1),
+                                 dict(alibi=2, wl=200)])
+def test_masks_caps_and_slopes(P, form, opt):
+    b = Batch(P, [1, 4, 30, 1, 150], [500, 257, 30, 3, 600], form=form, page=32, seed=3)
+    o = dict(opt)
+    if "alibi" in o:
+        a = torch.rand((b.hq,) if o["alibi"] == 1 else (5, b.hq), generator=b.g, device="cuda")
+        o["alibi"] = a
+    c = cfg(P, 128, **o)
+    b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,lk", [([700], [700]), ([128, 1, 65, 300], [1000, 900, 65, 2000]), ([33, 32, 31, 64, 1, 1, 1, 1], [64, 2000, 31, 64, 5, 1, 400, 3000]), ([257], [4001]),
+                                   ([17], [17]), ([1500, 900], [1500, 1030])])
+def test_chunks(P, form, d, lq, lk):
+    b = Batch(P, lq, lk, hq=8, hkv=2, d=d, form=form, dt="f16" if d == 64 else "bf16", seed=len(lq) + d)
+    c = cfg(P, d)
+    b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("page", [5, 8, 24, 64, 512])
+@pytest.mark.parametrize("hq,hkv", [(4, 4), (12, 4), (16, 1)])
+def test_chunks_on_other_pages_and_groups(P, page, hq, hkv):
+    b = Batch(P, [200, 3, 77], [333, 150, 1200], hq=hq, hkv=hkv, page=page, dt="f16", form="mxfp8" if page in (24, 64) else None, seed=page)
+    c = cfg(P, 128, wl=700)
+    b.check(b.run(c), c)
+
+
+def test_empty_sequences_and_rows_behind_the_last(P):
+    """Sequences without new tokens or without keys, tokens in front of the first key, and padded rows, which stay as they were."""
+    b = Batch(P, [0, 1, 0, 2, 5, 0, 40, 0], [10, 0, 0, 300, 3, 500, 20, 0], pad=9, seed=1)
+    c = cfg(P, 128)
+    out = torch.full_like(b.q, 7.5)
+    got = b.run(c, out=out)
+    assert got is out
+    n = int(b.cu[-1])
+    assert bool((out[n:] == 7.5).all())
+    b.check(out[:n], c)
+    assert bool((out[3:5] == 0).all())  # two of the five tokens lie in front of key 0
+    idle = Batch(P, [0, 0], [10, 0], pad=3)
+    out = torch.full_like(idle.q, 7.5)
+    idle.pool.attention(idle.q, idle.cu, idle.table, idle.kv_len, 1, 10, c, out=out)
+    assert bool((out == 7.5).all())
+
+
+@pytest.mark.parametrize("lq", [1, 5, 100])
+def test_what_nobody_sees_stays_out(P, lq):
+    """Infinities and NaNs behind a sequence's last key in its page, in pages of others, and in front of a window do not reach it."""
+    for form in (None, "mxfp8"):
+        b = Batch(P, [lq, lq], [203, 410], form=form, page=32, seed=lq)
+        c = cfg(P, 128, wl=100)
+        want = b.check(b.run(c), c).clone()
+        used = torch.zeros((b.pool.num_blocks, b.page), dtype=torch.bool, device="cuda")
+        for i in range(2):
+            lo = max(0, b.lk[i] - lq - 100)
+            j = torch.arange(lo, b.lk[i], device="cuda")
+            used[b.table[i, j // 32].long(), j % 32] = True
+        for t in (b.pool.k, b.pool.v):
+            if form is None:
+                t[~used] = math.nan
+                t[(~used) & (torch.rand(used.shape, device="cuda") < 0.5)] = math.inf
+            else:
+                t.view(torch.uint8)[~used] = 0x7f
+        assert torch.equal(b.run(c), want)
+
+
+def test_a_seen_nan_or_infinity_shows(P):
+    b = Batch(P, [1, 1], [40, 500], seed=4)
+    c = cfg(P, 128)
+    b.pool.v[b.table[1, 3].long(), 2, 0, 5] = math.nan
+    b.pool.k[b.table[0, 1].long(), 2, 1, 5] = math.inf
+    out = b.run(c)
+    assert bool(out[1, :4, 5].isnan().all()) and bool(out[1, :4, 6].isfinite().all()) and bool(out[1, 4:].isfinite().all())
+    assert bool(out[0, :4].isfinite().all()) and bool(((out[0, 4:].isnan().any(-1)) | (b.q[0, 4:, 5] < 0)).all())
+
+
+@pytest.mark.parametrize("dt,scale", [("f16", 2.0 ** -22), ("bf16", 2.0 ** 30), ("bf16", 2.0 ** -60), ("f16", 200.0)])
+def test_scales_far_from_one(P, dt, scale):
+    """MXFP8 values whose powers of two leave a 16-bit type's range or its normal numbers."""
+    b = Batch(P, [1, 3, 60], [100, 333, 64], dt=dt, form="mxfp8", hot=scale, seed=8)
+    c = P.FlashAttnConfig(128 ** -0.5 / scale if scale > 1 else 128 ** -0.5).causal()
+    b.check(b.run(c), c)
+
+
+def test_pages_outside_the_pool_hold_zeros(P):
+    b = Batch(P, [1, 1, 40], [64, 100, 90], seed=5, page=16)
+    c = cfg(P, 128)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    b.run(c, status=status)
+    assert int(status) == 0
+    for bad, seq in ((-3, 1), (b.pool.num_blocks, 2), (2 ** 31 - 1, 2)):
+        table = b.table.clone()
+        keep = b.table[seq, 2].clone()
+        table[seq, 2] = bad
+        status.zero_()
+        got = b.pool.attention(b.q, b.cu, table, b.kv_len, 40, 100, c, status=status).clone()
+        assert int(status) == 3
+        hold = [(t, t[keep.long()].clone()) for t in (b.pool.k, b.pool.v)]
+        for t, _ in hold:
+            t[keep.long()] = 0
+        b.check(got, c)
+        for t, x in hold:
+            t[keep.long()] = x
+
+
+def test_lengths_beyond_the_bounds_are_cut(P):
+    """Device lengths that pass max_k, the table or total_q are cut: nothing outside the tensors is touched."""
+    b = Batch(P, [1, 2], [80, 40], page=16, seed=6)
+    c = cfg(P, 128)
+    long = torch.tensor([10 ** 9, 40], dtype=torch.int32, device="cuda")
+    want = b.run(c)
+    got = b.pool.attention(b.q, b.cu, b.table, long, 2, 80, c)
+    assert torch.equal(got, want)
+    got = b.pool.attention(b.q, b.cu, b.table[:, :5], long, 2, 4000, c)  # five columns hold 80 keys
+    assert torch.equal(got, want)
+    cu = torch.tensor([0, 1, 10 ** 6], dtype=torch.int32, device="cuda")
+    got = b.pool.attention(b.q, cu, b.table, b.kv_len, 2, 80, c)
+    assert torch.equal(got, want)
+    got = b.pool.attention(b.q, b.cu, b.table, torch.tensor([-5, 40], dtype=torch.int32, device="cuda"), 2, 80, c)
+    assert bool((got[0] == 0).all()) and torch.equal(got[1:], want[1:])
+
+
+@pytest.mark.parametrize("n", [1, 3, 150, 700])
+def test_many_sequences_in_all_shares(P, n):
+    """Shares that begin and end anywhere in columns: random lengths, some sequences empty."""
+    g = torch.Generator().manual_seed(n)
+    lk = torch.randint(0, 900, (n,), generator=g).tolist()
+    lq = torch.randint(0, 4, (n,), generator=g).tolist()
+    lq[0] = 2
+    b = Batch(P, lq, lk, hq=8, hkv=2, d=64, page=32, dt="f16", seed=n)
+    c = cfg(P, 64)
+    b.check(b.run(c), c)
+
+
+def test_one_long_sequence(P):
+    for hq, hkv, form in ((8, 1, None), (8, 2, "mxfp8")):
+        b = Batch(P, [1], [70001], hq=hq, hkv=hkv, form=form, page=64, seed=2)
+        c = cfg(P, 128)
+        b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("lq", [1, 64])
+def test_strides_orders_and_streams(P, lq):
+    c = cfg(P, 128)
+    b = Batch(P, [lq, lq], [300, 777], seed=7, order="heads")
+    want = b.check(b.run(c), c).clone()
+    wide = torch.zeros((2 * lq, 3, b.hq, 128), device="cuda", dtype=b.q.dtype)
+    wide[:, 1] = b.q
+    out = torch.full((b.hq, 2 * lq, 136), 3.0, device="cuda", dtype=b.q.dtype)
+    view = out[..., :128].transpose(0, 1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = b.pool.attention(wide[:, 1], b.cu.long(), b.table.long(), b.kv_len.long(), lq, 777, c, out=view)
+    s.synchronize()
+    assert torch.equal(got, want) and bool((out[..., 128:] == 3).all())
+
+
+def test_a_step_in_a_graph_follows_the_lengths(P):
+    """append and attention captured together; replays after new lengths, slots and positions give what eager calls give."""
+    b = Batch(P, [1, 1, 1], [10, 200, 90], page=16, form="mxfp8", seed=11)
+    c = cfg(P, 128)
+    r = P.RotaryAxes(torch.linspace(1, 0.001, 64))
+    k, v = (torch.randn((3, 2, 128), device="cuda").bfloat16() for _ in range(2))
+    pos = torch.tensor([9, 199, 89], device="cuda")
+    rows = torch.arange(3, device="cuda")
+    slots = b.table[rows, pos // 16].long() * 16 + pos % 16
+    out = torch.empty_like(b.q)
+    pos_a, slots_a, len_a = pos[None].clone(), slots.clone(), b.kv_len.clone()
+
+    def step():
+        q = b.pool.append(k, v, slots_a, r, pos_a, b.q)
+        b.pool.attention(q, b.cu, b.table, len_a, 1, 250, c, out=out)
+
+    step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        step()
+    for back in (0, 1, 5):  # earlier places, shorter lengths
+        pos_a.copy_((pos - back)[None])
+        slots_a.copy_(b.table[rows, (pos - back) // 16].long() * 16 + (pos - back) % 16)
+        len_a.copy_(b.kv_len - back)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        step()
+        assert torch.equal(got, out)
+
+
+def test_two_graphs_on_one_stream_keep_their_scratch(P):
+    """Two captured calls replayed side by side do not share partial results."""
+    c = cfg(P, 128)
+    bs = [Batch(P, [1, 1], [3000, 2500], seed=20 + i) for i in range(2)]
+    outs = [torch.empty_like(b.q) for b in bs]
+    want = [b.run(c).clone() for b in bs]
+    graphs = []
+    s = torch.cuda.Stream()
+    for b, o in zip(bs, outs):
+        gr = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(gr, stream=s):
+            for _ in range(4):
+                b.run(c, out=o)
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_a_serving_run(P):
+    """Prompts in chunks beside generating sequences, step by step: positions on three axes, keys and values written, attended over and
+    read back, against the whole attention of what was written."""
+    torch.manual_seed(0)
+    hq, hkv, d, page = 8, 2, 128, 16
+    for form in ("bf16", "mxfp8"):
+        pool = P.PagedKvPool(64, page, hkv, d, form)
+        r = P.RotaryAxes(10000.0 ** (-torch.arange(64) / 64), [24, 20, 20])
+        table = torch.randperm(64, device="cuda")[:60].view(3, 20).int()
+        lens = [0, 0, 0]
+        plan = [[100, 0, 7], [50, 90, 1], [1, 33, 1], [1, 1, 1], [1, 1, 1]]
+        c = cfg(P, d)
+        for lq in plan:
+            n = sum(lq)
+            q, k, v = (torch.randn((n, h, d), device="cuda").bfloat16() for h in (hq, hkv, hkv))
+            at = torch.cat([torch.arange(l, l + m) for l, m in zip(lens, lq)]).cuda()
+            seq = torch.repeat_interleave(torch.arange(3), torch.tensor(lq)).cuda()
+            pos = torch.stack([at, at // 3, at % 7])
+            qr = pool.append(k, v, table[seq, at // page].long() * page + at % page, r, pos, q)
+            lens = [a + m for a, m in zip(lens, lq)]
+            cu = torch.tensor([0, lq[0], lq[0] + lq[1], n], dtype=torch.int32, device="cuda")
+            kv_len = torch.tensor(lens, dtype=torch.int32, device="cuda")
+            out = pool.attention(qr, cu, table, kv_len, max(lq), max(lens), c)
+            whole = Batch.__new__(Batch)
+            whole.lq, whole.lk, whole.hq, whole.hkv, whole.d, whole.page, whole.pool, whole.table, whole.q = lq, lens, hq, hkv, d, page, pool, table, qr
+            whole.check(out, c)
+            cuk = torch.tensor([0, lens[0], lens[0] + lens[1], sum(lens)], dtype=torch.int32, device="cuda")
+            kk, vv = pool.keys_values(table, cuk, sum(lens), dtype=torch.float32)
+            for i in range(3):
+                if lens[i]:
+                    assert torch.equal(kk[cuk[i]:cuk[i + 1]].double(), whole.rows("k", i)) and torch.equal(vv[cuk[i]:cuk[i + 1]].double(), whole.rows("v", i))
+
+
+def test_against_the_gathering_call(P):
+    """The call that gathers the pages first (flash_attn_varlen_paged_windowed) computes the same attention."""
+    b = Batch(P, [64, 1, 20], [300, 77, 20], dt="f16", seed=12)
+    c = cfg(P, 128)
+    cuk = torch.tensor([0, 300, 377, 397], dtype=torch.int32, device="cuda")
+    old = P.flash_attn.flash_attn_varlen_paged_windowed(b.q, b.pool.k, b.pool.v, b.cu, cuk, b.table.clamp_min(0), None, 64, 300, 128 ** -0.5, None, 0, 16)
+    b.check(b.run(c), c)
+    b.check(old, c)

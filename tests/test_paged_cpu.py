@@ -20,7 +20,7 @@ def test_struct_sizes_match_the_header(P):
     from pathlib import Path
     A = P._abi
     names = {"B200Rotary": A.Rotary, "B200RotaryArgs": A.RotaryArgs, "B200PagedPool": A.PagedPool, "B200PagedAppendArgs": A.PagedAppendArgs,
-             "B200PagedUnpackArgs": A.PagedUnpackArgs}
+             "B200PagedUnpackArgs": A.PagedUnpackArgs, "B200PagedAttnArgs": A.PagedAttnArgs}
     src = '#include <stdio.h>\n#include <stddef.h>\n#include "b200attn.h"\nint main(void){' + "".join(
         f'printf("{n} %zu' + " %zu" * len(t._fields_) + f'\\n", sizeof({n}), ' + ", ".join(f"offsetof({n}, {f})" for f, _ in t._fields_) + ");"
         for n, t in names.items()) + "return 0;}"
@@ -50,7 +50,7 @@ def test_packed_arguments_mirror_the_ctypes_ones(P):
         return obj
 
     for packers, cls in (((T._POOL,), A.PagedPool), ((T._ROTARY_ARGS,), A.RotaryArgs), ((T._POOL, T._APPEND_ARGS), A.PagedAppendArgs),
-                         ((T._POOL, T._UNPACK_ARGS), A.PagedUnpackArgs)):
+                         ((T._POOL, T._UNPACK_ARGS), A.PagedUnpackArgs), ((T._POOL, T._ATTN_ARGS), A.PagedAttnArgs)):
         fields = list(flat(cls))
         values = iter(range(1, 1000))
         given = [[next(values) for _ in range(n)] for _, n in fields]
@@ -161,3 +161,35 @@ def test_host_refusals(P):
         P.PagedKvPool.from_tensors(z.half(), z.bfloat16())
     with pytest.raises(RuntimeError, match="CUDA"):
         P.PagedKvPool.from_tensors(z.half(), z.half())
+
+
+def attn(A, pool_over=None, **over):
+    a = A.PagedAttnArgs()
+    a.pool = pool(A, **(pool_over or {}))
+    a.q = a.out = a.cu_q = a.kv_len = a.table = a.workspace = 1 << 20
+    a.q_strides = a.out_strides = A.u64x2(8 * 128, 128)
+    a.b, a.total_q, a.max_q, a.max_k, a.hq, a.table_cols, a.q_dtype, a.scale, a.wl = 2, 2, 1, 1000, 8, 63, A.BF16, 0.1, -1
+    a.workspace_bytes = 1 << 40
+    for n, v in over.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("pool_over,over,code,text", [
+    (dict(dtype=0), {}, -1, "holds"), (dict(dtype=1), {}, -1, "under queries"), ({}, dict(q_dtype=0), -1, "query dtype"), ({}, dict(hq=7), -1, "multiple"), ({}, dict(hq=0), -1, "multiple"),
+    (dict(d=264), {}, -2, "head dim"), ({}, dict(max_k=1 << 30), -2, "keys"), ({}, dict(total_q=1 << 30), -2, "tokens"), ({}, dict(max_q=0xffffffff), -2, "tokens"),
+    ({}, dict(q=(1 << 20) + 4), -2, "16 bytes"), ({}, dict(cu_q=None), -1, "null"), ({}, dict(table=None), -1, "null"), ({}, dict(out=None), -1, "null"),
+    ({}, dict(workspace=None), -4, "needed"), ({}, dict(workspace_bytes=100), -4, "needed"), ({}, dict(workspace=(1 << 20) + 8), -1, "aligned")])
+def test_attention_refusals(P, pool_over, over, code, text):
+    A = P._abi
+    assert A.lib().b200_paged_attention(C.byref(attn(A, pool_over, **over)), None) == code
+    assert text in A.lib().b200_last_error().decode()
+
+
+def test_attention_workspace(P):
+    """Bounded by the device, not by the lengths; nothing for calls that are refused."""
+    A = P._abi
+    need = lambda **k: A.lib().b200_paged_attention_workspace_bytes(C.byref(attn(A, **k)))
+    assert 0 < need() <= need(b=500, total_q=500, max_k=1 << 20) <= 64 << 20
+    assert need(hq=7) == 0 and A.lib().b200_paged_attention_workspace_bytes(None) == 0
+    assert A.lib().b200_paged_attention(C.byref(attn(A, b=0, q=None)), None) == 0 and A.lib().b200_paged_attention(None, None) == -1

@@ -2,6 +2,7 @@
 // shape; fa_prefill_sm100.cu: tcgen05 tiles for long prefill chunks).
 #pragma once
 #include "common.cuh"
+#include "paged.cuh"
 
 struct CUtensorMap_st;
 
@@ -41,6 +42,24 @@ int fa_prefill_sm100_launch(const FaParams &p, bool bf16, cudaStream_t stream);
 // arrive). `order`: the coordinates' places of head, key and batch entry, two bits each, K in bits 0-5, V in bits 8-13. With
 // k == null only whether maps can describe the tensors. fa_prefill_sm100.cu.
 bool fa_kv_maps(const FaParams &p, bool bf16, uint32_t keys, CUtensorMap_st *k, CUtensorMap_st *v, uint32_t *order);
+
+// The same tiles over the pages of a pool (fa_prefill_sm100.cu): what FaParams does not say. There cu_q, lq and lk (bounds of the lengths),
+// hq, hkv, group, d, b, scale, wl, wr and the split buffers have their meaning, and q its (token, head) strides.
+struct FaPages {
+    PoolParams pool;
+    const int32_t *table, *kv_len;
+    int32_t *status;
+    uint64_t table_stride, o_ss, o_sh;  // (token, head) strides of the outputs, elements
+    uint32_t table_cols, total_q;
+    uint32_t row_cap;    // sequences of up to so many packed rows are another kernel's
+    uint32_t tile_rows;  // whole tokens' rows among 256
+    uint32_t g_mul, g_shr;  // n / group
+    uint32_t box;           // rows of a page that are copied at a time
+};
+// whether the tiles take the call, and in how many key splits (part_o and part_lse, [splits][token x head], for paged_split_join)
+bool fa_paged_tiles_take(const FaParams &p, FaPages &pg, int pool_dtype);
+uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sms);
+int fa_paged_tiles_launch(const FaParams &p, const FaPages &pg, int pool_dtype, cudaStream_t stream);
 
 // decode over 16-bit K / V by tensor copies (fa_decode_tma.cu): grid (1, hkv, b * n_splits)
 bool fa_decode_tma_takes(const FaParams &p, bool paged, uint32_t sms);

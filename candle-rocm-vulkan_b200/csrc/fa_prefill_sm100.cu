@@ -975,21 +975,25 @@ __global__ void __launch_bounds__(P2_THREADS, 1) fa_prefill_sm100_kernel2(const 
 // A group skips the key tiles that none of its rows sees.
 // ---------------------------------------------------------------------------------------------
 constexpr int P3_THREADS = 384, P3_ROWS = 256, P3_BN = 128, P3_LOADER = 8, P3_ISSUER = 9, P3_OWNER = 11;
-template <int HD>
+// KV, where keys and values come from: 0 tensors, 1 pages of 16-bit elements, 2 MXFP8 pages (fa_paged_tma_kernel). Warps 12-15 of
+// the last widen the codes: one stage of raw tiles lies where the others stage their output rows.
+template <int HD, int KV = 0>
 struct P3 {
+    static constexpr int THREADS = KV == 2 ? 512 : P3_THREADS;
     static constexpr int HALVES = HD / 64, STAGES = HD == 128 ? 2 : 4;
     static constexpr uint32_t Q_HALF = P3_ROWS * 128, Q_BYTES = HALVES * Q_HALF;          // [half][row][128 bytes, swizzled]
     static constexpr uint32_t T_HALF = P3_BN * 128, T_BYTES = HALVES * T_HALF;             // a K or V tile, likewise
-    static constexpr uint32_t SM_K = Q_BYTES, SM_V = SM_K + STAGES * T_BYTES, SM_OUT = SM_V + STAGES * T_BYTES, SM_BAR = SM_OUT + 8 * 4096, SMEM = SM_BAR + 512;
+    static constexpr uint32_t SM_K = Q_BYTES, SM_V = SM_K + STAGES * T_BYTES, SM_OUT = SM_V + STAGES * T_BYTES, SM_BAR = SM_OUT + 8 * 4096, SMEM = SM_BAR + (KV ? 576 : 512);
+    static constexpr uint32_t RAW = P3_BN * HD;  // a tile of codes: K at SM_OUT, V behind it
     // barriers
     static constexpr int KF = 0, VF = STAGES, KE = 2 * STAGES, VE = 3 * STAGES, QF = 4 * STAGES, QE = QF + 1, S = QE + 1, P0 = S + 2, P1 = P0 + 2, O = P1 + 2,
-                         DRAIN = O + 2, TK = DRAIN + 2, SR = TK + 8, PV = SR + 2, VT = PV + 2, IF = VT + STAGES, IE = IF + 2, CL = IE + 2, GO = CL + 1, COUNT = GO + 1;
+                         DRAIN = O + 2, TK = DRAIN + 2, SR = TK + 8, PV = SR + 2, VT = PV + 2, IF = VT + STAGES, IE = IF + 2, CL = IE + 2, GO = CL + 1, LV = GO + 1, RF = LV + 1, RE = RF + 2, COUNT = RE + 2;
     // Head dim 64 leaves tensor memory for P beside S: the next scores are formed as soon as the last ones are in registers.
     // At 128 P lies over the first columns of S, and the next scores follow the products that read it.
     static constexpr bool EARLY = HD == 64;
     static constexpr bool TURNS = !EARLY;  // the groups' exponentials take turns (see the softmax warps)
     __host__ __device__ static constexpr uint32_t p_col(int g) { return EARLY ? 384u + 64u * g : 128u * g; }
-    static_assert(COUNT * 8 <= 464, "barriers");  // then the answer (464), item numbers (480), tensor memory (496), give-up flag (504)
+    static_assert(COUNT * 8 <= 464, "barriers");  // then the answer (464), item numbers (480), tensor memory (496), give-up flag (504), paged items (512)
 };
 
 // The grid's work: items = (batch entries x kv heads) x row tiles x key splits (p.n_splits). The pairs are taken `hpc` at a time (their keys and
@@ -1001,16 +1005,25 @@ struct P3Grid {
     float lag;  // how far (log 2) a row's reference may stay behind its maximum before O is rescaled
 };
 
-struct P3Item {
+template <int KV = 0>
+struct P3ItemOf {
     uint32_t b, hk, row0, R, gl, split;
     uint64_t q0, k0;
     int lq, lk;
     int t_lo, t_hi;  // the keys that some row of the item sees, within the item's key split
     int ntiles;
+    // pages: t_lo lies on a whole tile, v_lo is the first key seen; R ends the item's rows; groups of any size
+    int v_lo;
+    uint32_t g, g_mul, g_shr;
+    // the token and the head in its group of packed row r
+    __device__ __forceinline__ uint32_t tok(uint32_t r) const { return KV ? pool_div(r, g_mul, g_shr) : r >> gl; }
+    __device__ __forceinline__ uint32_t head(uint32_t r) const { return KV ? hk * g + (r - tok(r) * g) : (hk << gl) + (r & ((1u << gl) - 1)); }
 };
+using P3Item = P3ItemOf<0>;
 // the keys [lo, hi) that row r sees
-__device__ __forceinline__ void p3_range(const FaParams &p, const P3Item &it, uint32_t r, int &lo, int &hi) {
-    const int pos = (int)(r >> it.gl) + it.lk - it.lq;
+template <int KV>
+__device__ __forceinline__ void p3_range(const FaParams &p, const P3ItemOf<KV> &it, uint32_t r, int &lo, int &hi) {
+    const int pos = (int)it.tok(r) + it.lk - it.lq;
     lo = p.wl >= 0 && pos > p.wl ? min(pos - p.wl, it.lk) : 0;
     hi = p.wr >= 0 && pos < it.lk - p.wr - 1 ? pos + p.wr + 1 : it.lk;
     hi = max(hi, lo);
@@ -1054,7 +1067,8 @@ __device__ __forceinline__ bool p3_item(const FaParams &p, const P3Grid &gr, uin
     return true;
 }
 // the key tiles [t0, t1) of the item that some row of group g sees (empty: t0 == t1), and these keys [lo, hi)
-__device__ __forceinline__ void p3_group(const FaParams &p, const P3Item &it, int g, int &t0, int &t1, int &lo, int &hi) {
+template <int KV>
+__device__ __forceinline__ void p3_group(const FaParams &p, const P3ItemOf<KV> &it, int g, int &t0, int &t1, int &lo, int &hi) {
     t0 = t1 = lo = hi = 0;
     const uint32_t first = it.row0 + g * PF_BM;
     if (first >= it.R || it.ntiles == 0) return;
@@ -1071,8 +1085,73 @@ __device__ __forceinline__ void p3_group(const FaParams &p, const P3Item &it, in
 // steps of 16 keys that hold some it sees, and where the item's keys end inside such a step the owner warp clears the rest of
 // it: true for the item's last tile, at key j0, if what follows is another key (masked for all rows of the item) or
 // another sequence; past the end of the tensor the copy brings zeros.
-__device__ __forceinline__ bool p3_clears(const FaParams &p, const P3Item &it, int j0) {
-    return (p.varlen || it.t_hi < it.lk) && j0 + P3_BN > it.t_hi && ((it.t_hi - j0) & 15) != 0;
+// Pages: always, since what follows in a page is an old row, and at the item's first keys alike (the loader's: p3_low). MXFP8 rows are
+// cleared as they are widened.
+template <int KV>
+__device__ __forceinline__ bool p3_clears(const FaParams &p, const P3ItemOf<KV> &it, int j0) {
+    if (KV == 2) return false;
+    return (KV == 1 || p.varlen || it.t_hi < it.lk) && j0 + P3_BN > it.t_hi && ((it.t_hi - j0) & 15) != 0;
+}
+template <int KV>
+__device__ __forceinline__ bool p3_low(const P3ItemOf<KV> &it) { return KV == 1 && (it.v_lo & 15) != 0; }
+// The same for pages. `w`: sequence, kv head, row tile, key split, as the owner warp found them.
+template <int KV>
+__device__ __forceinline__ void p3_paged_item(const FaParams &p, const FaPages &pg, const int4 &w, P3ItemOf<KV> &it) {
+    it.b = (uint32_t)w.x, it.hk = (uint32_t)w.y, it.split = (uint32_t)w.w;
+    it.g = p.group, it.g_mul = pg.g_mul, it.g_shr = pg.g_shr;
+    const uint32_t q0 = min(p.cu_q[it.b], pg.total_q), q1 = min(p.cu_q[it.b + 1], pg.total_q);
+    it.q0 = q0;
+    it.k0 = 0;
+    it.lq = q1 > q0 ? (int)min(q1 - q0, p.lq) : 0;
+    it.lk = max(0, min(pg.kv_len[it.b], (int)p.lk));
+    it.row0 = (uint32_t)w.z * pg.tile_rows;
+    it.R = min((uint32_t)it.lq * p.group, it.row0 + pg.tile_rows);
+    it.ntiles = it.t_lo = it.t_hi = it.v_lo = 0;
+    if (it.row0 >= it.R) return;
+    int tmp;
+    p3_range(p, it, it.row0, it.v_lo, tmp);
+    p3_range(p, it, it.R - 1, tmp, it.t_hi);
+    it.t_hi = max(it.t_hi, it.v_lo);
+    it.t_lo = it.v_lo / P3_BN * P3_BN;
+    it.ntiles = it.t_hi > it.v_lo ? (it.t_hi - it.t_lo + P3_BN - 1) / P3_BN : 0;
+    if (p.n_splits > 1) {  // whole tiles
+        const int per = (it.ntiles + (int)p.n_splits - 1) / (int)p.n_splits, first = min((int)it.split * per, it.ntiles);
+        it.ntiles = min(per, it.ntiles - first);
+        it.t_lo += first * P3_BN;
+        it.v_lo = max(it.v_lo, it.t_lo);
+        it.t_hi = max(min(it.t_hi, it.t_lo + it.ntiles * P3_BN), it.t_lo);
+    }
+}
+// Owner warp: the sequence, kv head, row tile and key split of item n, counted over the sequences whose rows are this kernel's (a row tile's
+// heads and splits next to one another, the tiles with the most keys first). `base`, `before`: where the last search ended; items
+// mostly come in ascending order. False: there are no more than n.
+__device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, uint32_t n, uint32_t &base, uint32_t &before, int lane, int4 &w) {
+    if (n < before) base = before = 0;
+    for (; base < p.b; base += 32) {
+        const uint32_t seq = base + lane;
+        uint32_t tiles = 0;
+        if (seq < p.b) {
+            const uint32_t q0 = min(p.cu_q[seq], pg.total_q), q1 = min(p.cu_q[seq + 1], pg.total_q);
+            const uint32_t rows = q1 > q0 ? min(q1 - q0, p.lq) * p.group : 0u;
+            if (rows > pg.row_cap) tiles = (rows + pg.tile_rows - 1) / pg.tile_rows;
+        }
+        const uint32_t per = p.hkv * p.n_splits;
+        uint32_t upto = tiles * per;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, n - before < upto);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            const uint32_t rest = n - before - (__shfl_sync(0xffffffffu, upto, at) - __shfl_sync(0xffffffffu, tiles, at) * per), rank = rest / per, hs = rest - rank * per;
+            w = make_int4((int)(base + at), (int)(hs / p.n_splits), (int)(__shfl_sync(0xffffffffu, tiles, at) - 1 - rank), (int)(hs % p.n_splits));
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t e;
@@ -1110,11 +1189,23 @@ __device__ __forceinline__ int clc_answer(uint32_t answer) {
     return given ? (int)x : -1;
 }
 
-template <int HD, bool BF16>
-__global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaParams p, const __grid_constant__ CUtensorMap tm_k,
-                                                                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_q,
-                                                                       const P3Grid gr) {
-    using C = P3<HD>;
+// A tile's keys out of pages: lane i has the page of rows i x box .. of the tile that begins at key j0 (-1: no row of the item sees one of
+// them, or they are behind the last key; -2: it is no page of the pool).
+template <int KV>
+__device__ __forceinline__ int p3_page(const FaPages &pg, const P3ItemOf<KV> &it, int j0, int lane) {
+    const int j = j0 + lane * (int)pg.box;
+    if (lane * (int)pg.box >= P3_BN || j >= it.t_hi || j + (int)pg.box <= it.v_lo) return -1;
+    const uint32_t page = pool_div((uint32_t)j, pg.pool.div_mul, pg.pool.div_shr);
+    const int id = page < pg.table_cols ? pg.table[it.b * pg.table_stride + page] : -1;
+    if (id >= 0 && (uint32_t)id < pg.pool.n_blocks) return id;
+    if (pg.status) atomicExch(pg.status, 3);
+    return -2;
+}
+
+template <int HD, bool BF16, int KV>
+__device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm_k, const CUtensorMap &tm_v, const CUtensorMap &tm_q, const P3Grid &gr, const FaPages &pg) {
+    using C = P3<HD, KV>;
+    using P3Item = P3ItemOf<KV>;
     constexpr int NS = C::STAGES;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = smem_u32(smem), bar0 = sbase + C::SM_BAR;
@@ -1125,8 +1216,8 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
     if (*reinterpret_cast<volatile int *>(&g_wait_failed)) return;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&bars[C::KF + i], 1);
-            mbar_init(&bars[C::VF + i], 1);
+            mbar_init(&bars[C::KF + i], KV == 2 ? 4 : 1);
+            mbar_init(&bars[C::VF + i], KV == 2 ? 4 : 1);
             mbar_init(&bars[C::KE + i], 2);
             mbar_init(&bars[C::VE + i], 2);
             mbar_init(&bars[C::VT + i], 1);
@@ -1145,8 +1236,13 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
         for (int i = 0; i < 8; ++i) mbar_init(&bars[C::TK + i], 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars[C::IF + i], 1);
-            mbar_init(&bars[C::IE + i], 11);  // loader, two issuers, eight softmax warps
+            mbar_init(&bars[C::IE + i], KV == 2 ? 15 : 11);  // loader, two issuers, eight softmax warps (and four that widen)
+            if (KV) {
+                mbar_init(&bars[C::RF + i], 1);
+                mbar_init(&bars[C::RE + i], 4);
+            }
         }
+        if (KV) mbar_init(&bars[C::LV], 1);
         mbar_init(&bars[C::CL], 1);
         mbar_init(&bars[C::GO], 1);
         *abort_flag = 0;
@@ -1161,32 +1257,45 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
-    volatile int *items = reinterpret_cast<volatile int *>(smem + C::SM_BAR + 480);
+    volatile int *items = reinterpret_cast<volatile int *>(smem + (KV ? C::SM_BAR + 512 : C::SM_BAR + 480));
+    int4 found = make_int4(0, 0, 0, 0);
     // the block's k-th work item, as the owner warp announces it; false: there is none (or a wait has run out)
     auto next_item = [&](int k, int &n) {
         if (!ok || !(ok = p3_wait(bar0 + 8 * (C::IF + (k & 1)), (k >> 1) & 1, abort_flag))) return false;
-        n = items[k & 1];
+        if (KV) {
+            const volatile int *w = items + 4 * (k & 1);
+            found = make_int4(w[0], w[1], w[2], w[3]);
+            n = found.x;
+        } else {
+            n = items[k & 1];
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[C::IE + (k & 1)]);
         return n >= 0;
     };
+    auto the_item = [&](int n, P3Item &it) {
+        if constexpr (KV == 0) p3_item(p, gr, (uint32_t)n, it);
+        else p3_paged_item(p, pg, found, it);
+    };
 
     if (warp >= 8) {
-        // 128 threads x 56 + 256 x 224 = the launch's 384 x 168 registers
+        // 128 threads x 56 + 256 x 224 = the launch's 384 x 168 registers; with the widening warps 256 x 56 + 256 x 200 = 512 x 128
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == P3_LOADER) {
             // ============================================================ loader
             uint32_t kv = 0, nq = 0;  // key tiles and Q tiles so far
+            uint32_t low_n = 0, raw_n[2] = {0, 0};  // tiles on the barrier of first tiles; raw tiles of K and V asked for
             uint32_t tail = 0, tail_n = 0;  // a bit per stage: its V tile lands on the tail's barrier; the parity of that barrier's last copy
-            const uint64_t k_total = p.varlen ? p.cu_k[p.b] : 0;
+            const uint64_t k_total = KV == 0 && p.varlen ? p.cu_k[p.b] : 0;
             const char *kbase = reinterpret_cast<const char *>(p.k), *vbase = reinterpret_cast<const char *>(p.v);
             for (int k = 0, n; next_item(k, n); ++k) {
                 P3Item it;
-                p3_item(p, gr, n, it);
+                the_item(n, it);
                 if (it.ntiles == 0) {
                     if (lane == 0) mbar_arrive(&bars[C::GO]);
                     continue;
                 }
+                int page = KV ? p3_page(pg, it, it.t_lo, lane) : 0;  // looked up a tile ahead
                 auto load = [&](const CUtensorMap *map, uint32_t ord, uint32_t dst, int j, uint32_t bar) {
                     const uint32_t ph = ord & 3u, pk = (ord >> 2) & 3u;
                     const int bb = p.varlen ? 0 : (int)it.b;
@@ -1198,16 +1307,78 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                 if (lane == 0) {
                     // Q: coordinates (element, head in group, kv head, token, batch entry); a box is 64 elements of all heads of
                     // the group for 256 / G tokens = 256 packed rows (row = token * G + head)
-                    mbar_expect_tx(&bars[C::QF], C::Q_BYTES);
-                    const int tok = (int)((p.varlen ? it.q0 : 0) + (it.row0 >> it.gl));
+                    mbar_expect_tx(&bars[C::QF], KV ? C::HALVES * pg.tile_rows * 128 : C::Q_BYTES);
+                    const int tok = (int)((KV || p.varlen ? it.q0 : 0) + it.tok(it.row0));
                     for (int hf = 0; hf < C::HALVES; ++hf)
-                        tma_load_5d(sbase + hf * C::Q_HALF, &tm_q, 64 * hf, 0, (int)it.hk, tok, p.varlen ? 0 : (int)it.b, bar0 + 8 * C::QF);
+                        tma_load_5d(sbase + hf * C::Q_HALF, &tm_q, 64 * hf, 0, (int)it.hk, tok, KV || p.varlen ? 0 : (int)it.b, bar0 + 8 * C::QF);
                 }
                 __syncwarp();
                 ++nq;
                 for (int t = 0; t < it.ntiles; ++t, ++kv) {
                     const int st = kv % NS, j0 = it.t_lo + t * P3_BN;
                     const uint32_t ph = ((kv / NS) - 1) & 1, dk = sbase + C::SM_K + st * C::T_BYTES, dv = sbase + C::SM_V + st * C::T_BYTES;
+                    if constexpr (KV != 0) {
+                        // `box` rows of a page at a time, each by the lane that knows the page; a page that the pool does not have reads as zeros
+                        const int at = page, n_box = __popc(__ballot_sync(0xffffffffu, at != -1));
+                        if (t + 1 < it.ntiles) page = p3_page(pg, it, j0 + P3_BN, lane);
+                        const int blk = at == -2 ? (int)pg.pool.n_blocks : at, row = (int)((uint32_t)(j0 + lane * (int)pg.box) % pg.pool.block_rows);
+                        constexpr int COLS = KV == 2 ? 1 : C::HALVES;  // columns of 128 bytes (64: MXFP8 rows of no more)
+                        constexpr uint32_t ROW_B = KV == 2 && HD == 64 ? 64 : 128;
+                        auto copy = [&](const CUtensorMap *map, uint32_t ord, uint32_t dst, uint32_t bar) {
+                            if (lane == 0) mbar_expect_tx(&bars[bar], (uint32_t)n_box * pg.box * ROW_B * COLS);
+                            __syncwarp();
+                            if (at == -1) return;
+                            const uint32_t ph = ord & 3u, pk = (ord >> 2) & 3u;
+                            const int c1 = ph == 0 ? (int)it.hk : (pk == 0 ? row : blk), c2 = ph == 1 ? (int)it.hk : (pk == 1 ? row : blk), c3 = ph == 2 ? (int)it.hk : (pk == 2 ? row : blk);
+#pragma unroll
+                            for (int hf = 0; hf < COLS; ++hf) tma_load_4d(dst + hf * C::T_HALF + lane * pg.box * ROW_B, map, 64 * hf, c1, c2, c3, bar0 + 8 * bar);
+                        };
+                        if constexpr (KV == 1) {
+                            if (kv >= NS && !(ok = p3_wait(bar0 + 8 * (C::KE + st), ph, abort_flag))) break;
+                            copy(&tm_k, gr.tm_order & 0x3fu, dk, C::KF + st);
+                            __syncwarp();
+                            if (kv >= NS && !(ok = p3_wait(bar0 + 8 * (C::VE + st), ph, abort_flag))) {
+                                if (lane == 0) pf_wait_landed(bar0 + 8 * (C::KF + st), (kv / NS) & 1);
+                                break;
+                            }
+                            if (t == 0 && p3_low(it)) {
+                                // values in front of the first key that is seen, in its step of 16 keys (and, in a single tile, those behind the last)
+                                copy(&tm_v, (gr.tm_order >> 8) & 0x3fu, dv, C::LV);
+                                __syncwarp();
+                                if (!(ok = p3_wait(bar0 + 8 * C::LV, low_n++ & 1, abort_flag))) {
+                                    if (lane == 0) pf_wait_landed(bar0 + 8 * C::LV, (low_n - 1) & 1), pf_wait_landed(bar0 + 8 * (C::KF + st), (kv / NS) & 1);
+                                    break;
+                                }
+                                const int lo = it.v_lo - j0, hi = it.ntiles == 1 ? it.t_hi - j0 : P3_BN;
+                                auto clear = [&](int from, int to) {
+                                    for (int idx = from * 8 + lane; idx < to * 8; idx += 32)
+#pragma unroll
+                                        for (int hf = 0; hf < C::HALVES; ++hf) *reinterpret_cast<uint4 *>(smem + C::SM_V + st * C::T_BYTES + hf * C::T_HALF + idx * 16) = make_uint4(0, 0, 0, 0);
+                                };
+                                clear(lo & ~15, lo);
+                                clear(hi, (hi + 15) & ~15);
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&bars[C::VF + st]);
+                                tail |= 1u << (st + 8);  // nothing is left to land on this stage's barriers
+                            } else {
+                                const int full = p3_clears(p, it, j0) ? C::VT + st : C::VF + st;
+                                copy(&tm_v, (gr.tm_order >> 8) & 0x3fu, dv, (uint32_t)full);
+                                tail = (full == C::VT + st ? tail | 1u << st : tail & ~(1u << st)) & ~(1u << (st + 8));
+                                if (full == C::VT + st) tail_n ^= 1u << st;
+                            }
+                            __syncwarp();
+                        } else {
+                            for (int x = 0; x < 2; ++x) {
+                                if (kv > 0 && !(ok = p3_wait(bar0 + 8 * (C::RE + x), (kv - 1) & 1, abort_flag))) break;
+                                copy(x ? &tm_v : &tm_k, (x ? gr.tm_order >> 8 : gr.tm_order) & 0x3fu, sbase + C::SM_OUT + x * C::RAW, C::RF + x);
+                                __syncwarp();
+                                raw_n[x] = kv + 1;
+                            }
+                            if (!ok) break;
+                        }
+                        continue;
+                    }
                     if (p.varlen && it.k0 + j0 + P3_BN > k_total) {
                         // the end of the last sequence: its rows alone, by 16-byte chunks in the layout of the tensor copies
                         if (kv >= NS && !(ok = p3_wait(bar0 + 8 * (C::KE + st), ph, abort_flag) && p3_wait(bar0 + 8 * (C::VE + st), ph, abort_flag))) break;
@@ -1257,9 +1428,15 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                 *abort_flag = 1;
                 if (lane == 0) {
                     if (nq > 0) pf_wait_landed(bar0 + 8 * C::QF, (nq - 1) & 1);
+                    if (KV == 2) {
+                        for (int x = 0; x < 2; ++x)
+                            if (raw_n[x] > 0) pf_wait_landed(bar0 + 8 * (C::RF + x), (raw_n[x] - 1) & 1);
+                        kv = 0;
+                    }
                     for (uint32_t t = kv > NS ? kv - NS : 0; t < kv; ++t) {
                         pf_wait_landed(bar0 + 8 * (C::KF + t % NS), (t / NS) & 1);
                         const uint32_t st = t % NS;
+                        if (KV == 1 && (tail >> (st + 8) & 1u)) continue;
                         if (tail >> st & 1u) pf_wait_landed(bar0 + 8 * (C::VT + st), (tail_n >> st & 1u) ^ 1u);
                         else pf_wait_landed(bar0 + 8 * (C::VF + st), (t / NS) & 1);
                     }
@@ -1271,7 +1448,16 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
             // (heaviest first), so that late items go where there is time; items without rows end here. It asks when the last
             // tile of an item has been requested: the answer comes while the tiles in flight are worked on (asked for at an item's
             // start, the early blocks claim too much: 181 against 142 us for 512 items of 1 to 32 tiles).
-            const uint64_t k_total = p.varlen ? p.cu_k[p.b] : 0;
+            const uint64_t k_total = KV == 0 && p.varlen ? p.cu_k[p.b] : 0;
+            uint32_t base = 0, before = 0;  // where the search among the sequences ended
+            auto resolve = [&](int n, P3Item &x) {
+                if constexpr (KV == 0) return p3_item(p, gr, (uint32_t)n, x);
+                else {
+                    if (!p3_find(p, pg, (uint32_t)n, base, before, lane, found)) return false;
+                    p3_paged_item(p, pg, found, x);
+                    return true;
+                }
+            };
             uint32_t kv = 0, asked = 0, parity = 0;  // parity: of each stage's tail barrier, a bit each
             P3Item it, ahead;
             int n = (int)blockIdx.x;
@@ -1290,18 +1476,23 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                     n = clc_answer(sbase + C::SM_BAR + 464);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before the next answer is written
                     __syncwarp();
-                    if (n < 0 || p3_item(p, gr, (uint32_t)n, x)) return;
+                    if (n < 0 || resolve(n, x)) return;
                 }
             };
             auto announce = [&](int k) {
                 if (k >= 2 && !(ok = ok && p3_wait(bar0 + 8 * (C::IE + (k & 1)), ((k >> 1) - 1) & 1, abort_flag))) return;
                 if (lane == 0) {
-                    items[k & 1] = n;
+                    if (KV) {
+                        volatile int *w = items + 4 * (k & 1);
+                        w[0] = n < 0 ? -1 : found.x, w[1] = found.y, w[2] = found.z, w[3] = found.w;
+                    } else {
+                        items[k & 1] = n;
+                    }
                     mbar_arrive(&bars[C::IF + (k & 1)]);
                 }
                 __syncwarp();
             };
-            if (!p3_item(p, gr, (uint32_t)n, it)) take(it);
+            if (!resolve(n, it)) take(it);
             announce(0);
             for (int k = 1; ok && n >= 0; ++k, it = ahead) {
                 if (!(ok = p3_wait(bar0 + 8 * C::GO, (k - 1) & 1, abort_flag))) break;
@@ -1310,7 +1501,8 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                 if (!ok || it.ntiles == 0) continue;
                 kv += it.ntiles;
                 const int st = (kv - 1) % NS, j0 = it.t_lo + (it.ntiles - 1) * P3_BN;
-                if (!p3_clears(p, it, j0) || (p.varlen && it.k0 + j0 + P3_BN > k_total)) continue;
+                if (!p3_clears(p, it, j0) || (KV == 0 && p.varlen && it.k0 + j0 + P3_BN > k_total)) continue;
+                if (KV == 1 && it.ntiles == 1 && p3_low(it)) continue;  // the loader has cleared it
                 // cleared before V is announced
                 if (!(ok = p3_wait(bar0 + 8 * (C::VT + st), (parity >> st) & 1, abort_flag))) break;
                 parity ^= 1u << st;
@@ -1323,6 +1515,85 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                 if (lane == 0) mbar_arrive(&bars[C::VF + st]);
             }
             if (!ok) *abort_flag = 1;
+        } else if (KV == 2 && warp >= 12) {
+            // ============================================================ MXFP8 codes -> 16-bit tiles, thread = key
+            if constexpr (KV == 2) {
+                const int key = tid - 384;
+                const uint32_t nb = p.d / 32;
+                uint32_t kv = 0;
+                // the scales of the key's row (four bytes, a lane's table entry and page looked up a tile ahead); 1 where nothing is seen
+                auto scales = [&](const P3Item &it, int j0, uint32_t &ks, uint32_t &vs) {
+                    ks = vs = 0x7f7f7f7fu;
+                    const int j = j0 + key;
+                    if (j < it.v_lo || j >= it.t_hi) return;
+                    const uint32_t page = pool_div((uint32_t)j, pg.pool.div_mul, pg.pool.div_shr);
+                    const int id = page < pg.table_cols ? pg.table[it.b * pg.table_stride + page] : -1;
+                    if (id < 0 || (uint32_t)id >= pg.pool.n_blocks) return;
+                    const uint64_t at = (((uint64_t)id * pg.pool.hkv + it.hk) * pg.pool.block_rows + ((uint32_t)j - page * pg.pool.block_rows)) * nb;
+                    if (nb == 4) {
+                        ks = *reinterpret_cast<const uint32_t *>(pg.pool.ks + at);
+                        vs = *reinterpret_cast<const uint32_t *>(pg.pool.vs + at);
+                    } else {
+                        ks = vs = 0;
+                        for (uint32_t i = 0; i < nb; ++i) ks |= (uint32_t)pg.pool.ks[at + i] << (8 * i), vs |= (uint32_t)pg.pool.vs[at + i] << (8 * i);
+                    }
+                };
+                // row `key` of a raw tile, or zeros, into the layout of the tensor copies
+                auto widen = [&](uint32_t raw, uint32_t dst, uint32_t sc, bool zero) {
+                    constexpr int CH = HD / 16;  // raw chunks of 16 codes
+                    const uint32_t row = raw + key * HD;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ++ch) {
+                        uint4 w;
+                        const uint32_t sw = HD == 64 ? (ch ^ ((key >> 1) & 3)) : (ch ^ (key & 7));
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(row + (sw << 4)));
+                        const uint32_t e = (sc >> (8 * (ch >> 1))) & 0xffu, a[4] = {w.x, w.y, w.z, w.w};
+                        uint32_t rest, o[8];
+                        const uint32_t f = pool_scale2<BF16>(e, e, rest);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[2 * i] = pool_mul2<BF16>(pool_pair<BF16, 0>(a[i]), f);
+                            o[2 * i + 1] = pool_mul2<BF16>(pool_pair<BF16, 1>(a[i]), f);
+                        }
+                        if (BF16 ? e > 134u : e < 103u)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) o[i] = pool_mul2<BF16>(o[i], rest);
+                        if (zero)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) o[i] = 0u;
+                        const uint32_t c0 = 2 * ch, at = dst + (c0 >> 3) * C::T_HALF + key * 128;
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((c0 & 7) ^ (key & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + ((((c0 + 1) & 7) ^ (key & 7)) << 4)), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                    }
+                };
+                for (int k = 0, n; next_item(k, n); ++k) {
+                    P3Item it;
+                    the_item(n, it);
+                    uint32_t ks, vs, ks1 = 0, vs1 = 0;
+                    if (it.ntiles > 0) scales(it, it.t_lo, ks, vs);
+                    for (int t = 0; t < it.ntiles; ++t, ++kv, ks = ks1, vs = vs1) {
+                        const int st = kv % NS, j0 = it.t_lo + t * P3_BN;
+                        const uint32_t ph = ((kv / NS) - 1) & 1;
+                        if (t + 1 < it.ntiles) scales(it, j0 + P3_BN, ks1, vs1);
+                        const bool hidden = j0 + key < it.v_lo || j0 + key >= it.t_hi;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            if (!(ok = p3_wait(bar0 + 8 * (C::RF + x), kv & 1, abort_flag))) break;
+                            if (kv >= NS && !(ok = p3_wait(bar0 + 8 * ((x ? C::VE : C::KE) + st), ph, abort_flag))) break;
+                            widen(sbase + C::SM_OUT + x * C::RAW, sbase + (x ? C::SM_V : C::SM_K) + st * C::T_BYTES, x ? vs : ks, hidden);
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                            if (lane == 0) {
+                                mbar_arrive(&bars[(x ? C::VF : C::KF) + st]);
+                                mbar_arrive(&bars[C::RE + x]);
+                            }
+                        }
+                        if (!ok) break;
+                    }
+                    if (!ok) break;
+                }
+                if (!ok) *abort_flag = 1;
+            }
         } else {
             // ============================================================ matrix products of group g
             const int g = warp - P3_ISSUER;
@@ -1349,7 +1620,7 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
             };
             for (int k = 0, n; next_item(k, n); ++k) {
                 P3Item it;
-                p3_item(p, gr, n, it);
+                the_item(n, it);
                 if (it.ntiles == 0) continue;
                 int t0, t1, lo, hi;
                 p3_group(p, it, g, t0, t1, lo, hi);
@@ -1431,7 +1702,8 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
         }
     } else {
         // ================================================================ softmax, thread = row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        if (KV == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int g = warp >> 2, w4 = warp & 3;
         const uint32_t lane_base = tmem + ((uint32_t)(w4 * 32) << 16), s_col = lane_base + 128u * g, p_col = lane_base + C::p_col(g), o_col = lane_base + 256u + (uint32_t)HD * g;
         const float sl2 = p.scale * p.kd * PF_LOG2E;
@@ -1442,7 +1714,7 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
         // first key on
         auto begin = [&](int k) {
             if (!next_item(k, n)) return false;
-            p3_item(p, gr, (uint32_t)n, it);
+            the_item(n, it);
             int lo, hi, tmp;
             p3_group(p, it, g, t0, t1, lo, hi);
             const uint32_t g_row0 = it.row0 + g * PF_BM, r = g_row0 + w4 * 32 + lane;
@@ -1456,7 +1728,7 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                 p3_range(p, it, min(g_row0 + PF_BM, it.R) - 1, lo, tmp);
                 p3_range(p, it, g_row0, tmp, hi);
                 lomax = lo - it.t_lo;
-                himin = g_row0 + PF_BM > it.R ? -1 : min(hi, it.t_hi) - it.t_lo;
+                himin = !KV && g_row0 + PF_BM > it.R ? -1 : min(hi, it.t_hi) - it.t_lo;  // (rows that do not exist need no mask, and over pages get none)
             }
             return true;
         };
@@ -1601,7 +1873,7 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                 // f32 rows, 32 elements at a time: outputs, or a key split with the logarithm of the row's sum for fa_combine_kernel
                 float *const dst = p.n_splits > 1 ? p.part_o : reinterpret_cast<float *>(p.o);
                 const uint64_t part = (uint64_t)cur.split * p.rows_total;
-                auto out_row = [&](uint32_t rr) { return (cur.q0 + (rr >> cur.gl)) * p.hq + (cur.hk << cur.gl) + (rr & ((1u << cur.gl) - 1)); };
+                auto out_row = [&](uint32_t rr) { return (cur.q0 + cur.tok(rr)) * p.hq + cur.head(rr); };
                 const uint32_t r = cur.row0 + g * PF_BM + w4 * 32 + lane;
                 if (p.n_splits > 1 && r < cur.R) p.part_lse[part + out_row(r)] = l == 0.0f ? -INFINITY : mref * 0.6931471805599453f + logf(l);  // a NaN stays one
 #pragma unroll 1
@@ -1614,6 +1886,14 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = 0u;
                     }
+                    if constexpr (KV == 2) {  // (the stage holds codes)
+                        if (r < cur.R)
+#pragma unroll
+                            for (int v4 = 0; v4 < 8; ++v4)
+                                if (c0 + 4 * v4 < p.d)
+                                    *reinterpret_cast<float4 *>(dst + (part + out_row(r)) * p.d + c0 + 4 * v4) =
+                                        make_float4(u2f(o[4 * v4]) * inv, u2f(o[4 * v4 + 1]) * inv, u2f(o[4 * v4 + 2]) * inv, u2f(o[4 * v4 + 3]) * inv);
+                    } else {
 #pragma unroll
                     for (int v4 = 0; v4 < 8; ++v4)
                         *reinterpret_cast<float4 *>(stage + lane * 128 + ((v4 ^ (lane & 7)) << 4)) =
@@ -1626,6 +1906,7 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                         if (rr < cur.R && c0 + 4 * c4 < p.d) *reinterpret_cast<float4 *>(dst + (part + out_row(rr)) * p.d + c0 + 4 * c4) = w;
                     }
                     __syncwarp();
+                    }
                 }
                 tc_fence_before();
                 continue;
@@ -1649,19 +1930,26 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
                         w.y = pf_pack2<BF16>(u2f(o[8 * v4 + 2]) * inv, u2f(o[8 * v4 + 3]) * inv);
                         w.z = pf_pack2<BF16>(u2f(o[8 * v4 + 4]) * inv, u2f(o[8 * v4 + 5]) * inv);
                         w.w = pf_pack2<BF16>(u2f(o[8 * v4 + 6]) * inv, u2f(o[8 * v4 + 7]) * inv);
+                        if (KV == 2) {
+                            const uint32_t rr = cur.row0 + g * PF_BM + w4 * 32 + lane;
+                            if (rr < cur.R && 64 * hf + 32 * ch + 8 * v4 < p.d)
+                                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.o) + (cur.q0 + cur.tok(rr)) * pg.o_ss + cur.head(rr) * pg.o_sh + 64 * hf + 32 * ch + 8 * v4) = w;
+                            continue;
+                        }
                         *reinterpret_cast<uint4 *>(stage + lane * 128 + (((ch * 4 + v4) ^ (lane & 7)) << 4)) = w;
                     }
                 }
+                if constexpr (KV != 2) {
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t row = i * 4 + (lane >> 3), c8 = lane & 7, rr = cur.row0 + g * PF_BM + w4 * 32 + row;
                     const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * 128 + ((c8 ^ (row & 7)) << 4));
-                    const uint64_t orow = (cur.q0 + (rr >> cur.gl)) * p.hq + (cur.hk << cur.gl) + (rr & ((1u << cur.gl) - 1));
-                    if (rr < cur.R && 64 * hf + 8 * c8 < p.d)
-                        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.o) + orow * p.d + 64 * hf + 8 * c8) = w;
+                    const uint64_t at = KV ? (cur.q0 + cur.tok(rr)) * pg.o_ss + cur.head(rr) * pg.o_sh : ((cur.q0 + cur.tok(rr)) * p.hq + cur.head(rr)) * p.d;
+                    if (rr < cur.R && 64 * hf + 8 * c8 < p.d) *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p.o) + at + 64 * hf + 8 * c8) = w;
                 }
                 __syncwarp();
+                }
             }
             tc_fence_before();  // O has been read before the next item's first P is announced
         }
@@ -1672,6 +1960,19 @@ __global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaP
     tc_fence_after();
     if (warp == P3_OWNER) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     if (tid == 0 && *abort_flag) atomicExch(&g_wait_failed, 1);
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(P3_THREADS, 1) fa_prefill_tma_kernel(const FaParams p, const __grid_constant__ CUtensorMap tm_k,
+                                                                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_q,
+                                                                       const P3Grid gr) {
+    p3_body<HD, BF16, 0>(p, tm_k, tm_v, tm_q, gr, FaPages{});
+}
+template <int HD, bool BF16, int KV>
+__global__ void __launch_bounds__(P3<HD, KV>::THREADS, 1) fa_paged_tma_kernel(const FaParams p, const __grid_constant__ CUtensorMap tm_k,
+                                                                              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_q,
+                                                                              const P3Grid gr, const FaPages pg) {
+    p3_body<HD, BF16, KV>(p, tm_k, tm_v, tm_q, gr, pg);
 }
 
 // ---- tensor maps -------------------------------------------------------------------------------------------------------
@@ -1693,22 +1994,22 @@ struct KvDims {
     uint64_t size[3], stride[3];
     uint32_t order;
 };
-static bool kv_dims(KvDims *m, const void *base, uint64_t nb, uint64_t hkv, uint64_t lk, uint64_t d_, uint64_t s_b, uint64_t s_h, uint64_t s_s) {
+static bool kv_dims(KvDims *m, const void *base, uint64_t nb, uint64_t hkv, uint64_t lk, uint64_t d_, uint64_t s_b, uint64_t s_h, uint64_t s_s, uint64_t es = 2) {
     if (reinterpret_cast<uintptr_t>(base) & 15) return false;
     struct Dim {
         uint64_t size, stride;
         int role;
-    } d[3] = {{hkv, s_h * 2, 0}, {lk, s_s * 2, 1}, {nb, s_b * 2, 2}};
+    } d[3] = {{hkv, s_h * es, 0}, {lk, s_s * es, 1}, {nb, s_b * es, 2}};
     std::stable_sort(d, d + 3, [](const Dim &a, const Dim &c) {
         if ((a.size == 1) != (c.size == 1)) return c.size == 1;  // entries of extent 1 go last
         return a.size > 1 && a.stride < c.stride;
     });
-    uint64_t prev = d_ * 2;
+    uint64_t prev = d_ * es;
     m->order = 0;
     for (int i = 0; i < 3; ++i) {
         if (d[i].size == 0) return false;
         if (d[i].size == 1) {
-            d[i].stride = (d_ * 2 + 15) / 16 * 16;  // any legal value: the coordinate is always 0
+            d[i].stride = (d_ * es + 15) / 16 * 16;  // any legal value: the coordinate is always 0
         } else {
             if ((d[i].stride & 15) || d[i].stride < prev || d[i].stride >= (1ull << 40) || d[i].size > (1ull << 31)) return false;
             prev += d[i].stride * (d[i].size - 1);
@@ -1853,6 +2154,83 @@ static int fa_prefill_tma_launch(const FaParams &p, cudaStream_t stream) {
     gr.lag = p.d == 128 && rows >= 512 && !p.copies ? PF_SLACK : 0.0f;
     fa_prefill_tma_kernel<HD, BF16><<<gr.items, P3_THREADS, P3<HD>::SMEM, stream>>>(p, tm_k, tm_v, tm_q, gr);
     return check_launch("flash_attn (tcgen05 tiles)");
+}
+
+// ---- the tiles over pages ------------------------------------------------------------------------------------------------
+// A pool's K or V as a map sees it: (block, row, head, d) as (batch, key, head, d).
+static bool pool_dims(const FaPages &pg, bool v, uint64_t es, KvDims *m) {
+    const PoolParams &pl = pg.pool;
+    return kv_dims(m, v ? pl.v : pl.k, pl.n_blocks, pl.hkv, pl.block_rows, pl.d, (v ? pl.v_sb : pl.k_sb) / es, (v ? pl.v_sh : pl.k_sh) / es, (v ? pl.v_sr : pl.k_sr) / es, es);
+}
+bool fa_paged_tiles_take(const FaParams &p, FaPages &pg, int pool_dtype) {
+    // pages in whole groups of eight rows, what the 128-byte swizzle repeats after; smaller ones stay on mma.sync
+    uint32_t box = 128;
+    while (pg.pool.block_rows % box) box /= 2;
+    if (box < 8 || p.d > 128 || p.softcap > 0.0f || p.alibi != nullptr || !(p.scale > 0.0f) || p.group > P3_ROWS) return false;
+    const uint64_t es = pool_dtype == B200_FP8 ? 1 : 2;
+    KvDims k, v;
+    if (!pool_dims(pg, false, es, &k) || !pool_dims(pg, true, es, &v)) return false;
+    const uint64_t row = (uint64_t)p.d * 2;
+    if (p.q_sh * 2 >= (1ull << 40) / p.hq || p.q_ss * 2 >= (1ull << 40) || (p.hq > 1 && p.q_sh * 2 < row) || (pg.total_q > 1 && p.q_ss * 2 < row)) return false;
+    pg.box = box;
+    pg.tile_rows = P3_ROWS / p.group * p.group;
+    pool_div_init(p.group, &pg.g_mul, &pg.g_shr);
+    return true;
+}
+// an upper bound of the work items of one key split: row tiles x kv heads
+static uint64_t paged_items(const FaParams &p, const FaPages &pg) {
+    const uint64_t tiles = ((uint64_t)p.lq * p.group + pg.tile_rows - 1) / pg.tile_rows, big = std::min<uint64_t>(p.b, pg.total_q / (pg.row_cap / p.group + 1));
+    return std::max<uint64_t>(std::min<uint64_t>(big * tiles, (uint64_t)pg.total_q * p.group / pg.tile_rows + big), 1) * p.hkv;
+}
+uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sms) {
+    // as fa_prefill_sm100_splits; the lengths are bounds here, and splits that find no keys cost a partial result of nothing
+    const uint64_t keys = p.wl >= 0 ? std::min<uint64_t>(p.lk, (uint64_t)p.wl + P3_ROWS) : p.lk;
+    return (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::min<uint64_t>(sms / paged_items(p, pg), keys / (4 * P3_BN)), 64), 1);
+}
+template <int HD, bool BF16, int KV>
+static int fa_paged_launch_as(const FaParams &p, const FaPages &pg, const P3Grid &gr, const CUtensorMap &tm_k, const CUtensorMap &tm_v, const CUtensorMap &tm_q, cudaStream_t stream) {
+    static thread_local bool done[16] = {};
+    const int rc = pf_opt_in(fa_paged_tma_kernel<HD, BF16, KV>, P3<HD, KV>::SMEM, done);
+    if (rc) return rc;
+    fa_paged_tma_kernel<HD, BF16, KV><<<gr.items, P3<HD, KV>::THREADS, P3<HD, KV>::SMEM, stream>>>(p, tm_k, tm_v, tm_q, gr, pg);
+    return check_launch("paged_attention (tcgen05 tiles)");
+}
+int fa_paged_tiles_launch(const FaParams &p, const FaPages &pg, int pool_dtype, cudaStream_t stream) {
+    const bool mx = pool_dtype == B200_FP8, bf16 = p.q_dtype == B200_BF16;
+    const uint64_t es = mx ? 1 : 2, items = paged_items(p, pg) * p.n_splits;
+    KvDims k, v;
+    const EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc || items >= (1ull << 31) || !pool_dims(pg, false, es, &k) || !pool_dims(pg, true, es, &v)) return FA_NO_MAP;
+    const CUtensorMapDataType t16 = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap tm_k, tm_v, tm_q;
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    for (int x = 0; x < 2; ++x) {
+        const KvDims &m = x ? v : k;
+        const cuuint64_t dims[4] = {(cuuint64_t)p.d, m.size[0], m.size[1], m.size[2]}, strides[3] = {m.stride[0], m.stride[1], m.stride[2]};
+        const bool narrow = mx && p.d <= 64;  // a row of codes in 64 bytes
+        cuuint32_t box[4] = {(cuuint32_t)(mx ? (narrow ? 64 : 128) : 64), 1, 1, 1};
+        box[1 + ((m.order >> 2) & 3u)] = pg.box;
+        if (enc(x ? &tm_v : &tm_k, mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : t16, 4, x ? pg.pool.v : pg.pool.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return FA_NO_MAP;
+    }
+    {
+        const uint64_t G = p.group, row = ((uint64_t)p.d * 2 + 15) / 16 * 16;
+        const cuuint64_t strides[4] = {p.hq > 1 ? p.q_sh * 2 : row, p.hkv > 1 ? G * p.q_sh * 2 : row, pg.total_q > 1 ? p.q_ss * 2 : row, row};
+        const cuuint64_t dims[5] = {(cuuint64_t)p.d, G, p.hkv, pg.total_q, 1};
+        const cuuint32_t box[5] = {64, (cuuint32_t)G, 1, (cuuint32_t)(P3_ROWS / G), 1};
+        if (enc(&tm_q, t16, 5, const_cast<void *>(p.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return FA_NO_MAP;
+    }
+    P3Grid gr = {};
+    gr.items = (uint32_t)items;
+    gr.tm_order = k.order | (v.order << 8);
+    gr.lag = p.d > 64 && (uint64_t)p.lq * p.group >= 512 ? PF_SLACK : 0.0f;  // as in fa_prefill_tma_launch
+#define B200_PAGED(HD, BF16) (mx ? fa_paged_launch_as<HD, BF16, 2>(p, pg, gr, tm_k, tm_v, tm_q, stream) : fa_paged_launch_as<HD, BF16, 1>(p, pg, gr, tm_k, tm_v, tm_q, stream))
+    if (p.d <= 64) return bf16 ? B200_PAGED(64, true) : B200_PAGED(64, false);
+    return bf16 ? B200_PAGED(128, true) : B200_PAGED(128, false);
+#undef B200_PAGED
 }
 
 int fa_prefill_sm100_launch(const FaParams &p, bool bf16, cudaStream_t stream) {

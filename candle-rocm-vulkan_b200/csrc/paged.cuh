@@ -22,6 +22,58 @@ inline void pool_div_init(uint32_t d, uint32_t *mul, uint32_t *shr) {
 }
 __device__ __forceinline__ uint32_t pool_div(uint32_t n, uint32_t mul, uint32_t shr) { return (uint32_t)(((uint64_t)__umulhi(n, mul) + n) >> shr); }
 
+template <bool BF16>
+__device__ __forceinline__ uint32_t pool_mul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// E4M3 codes as pairs of values: f16, or bf16 times 2^-120 (a code's exponent and mantissa in the places of a bf16's, its subnormals
+// among that type's). pool_codes: byte I of two words; pool_pair: bytes 2 I and 2 I + 1 of one.
+template <bool BF16, int I>
+__device__ __forceinline__ uint32_t pool_codes(uint32_t lo, uint32_t hi) {
+    if (BF16) {
+        const uint32_t t = __byte_perm(lo, hi, (4u + I) << 12 | I << 4);
+        return (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+    }
+    return cvt_e4m3x2_f16x2(__byte_perm(lo, hi, (4u + I) << 4 | I));
+}
+template <bool BF16, int I>
+__device__ __forceinline__ uint32_t pool_pair(uint32_t w) {
+    if (BF16) {
+        const uint32_t t = __byte_perm(w, w, (2u * I + 1u) << 12 | (2u * I) << 4);
+        return (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+    }
+    return I ? cvt_e4m3x2_hi_f16x2(w) : cvt_e4m3x2_f16x2(w);
+}
+// The multiplier that takes such a pair to its values, for the scales e0 and e1: f16 2^(e - 127), bf16 2^(e - 127 + 120). Scales outside the
+// type's range (f16 e < 103, bf16 e > 134) go in two steps: `rest` is the second.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pool_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
+    if (BF16) {
+        const uint32_t m0 = min(e0, 134u), m1 = min(e1, 134u);
+        rest = (e0 - m0 + 127u) << 7 | (e1 - m1 + 127u) << 23;
+        return (m0 + 120u) << 7 | (m1 + 120u) << 23;
+    }
+    const uint32_t m0 = max(e0, 103u), m1 = max(e1, 103u);
+    rest = pack_f16x2(e8m0_to_f(e0 + 127u - m0), e8m0_to_f(e1 + 127u - m1));
+    return pack_f16x2(e8m0_to_f(m0), e8m0_to_f(m1));
+}
+
+// the sequence of packed row t: the last i with cu[i] <= t among 0 .. b - 1 (a warp at once, 32 probes a step)
+__device__ __forceinline__ uint32_t pool_seq(const uint32_t *cu, uint32_t b, uint64_t t, int lane) {
+    uint32_t lo = 0, n = b;  // the answer is in [lo, lo + n)
+    while (n > 1) {
+        const uint32_t step = (n + 31) / 32, at = lo + lane * step;
+        const uint32_t hit = __ballot_sync(0xffffffffu, (uint32_t)lane * step < n && cu[at] <= t);
+        const uint32_t last = hit ? 31 - __clz(hit) : 0;  // (cu ascends)
+        lo += last * step;
+        n = min(step, n - last * step);
+    }
+    return lo;
+}
+
 // checks the description and fills the kernels' view of it
 int pool_params(const B200PagedPool &pool, const char *what, PoolParams *p);
 

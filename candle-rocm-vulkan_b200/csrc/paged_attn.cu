@@ -18,7 +18,7 @@
 // that type's range; weights are rounded to q's type, as for 16-bit pools (2^-9 or 2^-12 each, and they average out).
 #include <algorithm>
 
-#include "paged.cuh"
+#include "fa_params.cuh"
 
 namespace b200 {
 
@@ -41,6 +41,7 @@ struct PaParams {
     float scale, softcap;
     int32_t wl, wr;
     uint32_t blocks, min_units;
+    uint32_t row_cap;  // sequences of more packed rows are on the tcgen05 tiles; 0: all are here
 };
 
 // KIND: 0 f16, 1 bf16, 2 MXFP8 under f16 queries, 3 MXFP8 under bf16 queries
@@ -82,7 +83,7 @@ __device__ __forceinline__ uint64_t pa_seq(const PaParams &p, uint32_t b, int un
     s.rows = (uint32_t)s.lq * p.group;
     s.packs = (s.rows + PA_ROWS - 1) / PA_ROWS;
     s.ulo = s.uhi = 0;
-    if (s.rows == 0) return 0;
+    if (s.rows == 0 || (p.row_cap && s.rows > p.row_cap)) return 0;
     int lo, hi, x;
     pa_range(p, s, 0, lo, x);
     pa_range(p, s, s.rows - 1, x, hi);
@@ -194,37 +195,6 @@ __device__ __forceinline__ uint32_t pa_pack2(float lo, float hi) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t pa_mul2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-// the E4M3 codes of byte i of two words as a pair of values: f16, or bf16 times 2^-120 (a code's exponent and mantissa in the places
-// of a bf16's, its subnormals among that type's)
-template <bool BF16, int I>
-__device__ __forceinline__ uint32_t pa_codes(uint32_t lo, uint32_t hi) {
-    if (BF16) {
-        const uint32_t t = __byte_perm(lo, hi, (4u + I) << 12 | I << 4);
-        return (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
-    }
-    return cvt_e4m3x2_f16x2(__byte_perm(lo, hi, (4u + I) << 4 | I));
-}
-// The multiplier that takes such a pair to its values, for the scales e0 and e1: f16 2^(e - 127), bf16 2^(e - 127 + 120). Scales outside the
-// type's range (f16 e < 103, bf16 e > 134) go in two steps: `rest` is the second.
-template <bool BF16>
-__device__ __forceinline__ uint32_t pa_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
-    if (BF16) {
-        const uint32_t m0 = min(e0, 134u), m1 = min(e1, 134u);
-        rest = (e0 - m0 + 127u) << 7 | (e1 - m1 + 127u) << 23;
-        return (m0 + 120u) << 7 | (m1 + 120u) << 23;
-    }
-    const uint32_t m0 = max(e0, 103u), m1 = max(e1, 103u);
-    rest = pack_f16x2(e8m0_to_f(e0 + 127u - m0), e8m0_to_f(e1 + 127u - m1));
-    return pack_f16x2(e8m0_to_f(m0), e8m0_to_f(m1));
-}
-
 template <int HD, int KIND>
 __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_kernel(const PaParams p) {
     using C = PA<HD, KIND>;
@@ -475,7 +445,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
 #pragma unroll
                 for (int k = 0; k < 4; ++k) e[k] = pa_lds8(vsc + (kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8) * C::NB);
                 uint32_t rest0, rest1;
-                const uint32_t f0 = pa_scale2<BF16>(e[0], e[1], rest0), f1 = pa_scale2<BF16>(e[2], e[3], rest1);
+                const uint32_t f0 = pool_scale2<BF16>(e[0], e[1], rest0), f1 = pool_scale2<BF16>(e[2], e[3], rest1);
                 const uint32_t top = max(max(e[0], e[1]), max(e[2], e[3])), low = min(min(e[0], e[1]), min(e[2], e[3]));
                 const bool far = __any_sync(0xffffffffu, BF16 ? top > 134u : low < 103u);
 #pragma unroll
@@ -488,15 +458,15 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        uint32_t b0[4] = {pa_codes<BF16, 0>(w[0][x], w[1][x]), pa_codes<BF16, 1>(w[0][x], w[1][x]), pa_codes<BF16, 2>(w[0][x], w[1][x]),
-                                          pa_codes<BF16, 3>(w[0][x], w[1][x])};
-                        uint32_t b1[4] = {pa_codes<BF16, 0>(w[2][x], w[3][x]), pa_codes<BF16, 1>(w[2][x], w[3][x]), pa_codes<BF16, 2>(w[2][x], w[3][x]),
-                                          pa_codes<BF16, 3>(w[2][x], w[3][x])};
+                        uint32_t b0[4] = {pool_codes<BF16, 0>(w[0][x], w[1][x]), pool_codes<BF16, 1>(w[0][x], w[1][x]), pool_codes<BF16, 2>(w[0][x], w[1][x]),
+                                          pool_codes<BF16, 3>(w[0][x], w[1][x])};
+                        uint32_t b1[4] = {pool_codes<BF16, 0>(w[2][x], w[3][x]), pool_codes<BF16, 1>(w[2][x], w[3][x]), pool_codes<BF16, 2>(w[2][x], w[3][x]),
+                                          pool_codes<BF16, 3>(w[2][x], w[3][x])};
 #pragma unroll
                         for (int y = 0; y < 4; ++y) {
-                            b0[y] = pa_mul2<BF16>(b0[y], f0);
-                            b1[y] = pa_mul2<BF16>(b1[y], f1);
-                            if (far) b0[y] = pa_mul2<BF16>(b0[y], rest0), b1[y] = pa_mul2<BF16>(b1[y], rest1);
+                            b0[y] = pool_mul2<BF16>(b0[y], f0);
+                            b1[y] = pool_mul2<BF16>(b1[y], f1);
+                            if (far) b0[y] = pool_mul2<BF16>(b0[y], rest0), b1[y] = pool_mul2<BF16>(b1[y], rest1);
                             pa_mma<BF16>(oacc[(i + x) * 4 + y], pa[kk], b0[y], b1[y]);
                         }
                     }
@@ -678,13 +648,62 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const
     }
 }
 
+// Key splits of the tcgen05 tiles: one warp per token and head of the sequences that are theirs, as fa_combine_kernel.
+template <bool BF16>
+__global__ void __launch_bounds__(128) paged_split_join(const PaParams p, const uint32_t row_cap, const float *__restrict__ part_o, const float *__restrict__ part_lse,
+                                                        const uint32_t n_splits) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t rows = (uint64_t)p.total_q * p.hq;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint64_t row = (uint64_t)blockIdx.x * 4 + warp; row < rows; row += (uint64_t)gridDim.x * 4) {
+        const uint32_t tok = (uint32_t)(row / p.hq), h = (uint32_t)(row - (uint64_t)tok * p.hq);
+        if (tok >= p.cu_q[p.b]) return;
+        const uint32_t seq = pool_seq(p.cu_q, p.b, tok, lane), q0 = p.cu_q[seq], lq = p.cu_q[seq + 1] - q0;
+        if (tok < q0 || tok - q0 >= min(lq, p.max_q) || min(lq, p.max_q) * p.group <= row_cap) continue;
+        float e0 = (uint32_t)lane < n_splits ? part_lse[(uint64_t)lane * rows + row] : -INFINITY;
+        float e1 = (uint32_t)lane + 32 < n_splits ? part_lse[(uint64_t)(lane + 32) * rows + row] : -INFINITY;
+        float mx = fmaxf(e0, e1);
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+        e0 = e0 == -INFINITY ? 0.0f : expf(e0 - mx);
+        e1 = e1 == -INFINITY ? 0.0f : expf(e1 - mx);
+        float wsum = e0 + e1;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, k);
+        const uint32_t d = 4 * lane;  // (head dims up to 128)
+        float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s0 = 0; s0 < n_splits; s0 += 4) {
+            float4 v[4];
+            float w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t s = s0 + k;
+                w[k] = __shfl_sync(0xffffffffu, s < 32 ? e0 : e1, s & 31u);
+                if (s >= n_splits || d >= p.d) w[k] = 0.0f;
+                v[k] = w[k] != 0.0f ? *reinterpret_cast<const float4 *>(part_o + ((uint64_t)s * rows + row) * p.d + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[0] += w[k] * v[k].x, a[1] += w[k] * v[k].y, a[2] += w[k] * v[k].z, a[3] += w[k] * v[k].w;
+        }
+        if (d < p.d) {
+            const float inv = wsum == 0.0f ? 0.0f : 1.0f / wsum;
+            *reinterpret_cast<uint2 *>(p.out + (uint64_t)tok * p.o_st + h * p.o_sh + d * 2) = make_uint2(pa_pack2<BF16>(a[0] * inv, a[1] * inv), pa_pack2<BF16>(a[2] * inv, a[3] * inv));
+        }
+    }
+}
+
 struct PaPlan {
     PaParams p;
     int hd, kind, unit;
     size_t ws_bytes, off_ml;
+    // the tcgen05 tiles: sequences of more than 16 packed rows
+    bool tiles, steps;  // they are launched; the kernel of this file is
+    FaParams fa;
+    FaPages pg;
+    size_t off_split, off_lse;
 };
 
-static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl) {
+static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) {
     const char *what = "paged_attention";
     if (!a) return set_error(B200_ERR_BAD_ARG, "%s: null args", what);
     PaParams &p = pl.p;
@@ -712,14 +731,45 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl) {
     pl.unit = PA_WARPS * (pl.hd == 64 || (pl.hd == 128 && mx) ? 32 : 16);
     int sms = 148, dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    // Sequences of up to 16 packed rows (one group of mma.sync) are bound by their keys' bytes and stay here, longer ones by products:
+    // the tcgen05 tiles, where these take the call at all. Where all lengths are alike as far as the bounds tell, one kernel has all.
+    pl.tiles = false, pl.steps = true;
+    if (may_map && (uint64_t)a->max_q * p.group > PA_ROWS) {
+        FaParams &f = pl.fa;
+        FaPages &g = pl.pg;
+        memset(&f, 0, sizeof(f));
+        memset(&g, 0, sizeof(g));
+        f.q = a->q, f.o = a->out, f.cu_q = a->cu_q;
+        f.b = a->b, f.lq = a->max_q, f.lk = p.max_k, f.hq = p.hq, f.hkv = p.hkv, f.d = p.d, f.group = p.group;
+        f.q_ss = a->q_strides[0], f.q_sh = a->q_strides[1];
+        f.scale = a->scale, f.softcap = a->softcap, f.alibi = a->alibi, f.kd = f.vd = 1.0f;
+        f.wl = a->wl, f.wr = a->wr, f.varlen = 1, f.q_dtype = a->q_dtype;
+        f.rows_total = (uint64_t)a->total_q * a->hq;
+        g.pool = p.pool;
+        g.table = a->table, g.kv_len = a->kv_len, g.status = a->status, g.table_stride = a->table_stride, g.table_cols = a->table_cols;
+        g.o_ss = a->out_strides[0], g.o_sh = a->out_strides[1], g.total_q = a->total_q;
+        const bool alike = (uint64_t)a->b * a->max_q == a->total_q;
+        g.row_cap = alike ? 0 : PA_ROWS;
+        pl.tiles = fa_paged_tiles_take(f, g, a->pool.dtype);
+        if (pl.tiles) {
+            f.n_splits = fa_paged_tiles_splits(f, g, (uint32_t)sms);
+            pl.steps = !alike;
+            p.row_cap = PA_ROWS;
+        }
+    }
     // no more blocks than there can be units
-    const uint64_t rows = (uint64_t)a->max_q * p.group, packs = (rows + PA_ROWS - 1) / PA_ROWS;
+    const uint64_t rows = pl.tiles ? PA_ROWS : (uint64_t)a->max_q * p.group, packs = (rows + PA_ROWS - 1) / PA_ROWS;
     const uint64_t most = std::max<uint64_t>((uint64_t)a->b * p.hkv * packs * ((p.max_k + pl.unit - 1) / pl.unit + 1), 1);
     p.blocks = (uint32_t)std::min<uint64_t>((uint64_t)sms * (pl.hd == 256 ? 1 : 2), most);
     p.min_units = 1;
     const size_t part_o = (size_t)2 * p.blocks * PA_ROWS * p.d * 4;
     pl.off_ml = (part_o + 255) / 256 * 256;
-    pl.ws_bytes = p.blocks > 1 ? pl.off_ml + (size_t)2 * p.blocks * PA_ROWS * 8 : 0;
+    pl.ws_bytes = pl.steps && p.blocks > 1 ? pl.off_ml + (size_t)2 * p.blocks * PA_ROWS * 8 : 0;
+    if (pl.tiles && pl.fa.n_splits > 1) {
+        pl.off_split = (pl.ws_bytes + 255) / 256 * 256;
+        pl.off_lse = pl.off_split + (pl.fa.n_splits * pl.fa.rows_total * p.d * 4 + 255) / 256 * 256;
+        pl.ws_bytes = pl.off_lse + pl.fa.n_splits * pl.fa.rows_total * 4;
+    }
     return B200_OK;
 }
 
@@ -759,30 +809,65 @@ static int pa_kind(const PaPlan &pl, cudaStream_t stream) {
     }
 }
 
+static int pa_steps(const PaPlan &pl, cudaStream_t stream) {
+    if (pl.hd == 64) return pa_kind<64>(pl, stream);
+    if (pl.hd == 128) return pa_kind<128>(pl, stream);
+    return pa_kind<256>(pl, stream);
+}
+static int pa_tiles(const PaPlan &pl, int pool_dtype, cudaStream_t stream) {
+    int rc = fa_paged_tiles_launch(pl.fa, pl.pg, pool_dtype, stream);
+    if (rc || pl.fa.n_splits == 1) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<uint64_t>((pl.fa.rows_total + 3) / 4, 148ull * 16));
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, pl.kind & 1 ? paged_split_join<true> : paged_split_join<false>, pl.p, pl.pg.row_cap, (const float *)pl.fa.part_o,
+                                             (const float *)pl.fa.part_lse, pl.fa.n_splits);
+    if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention (split join): %s", cudaGetErrorString(e));
+    return check_launch("paged_attention (split join)");
+}
+
 }  // namespace b200
 
 using namespace b200;
 
 extern "C" size_t b200_paged_attention_workspace_bytes(const B200PagedAttnArgs *a) {
     PaPlan pl;
-    return pa_plan(a, pl) ? 0 : pl.ws_bytes;
+    if (pa_plan(a, pl)) return 0;
+    const size_t need = pl.ws_bytes;
+    if (!pl.tiles) return need;
+    pa_plan(a, pl, false);  // should the driver refuse a tensor map
+    return std::max(need, pl.ws_bytes);
 }
 
 extern "C" int b200_paged_attention(const B200PagedAttnArgs *a, b200_stream_t stream_) {
     PaPlan pl;
-    const int rc = pa_plan(a, pl);
+    int rc = pa_plan(a, pl);
     if (rc) return rc;
     if (a->b == 0 || a->total_q == 0 || a->max_q == 0) return B200_OK;
     if (!a->q || !a->out || !a->cu_q || !a->kv_len || !a->table) return set_error(B200_ERR_BAD_ARG, "paged_attention: null pointer");
-    if (pl.ws_bytes) {
-        if (!a->workspace || a->workspace_bytes < pl.ws_bytes)
-            return set_error(B200_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes needed, %zu given", pl.ws_bytes, a->workspace ? a->workspace_bytes : (size_t)0);
-        if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return set_error(B200_ERR_BAD_ARG, "paged_attention: workspace must be 16-byte aligned");
-        pl.p.part_o = static_cast<float *>(a->workspace);
-        pl.p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(a->workspace) + pl.off_ml);
-    }
     cudaStream_t stream = (cudaStream_t)stream_;
-    if (pl.hd == 64) return pa_kind<64>(pl, stream);
-    if (pl.hd == 128) return pa_kind<128>(pl, stream);
-    return pa_kind<256>(pl, stream);
+    for (int attempt = 0; attempt < 2; ++attempt) {
+        if (pl.ws_bytes) {
+            if (!a->workspace || a->workspace_bytes < pl.ws_bytes)
+                return set_error(B200_ERR_WORKSPACE, "paged_attention: workspace of %zu bytes needed, %zu given", pl.ws_bytes, a->workspace ? a->workspace_bytes : (size_t)0);
+            if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return set_error(B200_ERR_BAD_ARG, "paged_attention: workspace must be 16-byte aligned");
+            char *ws = static_cast<char *>(a->workspace);
+            pl.p.part_o = reinterpret_cast<float *>(ws);
+            pl.p.part_ml = reinterpret_cast<float2 *>(ws + pl.off_ml);
+            pl.fa.part_o = reinterpret_cast<float *>(ws + pl.off_split);
+            pl.fa.part_lse = reinterpret_cast<float *>(ws + pl.off_lse);
+        }
+        rc = pl.tiles ? pa_tiles(pl, a->pool.dtype, stream) : B200_OK;
+        if (rc != FA_NO_MAP) return rc || !pl.steps ? rc : pa_steps(pl, stream);
+        // the driver refuses a tensor map of this call's tensors: nothing has been launched
+        rc = pa_plan(a, pl, false);
+        if (rc) return rc;
+    }
+    return rc;
 }

@@ -330,19 +330,6 @@ struct UnpackParams {
     int32_t *status;
 };
 
-// the sequence of packed row t: the last i with cu[i] <= t among 0 .. b - 1 (a warp at once, 32 probes a step)
-__device__ __forceinline__ uint32_t seq_of(const uint32_t *cu, uint32_t b, uint64_t t, int lane) {
-    uint32_t lo = 0, n = b;  // the answer is in [lo, lo + n)
-    while (n > 1) {
-        const uint32_t step = (n + 31) / 32, at = lo + lane * step;
-        const uint32_t hit = __ballot_sync(0xffffffffu, (uint32_t)lane * step < n && cu[at] <= t);
-        const uint32_t last = hit ? 31 - __clz(hit) : 0;  // (cu ascends)
-        lo += last * step;
-        n = min(step, n - last * step);
-    }
-    return lo;
-}
-
 template <int DT, int POOL, int PDT, int LPR>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const UnpackParams p) {
     constexpr int RPW = 32 / LPR;
@@ -351,7 +338,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const Unpac
     const uint32_t part = (uint32_t)(unit % p.parts);
     const PoolParams &pl = p.pool;
     if (t >= p.total || t >= p.cu[p.b]) return;
-    const uint32_t seq = seq_of(p.cu, p.b, t, lane), j = (uint32_t)(t - p.cu[seq]);
+    const uint32_t seq = pool_seq(p.cu, p.b, t, lane), j = (uint32_t)(t - p.cu[seq]);
     const uint32_t page = pool_div(j, pl.div_mul, pl.div_shr), row = j - page * pl.block_rows;
     const int id = page < p.table_cols ? p.table[seq * p.table_stride + page] : -1;
     const bool there = id >= 0 && (uint32_t)id < pl.n_blocks, in = (uint32_t)c * 8 < pl.d;

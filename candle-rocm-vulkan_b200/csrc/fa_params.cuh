@@ -56,6 +56,9 @@ struct FaPages {
     uint32_t g_mul, g_shr;  // n / group
     uint32_t box;           // rows of a page that are copied at a time
 };
+// Tensor maps of a pool's K and V: boxes of 128-byte columns (64 where a row of codes is no longer) x `rows` rows of a page, swizzled over that
+// width; what lies past the head dim or outside the pool reads as zeros. `order` as in fa_kv_maps. k == null: only whether maps can describe them.
+bool fa_pool_maps(const PoolParams &pl, int pool_dtype, bool bf16, uint32_t rows, CUtensorMap_st *k, CUtensorMap_st *v, uint32_t *order);
 // whether the tiles take the call, and in how many key splits (part_o and part_lse, [splits][token x head], for paged_split_join)
 bool fa_paged_tiles_take(const FaParams &p, FaPages &pg, int pool_dtype);
 uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sms);

@@ -2158,18 +2158,34 @@ static int fa_prefill_tma_launch(const FaParams &p, cudaStream_t stream) {
 
 // ---- the tiles over pages ------------------------------------------------------------------------------------------------
 // A pool's K or V as a map sees it: (block, row, head, d) as (batch, key, head, d).
-static bool pool_dims(const FaPages &pg, bool v, uint64_t es, KvDims *m) {
-    const PoolParams &pl = pg.pool;
+static bool pool_dims(const PoolParams &pl, bool v, uint64_t es, KvDims *m) {
     return kv_dims(m, v ? pl.v : pl.k, pl.n_blocks, pl.hkv, pl.block_rows, pl.d, (v ? pl.v_sb : pl.k_sb) / es, (v ? pl.v_sh : pl.k_sh) / es, (v ? pl.v_sr : pl.k_sr) / es, es);
+}
+bool fa_pool_maps(const PoolParams &pl, int pool_dtype, bool bf16, uint32_t rows, CUtensorMap *tm_k, CUtensorMap *tm_v, uint32_t *order) {
+    const bool mx = pool_dtype == B200_FP8, narrow = mx && pl.d <= 64;
+    const EncodeTiledFn enc = encode_tiled_fn();
+    for (int x = 0; x < 2; ++x) {
+        KvDims m;
+        if (!pool_dims(pl, x, mx ? 1 : 2, &m)) return false;
+        if (!tm_k) continue;
+        const cuuint64_t dims[4] = {(cuuint64_t)pl.d, m.size[0], m.size[1], m.size[2]}, strides[3] = {m.stride[0], m.stride[1], m.stride[2]};
+        cuuint32_t box[4] = {(cuuint32_t)(mx && !narrow ? 128 : 64), 1, 1, 1};
+        box[1 + ((m.order >> 2) & 3u)] = rows;
+        const cuuint32_t estr[4] = {1, 1, 1, 1};
+        if (!enc || enc(x ? tm_v : tm_k, mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : (bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16), 4, x ? pl.v : pl.k, dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, mx ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+        *order = x ? *order | m.order << 8 : m.order;
+    }
+    return true;
 }
 bool fa_paged_tiles_take(const FaParams &p, FaPages &pg, int pool_dtype) {
     // pages in whole groups of eight rows, what the 128-byte swizzle repeats after; smaller ones stay on mma.sync
     uint32_t box = 128;
     while (pg.pool.block_rows % box) box /= 2;
     if (box < 8 || p.d > 128 || p.softcap > 0.0f || p.alibi != nullptr || !(p.scale > 0.0f) || p.group > P3_ROWS) return false;
-    const uint64_t es = pool_dtype == B200_FP8 ? 1 : 2;
-    KvDims k, v;
-    if (!pool_dims(pg, false, es, &k) || !pool_dims(pg, true, es, &v)) return false;
+    if (!fa_pool_maps(pg.pool, pool_dtype, false, box, nullptr, nullptr, nullptr)) return false;
     const uint64_t row = (uint64_t)p.d * 2;
     if (p.q_sh * 2 >= (1ull << 40) / p.hq || p.q_ss * 2 >= (1ull << 40) || (p.hq > 1 && p.q_sh * 2 < row) || (pg.total_q > 1 && p.q_ss * 2 < row)) return false;
     pg.box = box;
@@ -2197,35 +2213,20 @@ static int fa_paged_launch_as(const FaParams &p, const FaPages &pg, const P3Grid
 }
 int fa_paged_tiles_launch(const FaParams &p, const FaPages &pg, int pool_dtype, cudaStream_t stream) {
     const bool mx = pool_dtype == B200_FP8, bf16 = p.q_dtype == B200_BF16;
-    const uint64_t es = mx ? 1 : 2, items = paged_items(p, pg) * p.n_splits;
-    KvDims k, v;
-    const EncodeTiledFn enc = encode_tiled_fn();
-    if (!enc || items >= (1ull << 31) || !pool_dims(pg, false, es, &k) || !pool_dims(pg, true, es, &v)) return FA_NO_MAP;
-    const CUtensorMapDataType t16 = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const uint64_t items = paged_items(p, pg) * p.n_splits;
     CUtensorMap tm_k, tm_v, tm_q;
-    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-    for (int x = 0; x < 2; ++x) {
-        const KvDims &m = x ? v : k;
-        const cuuint64_t dims[4] = {(cuuint64_t)p.d, m.size[0], m.size[1], m.size[2]}, strides[3] = {m.stride[0], m.stride[1], m.stride[2]};
-        const bool narrow = mx && p.d <= 64;  // a row of codes in 64 bytes
-        cuuint32_t box[4] = {(cuuint32_t)(mx ? (narrow ? 64 : 128) : 64), 1, 1, 1};
-        box[1 + ((m.order >> 2) & 3u)] = pg.box;
-        if (enc(x ? &tm_v : &tm_k, mx ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : t16, 4, x ? pg.pool.v : pg.pool.k, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return FA_NO_MAP;
-    }
+    P3Grid gr = {};
+    if (items >= (1ull << 31) || !fa_pool_maps(pg.pool, pool_dtype, bf16, pg.box, &tm_k, &tm_v, &gr.tm_order)) return FA_NO_MAP;
     {
         const uint64_t G = p.group, row = ((uint64_t)p.d * 2 + 15) / 16 * 16;
         const cuuint64_t strides[4] = {p.hq > 1 ? p.q_sh * 2 : row, p.hkv > 1 ? G * p.q_sh * 2 : row, pg.total_q > 1 ? p.q_ss * 2 : row, row};
         const cuuint64_t dims[5] = {(cuuint64_t)p.d, G, p.hkv, pg.total_q, 1};
-        const cuuint32_t box[5] = {64, (cuuint32_t)G, 1, (cuuint32_t)(P3_ROWS / G), 1};
-        if (enc(&tm_q, t16, 5, const_cast<void *>(p.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+        const cuuint32_t box[5] = {64, (cuuint32_t)G, 1, (cuuint32_t)(P3_ROWS / G), 1}, estr[5] = {1, 1, 1, 1, 1};
+        if (encode_tiled_fn()(&tm_q, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void *>(p.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return FA_NO_MAP;
     }
-    P3Grid gr = {};
     gr.items = (uint32_t)items;
-    gr.tm_order = k.order | (v.order << 8);
     gr.lag = p.d > 64 && (uint64_t)p.lq * p.group >= 512 ? PF_SLACK : 0.0f;  // as in fa_prefill_tma_launch
 #define B200_PAGED(HD, BF16) (mx ? fa_paged_launch_as<HD, BF16, 2>(p, pg, gr, tm_k, tm_v, tm_q, stream) : fa_paged_launch_as<HD, BF16, 1>(p, pg, gr, tm_k, tm_v, tm_q, stream))
     if (p.d <= 64) return bf16 ? B200_PAGED(64, true) : B200_PAGED(64, false);
@@ -2266,13 +2267,15 @@ using namespace b200;
 namespace b200 {
 int decode_wait_status();  // tq_decode.cu: the same flag of the kernels over packed rows
 int decode_wait_clear();
+int paged_wait_status();  // paged_attn.cu
+int paged_wait_clear();
 }
 extern "C" int b200_device_wait_status(void) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_wait_failed, sizeof(int)) != cudaSuccess) return -1;
-    const int d = b200::decode_wait_status(), f = b200::fa_decode_wait_status();
-    if (d < 0 || f < 0) return -1;
-    return (v != 0 || d != 0 || f != 0) ? 1 : 0;
+    const int d = b200::decode_wait_status(), f = b200::fa_decode_wait_status(), g = b200::paged_wait_status();
+    if (d < 0 || f < 0 || g < 0) return -1;
+    return (v != 0 || d != 0 || f != 0 || g != 0) ? 1 : 0;
 }
 
 // B200_ERR_DEVICE_WAIT when a bounded device-side wait has run out on the current device since the library was loaded
@@ -2283,7 +2286,8 @@ extern "C" int b200_device_wait_check(int clear) {
     if (st < 0) return set_error(B200_ERR_LAUNCH, "device_wait_check: the flag cannot be read (%s)", cudaGetErrorString(cudaGetLastError()));
     if (clear) {
         const int zero = 0;
-        if (cudaMemcpyToSymbol(g_wait_failed, &zero, sizeof(int)) != cudaSuccess || b200::decode_wait_clear() != 0 || b200::fa_decode_wait_clear() != 0)
+        if (cudaMemcpyToSymbol(g_wait_failed, &zero, sizeof(int)) != cudaSuccess || b200::decode_wait_clear() != 0 || b200::fa_decode_wait_clear() != 0 ||
+            b200::paged_wait_clear() != 0)
             return set_error(B200_ERR_LAUNCH, "device_wait_check: the flag cannot be cleared");
     }
     if (st) return set_error(B200_ERR_DEVICE_WAIT, "a bounded device-side wait ran out: the outputs of the call that met it are incomplete");

@@ -30,14 +30,20 @@ __device__ __forceinline__ uint32_t pool_mul2(uint32_t a, uint32_t b) {
     return d;
 }
 // E4M3 codes as pairs of values: f16, or bf16 times 2^-120 (a code's exponent and mantissa in the places of a bf16's, its subnormals
-// among that type's). pool_codes: byte I of two words; pool_pair: bytes 2 I and 2 I + 1 of one.
-template <bool BF16, int I>
-__device__ __forceinline__ uint32_t pool_codes(uint32_t lo, uint32_t hi) {
+// among that type's). pool_codes4: the bytes of two words, pair by pair; pool_pair: bytes 2 I and 2 I + 1 of one.
+template <bool BF16>
+__device__ __forceinline__ void pool_codes4(uint32_t lo, uint32_t hi, uint32_t (&x)[4]) {
     if (BF16) {
-        const uint32_t t = __byte_perm(lo, hi, (4u + I) << 12 | I << 4);
-        return (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = __byte_perm(lo, hi, (4u + i) << 12 | i << 4);
+            x[i] = (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+        }
+    } else {
+        const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);
+        x[0] = cvt_e4m3x2_f16x2(a), x[1] = cvt_e4m3x2_hi_f16x2(a);
+        x[2] = cvt_e4m3x2_f16x2(b), x[3] = cvt_e4m3x2_hi_f16x2(b);
     }
-    return cvt_e4m3x2_f16x2(__byte_perm(lo, hi, (4u + I) << 4 | I));
 }
 template <bool BF16, int I>
 __device__ __forceinline__ uint32_t pool_pair(uint32_t w) {

@@ -3,20 +3,24 @@
 // token t sees, in one pass with a running maximum and sum.
 //
 // Sequences with few packed query rows (token x head of the group) are bound by memory: every key and value is read once for at
-// most 16 rows. The batch is ragged and only the device knows its lengths, so the work is divided there: a column is 16 rows of
-// one kv head, a unit is what a block's four warps score at a time (64 or 128 keys), and the units of all columns, one behind the other,
-// are cut into equal shares, one per block (two blocks per SM). A block that holds all of a column writes its rows; parts of
-// columns go to the workspace, two at most per block (where its share begins and where it ends), and a second grid joins
-// them: it has a block per border between shares, and the first border inside a column belongs to that column.
+// most 16 rows. The batch is ragged and only the device knows its lengths, so the work is divided there: a column is 16 rows of a
+// sequence, a unit is what a block's four warps score at a time (64 or 128 keys), and the units of all columns, one behind the
+// other, are cut into equal shares. Every kv head has the same shares, and blocks of neighbouring heads run side by side (two
+// blocks per SM): in a page the heads' rows of a key lie next to one another, so they are read at about the same time. A block that holds all of
+// a column writes its rows; parts of columns go to the workspace, two at most per block (where its share begins and
+// where it ends), and a second grid joins them: it has a block per head and border between shares, and the first border
+// inside a column belongs to that column.
 // In a block each warp has keys of its own, K and V in a ring of stages that it fills ahead of the column it is working on,
 // across columns too; scores and sums run on mma.sync m16n8k16, and the warps' partial results meet in shared memory at a
 // column's end.
 //
 // MXFP8 keys and values stay codes up to the registers. Scores: the codes are exact in f16; q is taken to f16 behind a power of
 // two per row (a bf16 element keeps its eight bits unless it is 2^28 below the row's largest), and a block of 32 elements adds its
-// sum times its scale in f32. Values: the codes times their power of two in q's type, which holds the product exactly unless it leaves
-// that type's range; weights are rounded to q's type, as for 16-bit pools (2^-9 or 2^-12 each, and they average out).
+// sum times its scale in f32. Values and weights: see the products. Weights are rounded to 16 bits (f16 2^-11, bf16 2^-8 at most each, and these
+// average out), as for 16-bit pools.
 #include <algorithm>
+#include <cuda.h>
+#include <type_traits>
 
 #include "fa_params.cuh"
 
@@ -35,12 +39,12 @@ struct PaParams {
     PoolParams pool;
     const float *alibi;
     int32_t *status;
-    float *part_o;    // [2 x blocks][16][d]
-    float2 *part_ml;  // [2 x blocks][16]: maximum (log 2), sum
+    float *part_o;    // [blocks][2][16][d]
+    float2 *part_ml;  // [blocks][2][16]: maximum (log 2), sum
     uint32_t b, hq, hkv, group, d, total_q, max_q, max_k, table_cols, alibi_bs;
     float scale, softcap;
     int32_t wl, wr;
-    uint32_t blocks, min_units;
+    uint32_t shares;  // per kv head; blocks = shares x hkv
     uint32_t row_cap;  // sequences of more packed rows are on the tcgen05 tiles; 0: all are here
 };
 
@@ -54,8 +58,10 @@ struct PA {
     static constexpr uint32_t TILE = KEYS * RB, STAGE = 2 * TILE;        // K, V
     static constexpr uint32_t SC = MX ? 2 * KEYS * NB : 0;               // scales of a stage
     static constexpr int NS = HD == 256 && !MX ? 2 : 3;
-    static constexpr int MROW = HD / 2 + 2;                              // floats per row of the merge: half a row, maximum, sum
-    static constexpr uint32_t SM_SC = PA_WARPS * NS * STAGE, SM_MERGE = SM_SC + PA_WARPS * NS * SC, SMEM = SM_MERGE + PA_WARPS * PA_ROWS * MROW * 4;
+    static constexpr int COLS = RB < 128 ? 1 : RB / 128, COL_B = RB < 128 ? 64 : 128;  // columns of a tile and their bytes per row
+    static constexpr int PARTS = HD == 128 && MX ? 4 : 2;                // pieces of a row that the warps' merge takes in turn (two blocks fit an SM)
+    static constexpr int PIECE = HD / PARTS, MROW = PIECE + 2;           // floats per row: a piece, maximum, sum
+    static constexpr uint32_t SM_SC = PA_WARPS * NS * STAGE, SM_MERGE = SM_SC + PA_WARPS * NS * SC, SM_BAR = SM_MERGE + PA_WARPS * PA_ROWS * MROW * 4, SMEM = SM_BAR + PA_WARPS * NS * 8;
     // 16-byte chunk ch of row r of a tile, in 128-byte columns (64 where a row is no longer), swizzled
     __device__ static __forceinline__ uint32_t at(int r, int ch) {
         if (RB == 64) return r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
@@ -74,7 +80,7 @@ __device__ __forceinline__ void pa_range(const PaParams &p, const PaSeq &s, uint
     hi = p.wr >= 0 && pos < s.lk - p.wr - 1 ? pos + p.wr + 1 : s.lk;
     hi = max(hi, lo);
 }
-// the sequence's units
+// the sequence's units (of one head)
 __device__ __forceinline__ uint64_t pa_seq(const PaParams &p, uint32_t b, int unit, PaSeq &s) {
     s.q0 = min(p.cu_q[b], p.total_q);
     const uint32_t end = min(p.cu_q[b + 1], p.total_q);
@@ -89,7 +95,7 @@ __device__ __forceinline__ uint64_t pa_seq(const PaParams &p, uint32_t b, int un
     pa_range(p, s, s.rows - 1, x, hi);
     s.ulo = lo / unit;
     s.uhi = hi > lo ? (hi + unit - 1) / unit : s.ulo + 1;  // rows that see nothing still have zeros to write
-    return (uint64_t)(uint32_t)(s.uhi - s.ulo) * s.packs * p.hkv;
+    return (uint64_t)(uint32_t)(s.uhi - s.ulo) * s.packs;
 }
 
 // Where the block (all of its threads; a multiple of 32, 256 at most) finds unit `target(total)` of all: the sequence and the unit
@@ -121,7 +127,7 @@ __device__ __forceinline__ PaPlace pa_place(const PaParams &p, int unit, uint64_
         if (w < warp) before += s_sum[w];
         at.total += s_sum[w];
     }
-    at.per = max((at.total + p.blocks - 1) / p.blocks, (uint64_t)p.min_units);
+    at.per = (at.total + p.shares - 1) / p.shares;
     const uint64_t want = target(at.per);
     if (want >= before && want < before + sum) {
         uint64_t rest = want - before;
@@ -144,22 +150,30 @@ __device__ __forceinline__ PaPlace pa_place(const PaParams &p, int unit, uint64_
 // a unit of a column of a sequence, and the way to the next one
 struct PaCursor {
     PaSeq s;
-    uint32_t seq, col;  // col = head x packs + pack
-    int u;
+    uint32_t seq, pack;
+    int u, lo, hi;  // the unit; the keys that some row of the column sees
+    __device__ __forceinline__ void enter(const PaParams &p) {
+        int x;
+        pa_range(p, s, pack * PA_ROWS, lo, x);
+        pa_range(p, s, min(pack * PA_ROWS + PA_ROWS, s.rows) - 1, x, hi);
+    }
     __device__ __forceinline__ void start(const PaParams &p, int unit, uint32_t seq_, uint64_t off) {
         seq = seq_;
         pa_seq(p, seq, unit, s);
         const uint32_t n = (uint32_t)(s.uhi - s.ulo);
-        col = (uint32_t)(off / n);
-        u = s.ulo + (int)(off - (uint64_t)col * n);
+        pack = (uint32_t)(off / n);
+        u = s.ulo + (int)(off - (uint64_t)pack * n);
+        enter(p);
     }
-    __device__ __forceinline__ void next(const PaParams &p, int unit) {
-        if (++u < s.uhi) return;
-        if (++col == s.packs * p.hkv) {
-            col = 0;
+    __device__ __forceinline__ bool next(const PaParams &p, int unit) {  // true: another column
+        if (++u < s.uhi) return false;
+        if (++pack == s.packs) {
+            pack = 0;
             while (++seq < p.b && pa_seq(p, seq, unit, s) == 0) {}
         }
         u = s.ulo;
+        if (seq < p.b) enter(p);
+        return true;
     }
 };
 
@@ -195,8 +209,12 @@ __device__ __forceinline__ uint32_t pa_pack2(float lo, float hi) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
-template <int HD, int KIND>
-__global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_kernel(const PaParams p) {
+__device__ int g_paged_wait_failed = 0;  // a bounded wait for copies ran out
+
+// TMA: tiles by tensor copies (pages of whole groups of `box` rows), else by 16-byte chunks, each lane for itself
+template <int HD, int KIND, bool TMA>
+__global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_kernel(const PaParams p, const __grid_constant__ CUtensorMap tm_k,
+                                                                                     const __grid_constant__ CUtensorMap tm_v, const uint32_t tm_order, const uint32_t box) {
     using C = PA<HD, KIND>;
     constexpr bool MX = C::MX, BF16 = C::BF16;
     constexpr int KSTEPS = HD / 16, NT = HD / 8, KEYS = C::KEYS, KG = KEYS / 16, UNIT = C::UNIT;
@@ -204,11 +222,18 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * C::NS * C::STAGE, scales = smem_u32(smem) + C::SM_SC + warp * C::NS * C::SC;
     float *const mg = reinterpret_cast<float *>(smem + C::SM_MERGE);
-    if (p.blocks > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining grid may get ready
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(smem + C::SM_BAR) + warp * C::NS;
+    if (TMA && lane == 0) {
+        for (int i = 0; i < C::NS; ++i) mbar_init(&bars[i], 1);
+        mbar_fence_init();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (p.shares > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining grid may get ready
     const PoolParams &pl = p.pool;
+    const uint32_t share = blockIdx.x / p.hkv, hk = blockIdx.x - share * p.hkv;
 
-    const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return blockIdx.x * per; });
-    const uint64_t u0 = blockIdx.x * place.per;
+    const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return share * per; });
+    const uint64_t u0 = share * place.per;
     if (u0 >= place.total) return;
     const int nu = (int)min(place.per, place.total - u0);
     PaCursor cur, lead;  // the unit being worked on, and the one to be asked for next
@@ -218,11 +243,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     // A warp's keys of the lead's unit into stage st: lane i finds key i's row, then C::CPR lanes copy a row. What no row of the column
     // sees, and what a page outside the pool would hold, is zeros.
     auto request = [&](int st) {
-        const uint32_t hk = lead.col / lead.s.packs, pack = lead.col - hk * lead.s.packs, r0 = pack * PA_ROWS;
-        int lo, hi, x;
-        pa_range(p, lead.s, r0, lo, x);
-        pa_range(p, lead.s, min(r0 + PA_ROWS, lead.s.rows) - 1, x, hi);
-        const int j = lead.u * UNIT + warp * KEYS + lane;
+        const int lo = lead.lo, hi = lead.hi, j = lead.u * UNIT + warp * KEYS + lane;
         const char *kr = nullptr, *vr = nullptr;
         uint64_t srow = 0;
         if (lane < KEYS && j >= lo && j < hi) {
@@ -258,13 +279,83 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
             }
         }
     };
-    for (int t = 0; t < C::NS; ++t) {
-        if (t < nu) {
-            request(t);
-            lead.next(p, UNIT);
+    // TMA. The page of rows i x box .. of the warp's keys in the lead's unit, in lane i (-1: no row of the column sees any of them; -2: no page of
+    // the pool, whose copy brings zeros); asked for one unit ahead, since the copies cannot leave without it.
+    int ahead_row = 0;
+    auto page_of = [&]() {
+        const int j = lead.u * UNIT + warp * KEYS + lane * (int)box;
+        ahead_row = 0;
+        if (lane * (int)box >= KEYS || j >= lead.hi || j + (int)box <= lead.lo) return -1;
+        const uint32_t page = pool_div((uint32_t)j, pl.div_mul, pl.div_shr);
+        ahead_row = j - (int)(page * pl.block_rows);
+        const int id = page < p.table_cols ? p.table[lead.seq * p.table_stride + page] : -1;
+        return id >= 0 && (uint32_t)id < pl.n_blocks ? id : -2;
+    };
+    // copies of the lead's unit into stage st; false: nobody sees any of the warp's keys, nothing comes
+    auto copy = [&](int st, int id, int row) {
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, id != -1));
+        if (n == 0) return false;
+        const uint32_t bar = smem_u32(&bars[st]), good = MX ? __popc(__ballot_sync(0xffffffffu, id >= 0)) : 0u;
+        if (lane == 0) mbar_expect_tx(&bars[st], n * box * 2 * C::RB + good * box * 2 * C::NB);
+        __syncwarp();
+        if (id != -1) {
+            const uint32_t dst = ring + st * C::STAGE + lane * box * C::COL_B;
+            const int blk = id < 0 ? (int)pl.n_blocks : id;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const uint32_t ord = kv ? tm_order >> 8 : tm_order, ph = ord & 3u, pk = (ord >> 2) & 3u;
+                const int c1 = ph == 0 ? (int)hk : (pk == 0 ? row : blk), c2 = ph == 1 ? (int)hk : (pk == 1 ? row : blk), c3 = ph == 2 ? (int)hk : (pk == 2 ? row : blk);
+#pragma unroll
+                for (int i = 0; i < C::COLS; ++i)
+                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+                                     dst + kv * C::TILE + i * (KEYS * 128)),
+                                 "l"(reinterpret_cast<uint64_t>(kv ? &tm_v : &tm_k)), "r"((MX ? 128 : 64) * i), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+                                 : "memory");
+            }
+            if (MX) {
+                uint8_t *const at = smem + C::SM_SC + (warp * C::NS + st) * C::SC + lane * box * C::NB;
+                if (id >= 0) {
+                    const uint64_t from = (((uint64_t)id * pl.hkv + hk) * pl.block_rows + row) * C::NB;
+                    bulk_g2s(at, pl.ks + from, box * C::NB, &bars[st]);
+                    bulk_g2s(at + KEYS * C::NB, pl.vs + from, box * C::NB, &bars[st]);
+                } else {
+                    if (p.status) atomicExch(p.status, 3);
+                    for (uint32_t i = 0; i < box * C::NB; ++i) at[i] = at[KEYS * C::NB + i] = 127;  // zeros times one
+                }
+            } else if (id < 0 && p.status) {
+                atomicExch(p.status, 3);
+            }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        return true;
+    };
+    uint32_t sent = 0, phase = 0;  // a bit per stage: copies are on their way; the parity that its barrier shows when they have landed
+    int ahead = -1;
+    if (TMA) {
+        int ids[C::NS + 1], rows[C::NS + 1];  // all lookups before the first copy
+#pragma unroll
+        for (int t = 0; t <= C::NS; ++t) {
+            ids[t] = t < nu ? page_of() : -1;
+            rows[t] = ahead_row;
+            if (t < nu - 1) lead.next(p, UNIT);
+        }
+        ahead = ids[C::NS];
+        lead = cur;
+#pragma unroll
+        for (int t = 0; t < C::NS; ++t)
+            if (t < nu) {
+                if (copy(t, ids[t], rows[t])) sent |= 1u << t;
+                lead.next(p, UNIT);
+            }
+    } else {
+        for (int t = 0; t < C::NS; ++t) {
+            if (t < nu) {
+                request(t);
+                lead.next(p, UNIT);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
     }
+    bool ok = true;
 
     uint32_t qa[KSTEPS][4];
     float m[2], l[2], oacc[NT][4], sc[2], slope[2];
@@ -274,7 +365,6 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     int seg_u = 0;
     uint32_t seg = 0;  // the block's segments so far
     for (int t = 0; t < nu; ++t) {
-        const uint32_t hk = cur.col / cur.s.packs, pack = cur.col - hk * cur.s.packs, row0 = pack * PA_ROWS;
         if (begin) {
             // ---- a column: its rows of q as A fragments, their keys and scales
             begin = false;
@@ -283,7 +373,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
             for (int n = 0; n < NT; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t r = row0 + g + 8 * e;
+                const uint32_t r = cur.pack * PA_ROWS + g + 8 * e;
                 m[e] = -INFINITY, l[e] = 0.0f, slope[e] = 0.0f, sc[e] = p.scale;
                 r_lo[e] = 0, r_hi[e] = cur.s.lk, r_pos[e] = 0;  // rows that do not exist see every key and are never stored
                 const bool there = r < cur.s.rows;
@@ -335,11 +425,30 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                 }
             }
             int x;
-            pa_range(p, cur.s, min(row0 + PA_ROWS, cur.s.rows) - 1, lomax, x);
-            pa_range(p, cur.s, row0, x, himin);
+            pa_range(p, cur.s, min(cur.pack * PA_ROWS + PA_ROWS, cur.s.rows) - 1, lomax, x);
+            pa_range(p, cur.s, cur.pack * PA_ROWS, x, himin);
         }
         const int j0 = cur.u * UNIT + warp * KEYS, st = t % C::NS;
-        asm volatile("cp.async.wait_group %0;" ::"n"(C::NS - 1) : "memory");
+        bool dirty = false;
+        if (TMA) {
+            if (sent >> st & 1u) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars[st], phase >> st & 1u));
+                phase ^= 1u << st;
+            }
+            // values that no row of the column sees (rows of the page behind the last key, in front of a window; what was not copied)
+            if (j0 < cur.lo || j0 + KEYS > cur.hi) {
+                dirty = true;
+                for (int i = lane; i < KEYS * C::CPR; i += 32) {
+                    const int row = i / C::CPR;
+                    if (j0 + row >= cur.lo && j0 + row < cur.hi) continue;
+                    *reinterpret_cast<uint4 *>(smem + (warp * C::NS + st) * C::STAGE + C::TILE + C::at(row, i % C::CPR)) = make_uint4(0u, 0u, 0u, 0u);
+                    if (MX && i % C::CPR == 0)
+                        for (int k = 0; k < C::NB; ++k) smem[C::SM_SC + (warp * C::NS + st) * C::SC + (KEYS + row) * C::NB + k] = 127;
+                }
+            }
+        } else {
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::NS - 1) : "memory");
+        }
         __syncwarp();
         const uint32_t tk = ring + st * C::STAGE, tv = tk + C::TILE, tsc = scales + st * C::SC;
 
@@ -361,21 +470,26 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         } else {
             const uint32_t nb = p.d / 32;
 #pragma unroll
-            for (int n = 0; n < 2 * KG; ++n)
+            for (int n = 0; n < 2 * KG; ++n) {
+                uint2 sw = make_uint2(0u, 0u);
+                if (C::NB == 4) sw = pa_lds64(tsc + (8 * n + 2 * c) * 4);  // the scales of this lane's two keys
 #pragma unroll
                 for (int i = 0; i < C::NB; ++i) {
-                    if ((uint32_t)i >= nb) break;
+                    if (!TMA && (uint32_t)i >= nb) break;
                     const uint2 w = pa_lds64(tk + C::at(8 * n + g, 2 * i + (c >> 1)) + (c & 1) * 8);
                     float z[4];
                     const uint32_t(&q0)[4] = qa[2 * i], (&q1)[4] = qa[2 * i + 1];
                     mma_f16_16816_z(z, q0[0], q0[1], q0[2], q0[3], cvt_e4m3x2_f16x2(w.x), cvt_e4m3x2_hi_f16x2(w.x));
                     mma_f16_16816(z, q1[0], q1[1], q1[2], q1[3], cvt_e4m3x2_f16x2(w.y), cvt_e4m3x2_hi_f16x2(w.y));
-                    const float s0 = e8m0_to_f(pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i)), s1 = e8m0_to_f(pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i));
+                    // (the smallest scale, 2^-127, counts as nothing here)
+                    const float s0 = u2f(C::NB == 4 ? (i < 3 ? sw.x << (23 - 8 * (i & 3)) : sw.x >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i) << 23);
+                    const float s1 = u2f(C::NB == 4 ? (i < 3 ? sw.y << (23 - 8 * (i & 3)) : sw.y >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i) << 23);
                     s[n][0] = fmaf(z[0], s0, s[n][0]);
                     s[n][1] = fmaf(z[1], s1, s[n][1]);
                     s[n][2] = fmaf(z[2], s0, s[n][2]);
                     s[n][3] = fmaf(z[3], s1, s[n][3]);
                 }
+            }
         }
         const bool full = plain && j0 >= lomax && j0 + KEYS <= himin;
         float mx[2] = {-INFINITY, -INFINITY};
@@ -413,77 +527,111 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                 for (int n = 0; n < NT; ++n) oacc[n][2 * e] *= f, oacc[n][2 * e + 1] *= f;
             }
         }
-        const float ms0 = m[0] == -INFINITY ? 0.0f : m[0], ms1 = m[1] == -INFINITY ? 0.0f : m[1];
-        uint32_t pa[KG][4];
+        // weights up to 2^8, so that f16 holds those down to 2^-32 of the largest
+        const float ms0 = m[0] == -INFINITY ? 0.0f : m[0] - 8.0f, ms1 = m[1] == -INFINITY ? 0.0f : m[1] - 8.0f;
 #pragma unroll
         for (int n = 0; n < 2 * KG; ++n) {
-            const float p0 = fast_exp2(s[n][0] - ms0), p1 = fast_exp2(s[n][1] - ms0), p2 = fast_exp2(s[n][2] - ms1), p3 = fast_exp2(s[n][3] - ms1);
-            l[0] += p0 + p1;
-            l[1] += p2 + p3;
-            pa[n >> 1][(n & 1) * 2] = pa_pack2<BF16>(p0, p1);
-            pa[n >> 1][(n & 1) * 2 + 1] = pa_pack2<BF16>(p2, p3);
+            s[n][0] = fast_exp2(s[n][0] - ms0);
+            s[n][1] = fast_exp2(s[n][1] - ms0);
+            s[n][2] = fast_exp2(s[n][2] - ms1);
+            s[n][3] = fast_exp2(s[n][3] - ms1);
+            l[0] += s[n][0] + s[n][1];
+            l[1] += s[n][2] + s[n][3];
         }
         // ---- O += P V
+        auto weights = [&](auto bf, int kk, uint32_t(&pa)[4]) {
+            pa[0] = pa_pack2<bf.value>(s[2 * kk][0], s[2 * kk][1]);
+            pa[1] = pa_pack2<bf.value>(s[2 * kk][2], s[2 * kk][3]);
+            pa[2] = pa_pack2<bf.value>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+            pa[3] = pa_pack2<bf.value>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+        };
         if (!MX) {
             const uint32_t vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = lane >> 4;
 #pragma unroll
-            for (int kk = 0; kk < KG; ++kk)
+            for (int kk = 0; kk < KG; ++kk) {
+                uint32_t pa[4];
+                weights(std::bool_constant<BF16>{}, kk, pa);
 #pragma unroll
                 for (int np = 0; np < NT / 2; ++np) {
                     uint32_t b0, b1, b2, b3;
                     pa_ldsm_trans(tv + C::at(kk * 16 + vr, np * 2 + vc), b0, b1, b2, b3);
-                    pa_mma<BF16>(oacc[2 * np], pa[kk], b0, b1);
-                    pa_mma<BF16>(oacc[2 * np + 1], pa[kk], b2, b3);
+                    pa_mma<BF16>(oacc[2 * np], pa, b0, b1);
+                    pa_mma<BF16>(oacc[2 * np + 1], pa, b2, b3);
                 }
+            }
         } else {
-            // column n = g of the products' tile i is element g HD / 8 + i: a lane reads the same bytes of its four keys
+            // Column n = g of the products' tile i is element g HD / 8 + i: a lane reads the same bytes of its four keys. Values and weights in f16, also
+            // under bf16 queries (the codes times 2^k with k from -22 to 7 are within 2^-11 of a block's largest there, and weights have three bits
+            // more); tiles with scales outside that take the second form: two factors, and bf16 under bf16 queries.
             constexpr int W = HD / 32;  // words of a lane's elements
-            const uint32_t blk = g * (HD / 8) / 32, vsc = tsc + KEYS * C::NB + blk;
+            const uint32_t vsc = tsc + KEYS * C::NB + g * (HD / 8) / 32;
+            uint32_t e[KG][4], top = 0, low = 255;
 #pragma unroll
-            for (int kk = 0; kk < KG; ++kk) {
-                uint32_t e[4];
+            for (int kk = 0; kk < KG; ++kk)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) e[k] = pa_lds8(vsc + (kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8) * C::NB);
-                uint32_t rest0, rest1;
-                const uint32_t f0 = pool_scale2<BF16>(e[0], e[1], rest0), f1 = pool_scale2<BF16>(e[2], e[3], rest1);
-                const uint32_t top = max(max(e[0], e[1]), max(e[2], e[3])), low = min(min(e[0], e[1]), min(e[2], e[3]));
-                const bool far = __any_sync(0xffffffffu, BF16 ? top > 134u : low < 103u);
+                for (int k = 0; k < 4; ++k) {
+                    e[kk][k] = pa_lds8(vsc + (kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8) * C::NB);
+                    top = max(top, e[kk][k]);
+                    low = min(low, e[kk][k]);
+                }
+            auto products = [&](auto bf, auto far) {
+                constexpr bool B = bf.value, FAR = far.value;
 #pragma unroll
-                for (int i = 0; i < W; i += 2) {
-                    uint32_t w[4][2];
+                for (int kk = 0; kk < KG; ++kk) {
+                    uint32_t pa[4], f[2], rest[2];
+                    weights(bf, kk, pa);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint2 v = pa_lds64(tv + C::at(kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8, (g * W + i) >> 2) + ((g * W + i) & 3) * 4);
-                        w[k][0] = v.x, w[k][1] = v.y;
-                    }
+                    for (int k = 0; k < 2; ++k) f[k] = pool_scale2<B>(e[kk][2 * k], e[kk][2 * k + 1], rest[k]);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t b0[4] = {pool_codes<BF16, 0>(w[0][x], w[1][x]), pool_codes<BF16, 1>(w[0][x], w[1][x]), pool_codes<BF16, 2>(w[0][x], w[1][x]),
-                                          pool_codes<BF16, 3>(w[0][x], w[1][x])};
-                        uint32_t b1[4] = {pool_codes<BF16, 0>(w[2][x], w[3][x]), pool_codes<BF16, 1>(w[2][x], w[3][x]), pool_codes<BF16, 2>(w[2][x], w[3][x]),
-                                          pool_codes<BF16, 3>(w[2][x], w[3][x])};
+                    for (int i = 0; i < W; i += 2) {
+                        uint32_t w[4][2];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            b0[y] = pool_mul2<BF16>(b0[y], f0);
-                            b1[y] = pool_mul2<BF16>(b1[y], f1);
-                            if (far) b0[y] = pool_mul2<BF16>(b0[y], rest0), b1[y] = pool_mul2<BF16>(b1[y], rest1);
-                            pa_mma<BF16>(oacc[(i + x) * 4 + y], pa[kk], b0[y], b1[y]);
+                        for (int k = 0; k < 4; ++k) {
+                            const uint2 v = pa_lds64(tv + C::at(kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8, (g * W + i) >> 2) + ((g * W + i) & 3) * 4);
+                            w[k][0] = v.x, w[k][1] = v.y;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t b[2][4];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                pool_codes4<B>(w[2 * k][x], w[2 * k + 1][x], b[k]);
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) {
+                                    b[k][y] = pool_mul2<B>(b[k][y], f[k]);
+                                    if (FAR) b[k][y] = pool_mul2<B>(b[k][y], rest[k]);
+                                }
+                            }
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) pa_mma<B>(oacc[(i + x) * 4 + y], pa, b[0][y], b[1][y]);
                         }
                     }
                 }
-            }
+            };
+            if (__any_sync(0xffffffffu, top > 134u || low < 105u)) products(std::bool_constant<BF16>{}, std::true_type{});
+            else products(std::false_type{}, std::false_type{});
         }
         __syncwarp();  // the stage has been read
-        if (t + C::NS < nu) {
-            request(st);
-            lead.next(p, UNIT);
+        if (TMA) {
+            if (t + C::NS < nu) {
+                if (dirty) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // it has been written, too
+                sent = copy(st, ahead, ahead_row) ? sent | 1u << st : sent & ~(1u << st);
+                lead.next(p, UNIT);
+                if (t + C::NS + 1 < nu) ahead = page_of();
+            } else {
+                sent &= ~(1u << st);
+            }
+        } else {
+            if (t + C::NS < nu) {
+                request(st);
+                lead.next(p, UNIT);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
 
         // ---- the end of the column, or of the block's share
         const PaCursor done = cur;
-        cur.next(p, UNIT);
-        begin = t + 1 == nu || cur.col != done.col || cur.seq != done.seq;
+        begin = cur.next(p, UNIT) || t + 1 == nu;
         if (!begin) continue;
         const bool whole = seg_u == done.s.ulo && done.u == done.s.uhi - 1;
         const uint64_t slot = 2ull * blockIdx.x + (seg ? 1 : 0);
@@ -494,40 +642,41 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
             l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
         }
         const int row = tid >> 3, ch = tid & 7;
-        const uint32_t r = row0 + row, tok = r / p.group;
+        const uint32_t r = done.pack * PA_ROWS + row, tok = r / p.group;
         const bool there = r < done.s.rows;
         char *const orow = p.out + (done.s.q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
-        // half of the elements at a time: the warps' sums (and their maxima and weights), then eight threads per row
+        // a piece of the elements at a time: the warps' sums (and their maxima and weights), then eight threads per row
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int piece = 0; piece < C::PARTS; ++piece) {
+            constexpr int NP = NT / C::PARTS;  // products' tiles of a piece
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float *dst = mg + (warp * PA_ROWS + g + 8 * e) * C::MROW;
 #pragma unroll
-                for (int n = 0; n < NT / 2; ++n) {
-                    const float x0 = oacc[hf * (NT / 2) + n][2 * e], x1 = oacc[hf * (NT / 2) + n][2 * e + 1];
-                    if (MX) dst[2 * c * (NT / 2) + n] = x0, dst[(2 * c + 1) * (NT / 2) + n] = x1;
+                for (int n = 0; n < NP; ++n) {
+                    const float x0 = oacc[piece * NP + n][2 * e], x1 = oacc[piece * NP + n][2 * e + 1];
+                    if (MX) dst[2 * c * NP + n] = x0, dst[(2 * c + 1) * NP + n] = x1;
                     else *reinterpret_cast<float2 *>(dst + 8 * n + 2 * c) = make_float2(x0, x1);
                 }
-                if (c == 0) dst[HD / 2] = m[e], dst[HD / 2 + 1] = l[e];
+                if (c == 0) dst[C::PIECE] = m[e], dst[C::PIECE + 1] = l[e];
             }
             __syncthreads();
             if (!there) continue;
             float f[PA_WARPS], M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, mg[(w * PA_ROWS + row) * C::MROW + HD / 2]);
+            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, mg[(w * PA_ROWS + row) * C::MROW + C::PIECE]);
             const float ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int w = 0; w < PA_WARPS; ++w) {
-                f[w] = fast_exp2(mg[(w * PA_ROWS + row) * C::MROW + HD / 2] - ms);
-                L += f[w] * mg[(w * PA_ROWS + row) * C::MROW + HD / 2 + 1];
+                f[w] = fast_exp2(mg[(w * PA_ROWS + row) * C::MROW + C::PIECE] - ms);
+                L += f[w] * mg[(w * PA_ROWS + row) * C::MROW + C::PIECE + 1];
             }
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll 4
-            for (int x = 2 * ch; x < HD / 2; x += 16) {
-                // the elements that stand at x: MX has HD / 16 neighbours of every group of HD / 8
-                const uint32_t dd = MX ? (x / (HD / 16)) * (HD / 8) + hf * (HD / 16) + x % (HD / 16) : hf * (HD / 2) + x;
+            for (int x = 2 * ch; x < C::PIECE; x += 16) {
+                // the element that stands at x: MX has NP neighbours of every group of NT
+                const uint32_t dd = MX ? x / NP * NT + piece * NP + x % NP : piece * C::PIECE + x;
                 if (dd >= p.d) continue;
                 float o0 = 0.0f, o1 = 0.0f;
 #pragma unroll
@@ -539,13 +688,17 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                 if (whole) *reinterpret_cast<uint32_t *>(orow + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
                 else *reinterpret_cast<float2 *>(p.part_o + (slot * PA_ROWS + row) * p.d + dd) = make_float2(o0, o1);
             }
-            if (!whole && hf == 0 && ch == 0) p.part_ml[slot * PA_ROWS + row] = make_float2(M, L);
+            if (!whole && piece == 0 && ch == 0) p.part_ml[slot * PA_ROWS + row] = make_float2(M, L);
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (TMA && !ok && lane == 0) {
+        for (int i = 0; i < C::NS; ++i) mbar_wait_bounded(&bars[i], 0, 1u << 12), mbar_wait_bounded(&bars[i], 1, 1u << 12);  // copies in flight land first
+        atomicExch(&g_paged_wait_failed, 1);
+    }
 }
 
-// Joins the parts of columns that lie in several shares. Block i stands at the border in front of share i + 1; the first border inside a
+// Joins the parts of columns that lie in several shares. Blocks (i, head) stand at the border in front of share i + 1; the first border inside a
 // column is the one that joins it. Its eight warps take rows and parts; a row's parts meet in shared memory.
 template <bool BF16>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const int unit) {
@@ -553,20 +706,21 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const
     __shared__ float s_l[8], s_m[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ uint64_t s_place[10];
+    const uint32_t share = blockIdx.x / p.hkv, hk = blockIdx.x - share * p.hkv;
     uint64_t border = 0;
-    const PaPlace place = pa_place(p, unit, s_place, [&](uint64_t per) { return border = (blockIdx.x + 1) * per; });
+    const PaPlace place = pa_place(p, unit, s_place, [&](uint64_t per) { return border = (share + 1) * per; });
     PaCursor at;
     uint64_t first = border, last = border;
     if (border < place.total) {
         at.start(p, unit, place.seq, place.off);
         first = border - (uint64_t)(at.u - at.s.ulo), last = first + (uint64_t)(at.s.uhi - at.s.ulo) - 1;
     }
-    if (first == border || blockIdx.x * place.per > first) {  // behind the last unit, between two columns, or not the column's first
+    if (first == border || share * place.per > first) {  // behind the last unit, between two columns, or not the column's first
         if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid does not end before the one it follows
         return;
     }
-    const uint32_t b0 = blockIdx.x, parts = (uint32_t)(last / place.per) - b0 + 1;
-    const uint32_t hk = at.col / at.s.packs, row0 = (at.col - hk * at.s.packs) * PA_ROWS, rows = min((uint32_t)PA_ROWS, at.s.rows - row0);
+    const uint32_t parts = (uint32_t)(last / place.per) - share + 1;
+    const uint32_t row0 = at.pack * PA_ROWS, rows = min((uint32_t)PA_ROWS, at.s.rows - row0);
     // warps per row, a power of two
     const uint32_t per_row = rows > 4 ? 1 : (rows > 2 ? 2 : (rows > 1 ? 4 : 8)), step = 8 / per_row;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -583,7 +737,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const
                 for (int k = 0; k < 4; ++k) {
                     const uint32_t part = k0 + k * per_row;
                     // a share's first segment is in its first slot; the column's first part is that only where column and share begin alike
-                    const uint64_t slot = 2ull * (b0 + part) + (part == 0 && first != b0 * place.per ? 1 : 0);
+                    const uint64_t slot = 2ull * ((share + part) * (uint64_t)p.hkv + hk) + (part == 0 && first != share * place.per ? 1 : 0);
                     const bool in = part < parts;
                     ml[k] = in ? p.part_ml[slot * PA_ROWS + row] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
@@ -695,6 +849,7 @@ __global__ void __launch_bounds__(128) paged_split_join(const PaParams p, const 
 struct PaPlan {
     PaParams p;
     int hd, kind, unit;
+    uint32_t box;  // rows of a tensor copy, 0: 16-byte chunks
     size_t ws_bytes, off_ml;
     // the tcgen05 tiles: sequences of more than 16 packed rows
     bool tiles, steps;  // they are launched; the kernel of this file is
@@ -729,6 +884,11 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     const bool mx = a->pool.dtype == B200_FP8;
     pl.kind = (mx ? 2 : 0) + (a->q_dtype == B200_BF16 ? 1 : 0);
     pl.unit = PA_WARPS * (pl.hd == 64 || (pl.hd == 128 && mx) ? 32 : 16);
+    // Tensor copies: pages of whole groups of at least eight rows; MXFP8 rows whose scales then move in 16-byte pieces. 16-byte chunks serve the others.
+    const uint32_t keys = (uint32_t)pl.unit / PA_WARPS;
+    pl.box = keys;
+    while (a->pool.block_rows % pl.box) pl.box /= 2;
+    if (pl.box < 8 || (mx && (p.d != (uint32_t)pl.hd || pl.box * (p.d / 32) % 16)) || !may_map || !fa_pool_maps(p.pool, a->pool.dtype, false, pl.box, nullptr, nullptr, nullptr)) pl.box = 0;
     int sms = 148, dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     // Sequences of up to 16 packed rows (one group of mma.sync) are bound by their keys' bytes and stay here, longer ones by products:
@@ -757,14 +917,13 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
             p.row_cap = PA_ROWS;
         }
     }
-    // no more blocks than there can be units
+    // as many shares as two blocks per SM (one at head dim 256), no more than there can be units
     const uint64_t rows = pl.tiles ? PA_ROWS : (uint64_t)a->max_q * p.group, packs = (rows + PA_ROWS - 1) / PA_ROWS;
-    const uint64_t most = std::max<uint64_t>((uint64_t)a->b * p.hkv * packs * ((p.max_k + pl.unit - 1) / pl.unit + 1), 1);
-    p.blocks = (uint32_t)std::min<uint64_t>((uint64_t)sms * (pl.hd == 256 ? 1 : 2), most);
-    p.min_units = 1;
-    const size_t part_o = (size_t)2 * p.blocks * PA_ROWS * p.d * 4;
-    pl.off_ml = (part_o + 255) / 256 * 256;
-    pl.ws_bytes = pl.steps && p.blocks > 1 ? pl.off_ml + (size_t)2 * p.blocks * PA_ROWS * 8 : 0;
+    const uint64_t most = std::max<uint64_t>((uint64_t)a->b * packs * ((p.max_k + pl.unit - 1) / pl.unit + 1), 1);
+    p.shares = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)sms * (pl.hd == 256 ? 1 : 2) / p.hkv, 1), most);
+    const size_t slots = (size_t)2 * p.shares * p.hkv;
+    pl.off_ml = (slots * PA_ROWS * p.d * 4 + 255) / 256 * 256;
+    pl.ws_bytes = pl.steps && p.shares > 1 ? pl.off_ml + slots * PA_ROWS * 8 : 0;
     if (pl.tiles && pl.fa.n_splits > 1) {
         pl.off_split = (pl.ws_bytes + 255) / 256 * 256;
         pl.off_lse = pl.off_split + (pl.fa.n_splits * pl.fa.rows_total * p.d * 4 + 255) / 256 * 256;
@@ -773,21 +932,29 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     return B200_OK;
 }
 
-template <int HD, int KIND>
-static int pa_launch(const PaPlan &pl, cudaStream_t stream) {
+template <int HD, int KIND, bool TMA>
+static int pa_launch_as(const PaPlan &pl, const CUtensorMap &tm_k, const CUtensorMap &tm_v, uint32_t order, cudaStream_t stream) {
     static thread_local bool done[16] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 16 || !done[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA<HD, KIND>::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, KIND, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA<HD, KIND>::SMEM);
         if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention: shared memory opt-in: %s", cudaGetErrorString(e));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    paged_decode_kernel<HD, KIND><<<pl.p.blocks, PA_THREADS, PA<HD, KIND>::SMEM, stream>>>(pl.p);
-    const int rc = check_launch("paged_attention");
-    if (rc || pl.p.blocks == 1) return rc;
+    paged_decode_kernel<HD, KIND, TMA><<<pl.p.shares * pl.p.hkv, PA_THREADS, PA<HD, KIND>::SMEM, stream>>>(pl.p, tm_k, tm_v, order, pl.box);
+    return check_launch("paged_attention");
+}
+template <int HD, int KIND>
+static int pa_launch(const PaPlan &pl, cudaStream_t stream) {
+    CUtensorMap tm_k, tm_v;
+    uint32_t order = 0;
+    memset(&tm_k, 0, sizeof(tm_k)), memset(&tm_v, 0, sizeof(tm_v));
+    const bool tma = pl.box && fa_pool_maps(pl.p.pool, KIND >= 2 ? B200_FP8 : (KIND & 1 ? B200_BF16 : B200_F16), KIND & 1, pl.box, &tm_k, &tm_v, &order);
+    const int rc = tma ? pa_launch_as<HD, KIND, true>(pl, tm_k, tm_v, order, stream) : pa_launch_as<HD, KIND, false>(pl, tm_k, tm_v, 0, stream);
+    if (rc || pl.p.shares == 1) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(pl.p.blocks - 1);
+    cfg.gridDim = dim3((pl.p.shares - 1) * pl.p.hkv);
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -830,6 +997,15 @@ static int pa_tiles(const PaPlan &pl, int pool_dtype, cudaStream_t stream) {
                                              (const float *)pl.fa.part_lse, pl.fa.n_splits);
     if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention (split join): %s", cudaGetErrorString(e));
     return check_launch("paged_attention (split join)");
+}
+
+int paged_wait_status() {
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_paged_wait_failed, sizeof(int)) == cudaSuccess ? v : -1;
+}
+int paged_wait_clear() {
+    const int zero = 0;
+    return cudaMemcpyToSymbol(g_paged_wait_failed, &zero, sizeof(int)) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace b200

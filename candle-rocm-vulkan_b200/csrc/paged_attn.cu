@@ -62,6 +62,8 @@ struct PA {
     static constexpr int PARTS = HD == 128 && MX ? 4 : 2;                // pieces of a row that the warps' merge takes in turn (two blocks fit an SM)
     static constexpr int PIECE = HD / PARTS, MROW = PIECE + 2;           // floats per row: a piece, maximum, sum
     static constexpr uint32_t SM_SC = PA_WARPS * NS * STAGE, SM_MERGE = SM_SC + PA_WARPS * NS * SC, SM_BAR = SM_MERGE + PA_WARPS * PA_ROWS * MROW * 4, SMEM = SM_BAR + PA_WARPS * NS * 8;
+    static constexpr uint32_t CL_ML = PA_ROWS * HD * 4;  // a cluster's partial rows lie at 0, their maxima and sums here
+    static_assert(CL_ML + PA_ROWS * 8 <= SM_SC, "over the rings");
     // 16-byte chunk ch of row r of a tile, in 128-byte columns (64 where a row is no longer), swizzled
     __device__ static __forceinline__ uint32_t at(int r, int ch) {
         if (RB == 64) return r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
@@ -98,15 +100,15 @@ __device__ __forceinline__ uint64_t pa_seq(const PaParams &p, uint32_t b, int un
     return (uint64_t)(uint32_t)(s.uhi - s.ulo) * s.packs;
 }
 
-// Where the block (all of its threads; a multiple of 32, 256 at most) finds unit `target(total)` of all: the sequence and the unit
-// within it. Every thread sums a run of sequences. `scratch`: ten words of shared memory.
+// Where the block (all of its threads; a multiple of 32, 512 at most) finds unit `target(total)` of all: the sequence and the unit
+// within it. Every thread sums a run of sequences. `scratch`: 18 words of shared memory.
 struct PaPlace {
     uint64_t total, per, off;
     uint32_t seq;
 };
 template <typename F>
 __device__ __forceinline__ PaPlace pa_place(const PaParams &p, int unit, uint64_t *scratch, F target) {
-    uint64_t *const s_sum = scratch, *const s_at = scratch + 8;
+    uint64_t *const s_sum = scratch, *const s_at = scratch + 16;
     const uint32_t n = (p.b + blockDim.x - 1) / blockDim.x, first = min(threadIdx.x * n, p.b), last = min(first + n, p.b);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     uint64_t sum = 0;
@@ -211,12 +213,36 @@ __device__ __forceinline__ uint32_t pa_pack2(float lo, float hi) {
 }
 __device__ int g_paged_wait_failed = 0;  // a bounded wait for copies ran out
 
-// TMA: tiles by tensor copies (pages of whole groups of `box` rows), else by 16-byte chunks, each lane for itself
-template <int HD, int KIND, bool TMA>
+// MODE, how a block gets its units and keys:
+//   PA_CHUNKS  a share; 16-byte chunks, each lane for itself (pages of odd sizes)
+//   PA_COPIES  a share; tensor copies of `box` rows
+//   PA_CLUSTER a column per cluster of blocks, each with every n-th unit, joined through distributed shared memory: no division of work to find out, no
+//              second grid. Tensor copies.
+enum { PA_CHUNKS = 0, PA_COPIES, PA_CLUSTER };
+__device__ __forceinline__ uint32_t pa_cluster_size() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+__device__ __forceinline__ uint32_t pa_cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void pa_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the pair of floats at shared address `addr` of the cluster's block `rank`
+__device__ __forceinline__ float2 pa_peer(uint32_t addr, uint32_t rank) {
+    float2 v;
+    asm volatile("{\n .reg .u32 a;\n mapa.shared::cluster.u32 a, %2, %3;\n ld.shared::cluster.v2.f32 {%0, %1}, [a];\n}" : "=f"(v.x), "=f"(v.y) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+template <int HD, int KIND, int MODE>
 __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_kernel(const PaParams p, const __grid_constant__ CUtensorMap tm_k,
                                                                                      const __grid_constant__ CUtensorMap tm_v, const uint32_t tm_order, const uint32_t box) {
     using C = PA<HD, KIND>;
-    constexpr bool MX = C::MX, BF16 = C::BF16;
+    constexpr bool MX = C::MX, BF16 = C::BF16, TMA = MODE != PA_CHUNKS, CLUSTER = MODE == PA_CLUSTER;
     constexpr int KSTEPS = HD / 16, NT = HD / 8, KEYS = C::KEYS, KG = KEYS / 16, UNIT = C::UNIT;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -228,17 +254,34 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         mbar_fence_init();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (p.shares > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining grid may get ready
+    if (!CLUSTER && p.shares > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining grid may get ready
     const PoolParams &pl = p.pool;
-    const uint32_t share = blockIdx.x / p.hkv, hk = blockIdx.x - share * p.hkv;
-
-    const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return share * per; });
-    const uint64_t u0 = share * place.per;
-    if (u0 >= place.total) return;
-    const int nu = (int)min(place.per, place.total - u0);
+    // which head, and which units: nu of them, every stride-th
+    const uint32_t ranks = CLUSTER ? pa_cluster_size() : 1, rank = CLUSTER ? pa_cluster_rank() : 0, column = blockIdx.x / ranks;
+    const uint32_t share = column / p.hkv, hk = column - share * p.hkv;
     PaCursor cur, lead;  // the unit being worked on, and the one to be asked for next
-    cur.start(p, UNIT, place.seq, place.off);
+    int nu;
+    if (CLUSTER) {
+        cur.seq = share;
+        cur.pack = 0;
+        const int n = (int)pa_seq(p, share, UNIT, cur.s);
+        if (n == 0) return;  // the whole cluster
+        cur.u = cur.s.ulo + (int)rank;
+        cur.enter(p);
+        nu = (int)rank < n ? (n - (int)rank - 1) / (int)ranks + 1 : 0;
+    } else {
+        const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return share * per; });
+        const uint64_t u0 = share * place.per;
+        if (u0 >= place.total) return;
+        nu = (int)min(place.per, place.total - u0);
+        cur.start(p, UNIT, place.seq, place.off);
+    }
     lead = cur;
+    auto advance = [&](PaCursor &at) {  // true: to another column
+        if (!CLUSTER) return at.next(p, UNIT);
+        at.u += (int)ranks;
+        return false;
+    };
 
     // A warp's keys of the lead's unit into stage st: lane i finds key i's row, then C::CPR lanes copy a row. What no row of the column
     // sees, and what a page outside the pool would hold, is zeros.
@@ -336,7 +379,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         for (int t = 0; t <= C::NS; ++t) {
             ids[t] = t < nu ? page_of() : -1;
             rows[t] = ahead_row;
-            if (t < nu - 1) lead.next(p, UNIT);
+            if (t < nu - 1) advance(lead);
         }
         ahead = ids[C::NS];
         lead = cur;
@@ -344,13 +387,13 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         for (int t = 0; t < C::NS; ++t)
             if (t < nu) {
                 if (copy(t, ids[t], rows[t])) sent |= 1u << t;
-                lead.next(p, UNIT);
+                advance(lead);
             }
     } else {
         for (int t = 0; t < C::NS; ++t) {
             if (t < nu) {
                 request(t);
-                lead.next(p, UNIT);
+                advance(lead);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
@@ -360,7 +403,72 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     uint32_t qa[KSTEPS][4];
     float m[2], l[2], oacc[NT][4], sc[2], slope[2];
     int r_lo[2], r_hi[2], r_pos[2], lomax = 0, himin = 0;
-    const bool plain = p.softcap <= 0.0f && p.alibi == nullptr;
+    const bool special = p.softcap > 0.0f || p.alibi != nullptr, plain = !special && p.scale > 0.0f;
+    if (CLUSTER) {  // a block may be without units
+        m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.0f;
+    }
+    // A column's end in this block: the four warps' partial results meet in shared memory, and go out as rows (whole), as a part to the workspace, or to
+    // the block's shared memory for its cluster.
+    auto finish = [&](const PaCursor &done, bool whole, uint64_t slot) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        }
+        const int row = tid >> 3, ch = tid & 7;
+        const uint32_t r = done.pack * PA_ROWS + row, tok = r / p.group;
+        const bool there = r < done.s.rows;
+        char *const orow = p.out + (done.s.q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
+        // a piece of the elements at a time: the warps' sums (and their maxima and weights), then eight threads per row
+#pragma unroll
+        for (int piece = 0; piece < C::PARTS; ++piece) {
+            constexpr int NP = NT / C::PARTS;  // products' tiles of a piece
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float *dst = mg + (warp * PA_ROWS + g + 8 * e) * C::MROW;
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    const float x0 = oacc[piece * NP + n][2 * e], x1 = oacc[piece * NP + n][2 * e + 1];
+                    if (MX) dst[2 * c * NP + n] = x0, dst[(2 * c + 1) * NP + n] = x1;
+                    else *reinterpret_cast<float2 *>(dst + 8 * n + 2 * c) = make_float2(x0, x1);
+                }
+                if (c == 0) dst[C::PIECE] = m[e], dst[C::PIECE + 1] = l[e];
+            }
+            __syncthreads();
+            if (!there) continue;
+            float f[PA_WARPS], M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, mg[(w * PA_ROWS + row) * C::MROW + C::PIECE]);
+            const float ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) {
+                f[w] = fast_exp2(mg[(w * PA_ROWS + row) * C::MROW + C::PIECE] - ms);
+                L += f[w] * mg[(w * PA_ROWS + row) * C::MROW + C::PIECE + 1];
+            }
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll 4
+            for (int x = 2 * ch; x < C::PIECE; x += 16) {
+                // the element that stands at x: MX has NP neighbours of every group of NT
+                const uint32_t dd = MX ? x / NP * NT + piece * NP + x % NP : piece * C::PIECE + x;
+                if (dd >= p.d) continue;
+                float o0 = 0.0f, o1 = 0.0f;
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const float2 v = *reinterpret_cast<const float2 *>(mg + (w * PA_ROWS + row) * C::MROW + x);
+                    o0 = fmaf(f[w], v.x, o0);
+                    o1 = fmaf(f[w], v.y, o1);
+                }
+                if (CLUSTER) *reinterpret_cast<float2 *>(smem + (row * HD + dd) * 4) = make_float2(o0, o1);
+                else if (whole) *reinterpret_cast<uint32_t *>(orow + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
+                else *reinterpret_cast<float2 *>(p.part_o + (slot * PA_ROWS + row) * p.d + dd) = make_float2(o0, o1);
+            }
+            if (CLUSTER && piece == 0 && ch == 0) *reinterpret_cast<float2 *>(smem + C::CL_ML + row * 8) = make_float2(M, L);
+            if (!CLUSTER && !whole && piece == 0 && ch == 0) p.part_ml[slot * PA_ROWS + row] = make_float2(M, L);
+        }
+    };
     bool begin = true;
     int seg_u = 0;
     uint32_t seg = 0;  // the block's segments so far
@@ -469,21 +577,23 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                 }
         } else {
             const uint32_t nb = p.d / 32;
+            uint2 sw[2 * KG];  // the scales of this lane's two keys of every eight
+            if (C::NB == 4)
 #pragma unroll
-            for (int n = 0; n < 2 * KG; ++n) {
-                uint2 sw = make_uint2(0u, 0u);
-                if (C::NB == 4) sw = pa_lds64(tsc + (8 * n + 2 * c) * 4);  // the scales of this lane's two keys
+                for (int n = 0; n < 2 * KG; ++n) sw[n] = pa_lds64(tsc + (8 * n + 2 * c) * 4);
 #pragma unroll
-                for (int i = 0; i < C::NB; ++i) {
-                    if (!TMA && (uint32_t)i >= nb) break;
+            for (int i = 0; i < C::NB; ++i) {
+                if (!TMA && (uint32_t)i >= nb) break;
+                const uint32_t(&q0)[4] = qa[2 * i], (&q1)[4] = qa[2 * i + 1];
+#pragma unroll
+                for (int n = 0; n < 2 * KG; ++n) {
                     const uint2 w = pa_lds64(tk + C::at(8 * n + g, 2 * i + (c >> 1)) + (c & 1) * 8);
                     float z[4];
-                    const uint32_t(&q0)[4] = qa[2 * i], (&q1)[4] = qa[2 * i + 1];
                     mma_f16_16816_z(z, q0[0], q0[1], q0[2], q0[3], cvt_e4m3x2_f16x2(w.x), cvt_e4m3x2_hi_f16x2(w.x));
                     mma_f16_16816(z, q1[0], q1[1], q1[2], q1[3], cvt_e4m3x2_f16x2(w.y), cvt_e4m3x2_hi_f16x2(w.y));
                     // (the smallest scale, 2^-127, counts as nothing here)
-                    const float s0 = u2f(C::NB == 4 ? (i < 3 ? sw.x << (23 - 8 * (i & 3)) : sw.x >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i) << 23);
-                    const float s1 = u2f(C::NB == 4 ? (i < 3 ? sw.y << (23 - 8 * (i & 3)) : sw.y >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i) << 23);
+                    const float s0 = u2f(C::NB == 4 ? (i < 3 ? sw[n].x << (23 - 8 * (i & 3)) : sw[n].x >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i) << 23);
+                    const float s1 = u2f(C::NB == 4 ? (i < 3 ? sw[n].y << (23 - 8 * (i & 3)) : sw[n].y >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i) << 23);
                     s[n][0] = fmaf(z[0], s0, s[n][0]);
                     s[n][1] = fmaf(z[1], s1, s[n][1]);
                     s[n][2] = fmaf(z[2], s0, s[n][2]);
@@ -491,27 +601,37 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                 }
             }
         }
-        const bool full = plain && j0 >= lomax && j0 + KEYS <= himin;
-        float mx[2] = {-INFINITY, -INFINITY};
+        // Tiles that every row sees as they are: the maximum of the sums, the scale in the exponent's multiply-add. The others (masks, soft cap, slopes,
+        // a negative scale): scaled and masked one by one, apart from the first form's path.
+        float mul[2] = {sc[0] * PA_LOG2E, sc[1] * PA_LOG2E}, mx[2];
+        if (plain && j0 >= lomax && j0 + KEYS <= himin) {
 #pragma unroll
-        for (int n = 0; n < 2 * KG; ++n)
+            for (int e = 0; e < 2; ++e) {
+                mx[e] = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int e = i >> 1;
-                float x = s[n][i] * (sc[e] * PA_LOG2E);
-                if (!full) {
-                    const int j = j0 + 8 * n + 2 * c + (i & 1);
-                    if (!plain) {
+                for (int n = 1; n < 2 * KG; ++n) mx[e] = fmaxf(mx[e], fmaxf(s[n][2 * e], s[n][2 * e + 1]));
+                mx[e] *= mul[e];
+            }
+        } else {
+            mx[0] = mx[1] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 2 * KG; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = i >> 1, j = j0 + 8 * n + 2 * c + (i & 1);
+                    float x = s[n][i] * mul[e];
+                    if (special) {
                         x = s[n][i] * sc[e];
                         if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
-                        if (slope[e] != 0.0f) x -= slope[e] * fabsf((float)(r_pos[e] - j));
+                        x -= slope[e] * fabsf((float)(r_pos[e] - j));
                         x *= PA_LOG2E;
                     }
                     if (!(j >= r_lo[e] && j < r_hi[e])) x = -INFINITY;
+                    s[n][i] = x;
+                    mx[e] = fmaxf(mx[e], x);
                 }
-                s[n][i] = x;
-                mx[e] = fmaxf(mx[e], x);
-            }
+            mul[0] = mul[1] = 1.0f;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
@@ -531,10 +651,10 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         const float ms0 = m[0] == -INFINITY ? 0.0f : m[0] - 8.0f, ms1 = m[1] == -INFINITY ? 0.0f : m[1] - 8.0f;
 #pragma unroll
         for (int n = 0; n < 2 * KG; ++n) {
-            s[n][0] = fast_exp2(s[n][0] - ms0);
-            s[n][1] = fast_exp2(s[n][1] - ms0);
-            s[n][2] = fast_exp2(s[n][2] - ms1);
-            s[n][3] = fast_exp2(s[n][3] - ms1);
+            s[n][0] = fast_exp2(fmaf(s[n][0], mul[0], -ms0));
+            s[n][1] = fast_exp2(fmaf(s[n][1], mul[0], -ms0));
+            s[n][2] = fast_exp2(fmaf(s[n][2], mul[1], -ms1));
+            s[n][3] = fast_exp2(fmaf(s[n][3], mul[1], -ms1));
             l[0] += s[n][0] + s[n][1];
             l[1] += s[n][2] + s[n][3];
         }
@@ -565,14 +685,13 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
             // more); tiles with scales outside that take the second form: two factors, and bf16 under bf16 queries.
             constexpr int W = HD / 32;  // words of a lane's elements
             const uint32_t vsc = tsc + KEYS * C::NB + g * (HD / 8) / 32;
-            uint32_t e[KG][4], top = 0, low = 255;
+            uint32_t e[KG][4], off = 0;
 #pragma unroll
             for (int kk = 0; kk < KG; ++kk)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     e[kk][k] = pa_lds8(vsc + (kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8) * C::NB);
-                    top = max(top, e[kk][k]);
-                    low = min(low, e[kk][k]);
+                    off = __viaddmax_u32(e[kk][k], 0u - 105u, off);
                 }
             auto products = [&](auto bf, auto far) {
                 constexpr bool B = bf.value, FAR = far.value;
@@ -581,7 +700,9 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                     uint32_t pa[4], f[2], rest[2];
                     weights(bf, kk, pa);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) f[k] = pool_scale2<B>(e[kk][2 * k], e[kk][2 * k + 1], rest[k]);
+                    for (int k = 0; k < 2; ++k)
+                        if (FAR) f[k] = pool_scale2<B>(e[kk][2 * k], e[kk][2 * k + 1], rest[k]);
+                        else f[k] = pack_f16x2(u2f(e[kk][2 * k] << 23), u2f(e[kk][2 * k + 1] << 23));
 #pragma unroll
                     for (int i = 0; i < W; i += 2) {
                         uint32_t w[4][2];
@@ -608,7 +729,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                     }
                 }
             };
-            if (__any_sync(0xffffffffu, top > 134u || low < 105u)) products(std::bool_constant<BF16>{}, std::true_type{});
+            if (__any_sync(0xffffffffu, off > 29u)) products(std::bool_constant<BF16>{}, std::true_type{});
             else products(std::false_type{}, std::false_type{});
         }
         __syncwarp();  // the stage has been read
@@ -616,7 +737,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
             if (t + C::NS < nu) {
                 if (dirty) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // it has been written, too
                 sent = copy(st, ahead, ahead_row) ? sent | 1u << st : sent & ~(1u << st);
-                lead.next(p, UNIT);
+                advance(lead);
                 if (t + C::NS + 1 < nu) ahead = page_of();
             } else {
                 sent &= ~(1u << st);
@@ -624,72 +745,51 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         } else {
             if (t + C::NS < nu) {
                 request(st);
-                lead.next(p, UNIT);
+                advance(lead);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
 
         // ---- the end of the column, or of the block's share
-        const PaCursor done = cur;
-        begin = cur.next(p, UNIT) || t + 1 == nu;
-        if (!begin) continue;
-        const bool whole = seg_u == done.s.ulo && done.u == done.s.uhi - 1;
-        const uint64_t slot = 2ull * blockIdx.x + (seg ? 1 : 0);
-        ++seg;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        if (!CLUSTER && (cur.u + 1 == cur.s.uhi || t + 1 == nu)) {
+            finish(cur, seg_u == cur.s.ulo && cur.u + 1 == cur.s.uhi, 2ull * blockIdx.x + (seg ? 1 : 0));
+            ++seg;
+            begin = true;
         }
-        const int row = tid >> 3, ch = tid & 7;
-        const uint32_t r = done.pack * PA_ROWS + row, tok = r / p.group;
-        const bool there = r < done.s.rows;
-        char *const orow = p.out + (done.s.q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
-        // a piece of the elements at a time: the warps' sums (and their maxima and weights), then eight threads per row
+        advance(cur);
+    }
+    if (CLUSTER) {
+        // the block's rows into its shared memory (the rings: every copy has been waited for), then the cluster's blocks share the outputs
+        finish(cur, false, 0);
+        pa_cluster_sync();
+        const uint32_t at = smem_u32(smem), pairs = cur.s.rows * (p.d / 2);
+        for (uint32_t i = rank * PA_THREADS + tid; i < pairs; i += ranks * PA_THREADS) {
+            const uint32_t row = i / (p.d / 2), dd = 2 * (i - row * (p.d / 2));
+            float2 ml[8], o[8];
 #pragma unroll
-        for (int piece = 0; piece < C::PARTS; ++piece) {
-            constexpr int NP = NT / C::PARTS;  // products' tiles of a piece
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float *dst = mg + (warp * PA_ROWS + g + 8 * e) * C::MROW;
-#pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    const float x0 = oacc[piece * NP + n][2 * e], x1 = oacc[piece * NP + n][2 * e + 1];
-                    if (MX) dst[2 * c * NP + n] = x0, dst[(2 * c + 1) * NP + n] = x1;
-                    else *reinterpret_cast<float2 *>(dst + 8 * n + 2 * c) = make_float2(x0, x1);
-                }
-                if (c == 0) dst[C::PIECE] = m[e], dst[C::PIECE + 1] = l[e];
+            for (uint32_t k = 0; k < 8; ++k) {
+                if (k >= ranks) break;
+                ml[k] = pa_peer(at + C::CL_ML + row * 8, k);
+                o[k] = pa_peer(at + (row * HD + dd) * 4, k);
             }
-            __syncthreads();
-            if (!there) continue;
-            float f[PA_WARPS], M = -INFINITY, L = 0.0f;
+            float M = -INFINITY, L = 0.0f, o0 = 0.0f, o1 = 0.0f;
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) M = fmaxf(M, mg[(w * PA_ROWS + row) * C::MROW + C::PIECE]);
+            for (uint32_t k = 0; k < 8; ++k)
+                if (k < ranks) M = fmaxf(M, ml[k].x);
             const float ms = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) {
-                f[w] = fast_exp2(mg[(w * PA_ROWS + row) * C::MROW + C::PIECE] - ms);
-                L += f[w] * mg[(w * PA_ROWS + row) * C::MROW + C::PIECE + 1];
-            }
-            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-#pragma unroll 4
-            for (int x = 2 * ch; x < C::PIECE; x += 16) {
-                // the element that stands at x: MX has NP neighbours of every group of NT
-                const uint32_t dd = MX ? x / NP * NT + piece * NP + x % NP : piece * C::PIECE + x;
-                if (dd >= p.d) continue;
-                float o0 = 0.0f, o1 = 0.0f;
-#pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) {
-                    const float2 v = *reinterpret_cast<const float2 *>(mg + (w * PA_ROWS + row) * C::MROW + x);
-                    o0 = fmaf(f[w], v.x, o0);
-                    o1 = fmaf(f[w], v.y, o1);
+            for (uint32_t k = 0; k < 8; ++k)
+                if (k < ranks) {
+                    const float f = fast_exp2(ml[k].x - ms);
+                    L = fmaf(f, ml[k].y, L);
+                    o0 = fmaf(f, o[k].x, o0);
+                    o1 = fmaf(f, o[k].y, o1);
                 }
-                if (whole) *reinterpret_cast<uint32_t *>(orow + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
-                else *reinterpret_cast<float2 *>(p.part_o + (slot * PA_ROWS + row) * p.d + dd) = make_float2(o0, o1);
-            }
-            if (!whole && piece == 0 && ch == 0) p.part_ml[slot * PA_ROWS + row] = make_float2(M, L);
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+            const uint32_t tok = row / p.group;
+            *reinterpret_cast<uint32_t *>(p.out + (cur.s.q0 + tok) * p.o_st + (hk * p.group + row - tok * p.group) * p.o_sh + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
         }
+        pa_cluster_sync();  // a block's shared memory is there until all have read it
     }
     if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (TMA && !ok && lane == 0) {
@@ -699,13 +799,13 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
 }
 
 // Joins the parts of columns that lie in several shares. Blocks (i, head) stand at the border in front of share i + 1; the first border inside a
-// column is the one that joins it. Its eight warps take rows and parts; a row's parts meet in shared memory.
+// column is the one that joins it. Its sixteen warps take rows and parts; a row's parts meet in shared memory.
 template <bool BF16>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const int unit) {
-    __shared__ float s_o[8][256];
-    __shared__ float s_l[8], s_m[8];
+__global__ void __launch_bounds__(512) paged_join_kernel(const PaParams p, const int unit) {
+    __shared__ float s_o[16][256];
+    __shared__ float s_l[16], s_m[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __shared__ uint64_t s_place[10];
+    __shared__ uint64_t s_place[18];
     const uint32_t share = blockIdx.x / p.hkv, hk = blockIdx.x - share * p.hkv;
     uint64_t border = 0;
     const PaPlace place = pa_place(p, unit, s_place, [&](uint64_t per) { return border = (share + 1) * per; });
@@ -722,7 +822,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PaParams p, const
     const uint32_t parts = (uint32_t)(last / place.per) - share + 1;
     const uint32_t row0 = at.pack * PA_ROWS, rows = min((uint32_t)PA_ROWS, at.s.rows - row0);
     // warps per row, a power of two
-    const uint32_t per_row = rows > 4 ? 1 : (rows > 2 ? 2 : (rows > 1 ? 4 : 8)), step = 8 / per_row;
+    const uint32_t per_row = rows > 8 ? 1 : (rows > 4 ? 2 : (rows > 2 ? 4 : (rows > 1 ? 8 : 16))), step = 16 / per_row;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (uint32_t base = 0; base < rows; base += step) {
         const uint32_t row = base + warp / per_row, sub = warp % per_row;
@@ -850,6 +950,7 @@ struct PaPlan {
     PaParams p;
     int hd, kind, unit;
     uint32_t box;  // rows of a tensor copy, 0: 16-byte chunks
+    uint32_t cluster;  // blocks of a cluster per column, 0: shares
     size_t ws_bytes, off_ml;
     // the tcgen05 tiles: sequences of more than 16 packed rows
     bool tiles, steps;  // they are launched; the kernel of this file is
@@ -921,6 +1022,18 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     const uint64_t rows = pl.tiles ? PA_ROWS : (uint64_t)a->max_q * p.group, packs = (rows + PA_ROWS - 1) / PA_ROWS;
     const uint64_t most = std::max<uint64_t>((uint64_t)a->b * packs * ((p.max_k + pl.unit - 1) / pl.unit + 1), 1);
     p.shares = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)sms * (pl.hd == 256 ? 1 : 2) / p.hkv, 1), most);
+    // Columns over few keys: a cluster of up to eight blocks each, as many as are resident at once (clusters do not fill every place: 37 of eight
+    // blocks took two waves, 32 one), up to 1152 keys a block, or 576 where the clusters leave half of the places empty. us, shares
+    // and clusters, 32 / 8 heads of 128 over bf16 (lengths alike; spread evenly up to the longest): 1 x 300 keys 10.2, 7.1; 1 x 2000 14.7,
+    // 10.8; 1 x 4000 16.3, 16.0; 1 x 8000 19.1, 25.9; 8 x 2000 24.2, 17.9 (18.0, 17.0); 8 x 4000 36.5, 30.7 (25.8, 27.3); 16 x 2000 36.7, 30.3
+    // (29.5, 27.1); 16 x 4000 57.3, 52.2 (41.6, 50.9); 37 x 1000 35.7, 31.9 (39.5, 27.2). MXFP8: 8 x 4000 31.5, 26.3 (22.1, 24.3).
+    const uint64_t blocks = (uint64_t)sms * (pl.hd == 256 ? 1 : 2), columns = (uint64_t)a->b * p.hkv;
+    pl.cluster = 0;
+    if (pl.box && packs == 1 && columns > 0 && columns <= blocks) {
+        uint32_t n = 8;
+        while (n > 1 && columns * n > blocks / 8 * 7) n /= 2;
+        if (p.max_k <= (uint64_t)(columns * n * 2 > blocks ? 1152 : 576) * n) pl.cluster = n;
+    }
     const size_t slots = (size_t)2 * p.shares * p.hkv;
     pl.off_ml = (slots * PA_ROWS * p.d * 4 + 255) / 256 * 256;
     pl.ws_bytes = pl.steps && p.shares > 1 ? pl.off_ml + slots * PA_ROWS * 8 : 0;
@@ -932,17 +1045,28 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     return B200_OK;
 }
 
-template <int HD, int KIND, bool TMA>
+template <int HD, int KIND, int MODE>
 static int pa_launch_as(const PaPlan &pl, const CUtensorMap &tm_k, const CUtensorMap &tm_v, uint32_t order, cudaStream_t stream) {
     static thread_local bool done[16] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 16 || !done[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, KIND, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA<HD, KIND>::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<HD, KIND, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PA<HD, KIND>::SMEM);
         if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention: shared memory opt-in: %s", cudaGetErrorString(e));
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
-    paged_decode_kernel<HD, KIND, TMA><<<pl.p.shares * pl.p.hkv, PA_THREADS, PA<HD, KIND>::SMEM, stream>>>(pl.p, tm_k, tm_v, order, pl.box);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(MODE == PA_CLUSTER ? pl.p.b * pl.p.hkv * pl.cluster : pl.p.shares * pl.p.hkv);
+    cfg.blockDim = dim3(PA_THREADS);
+    cfg.dynamicSmemBytes = PA<HD, KIND>::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pl.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = MODE == PA_CLUSTER ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<HD, KIND, MODE>, pl.p, tm_k, tm_v, order, pl.box);
+    if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
     return check_launch("paged_attention");
 }
 template <int HD, int KIND>
@@ -951,11 +1075,12 @@ static int pa_launch(const PaPlan &pl, cudaStream_t stream) {
     uint32_t order = 0;
     memset(&tm_k, 0, sizeof(tm_k)), memset(&tm_v, 0, sizeof(tm_v));
     const bool tma = pl.box && fa_pool_maps(pl.p.pool, KIND >= 2 ? B200_FP8 : (KIND & 1 ? B200_BF16 : B200_F16), KIND & 1, pl.box, &tm_k, &tm_v, &order);
-    const int rc = tma ? pa_launch_as<HD, KIND, true>(pl, tm_k, tm_v, order, stream) : pa_launch_as<HD, KIND, false>(pl, tm_k, tm_v, 0, stream);
+    if (tma && pl.cluster) return pa_launch_as<HD, KIND, PA_CLUSTER>(pl, tm_k, tm_v, order, stream);
+    const int rc = tma ? pa_launch_as<HD, KIND, PA_COPIES>(pl, tm_k, tm_v, order, stream) : pa_launch_as<HD, KIND, PA_CHUNKS>(pl, tm_k, tm_v, 0, stream);
     if (rc || pl.p.shares == 1) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((pl.p.shares - 1) * pl.p.hkv);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(512);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -8,7 +8,7 @@
 // All three kernels are bound by memory: every element is read once and written once, in 16-byte pieces (8 elements a lane), a
 // head's row by neighbouring lanes of one warp. The two elements of a pair that lie rot / 2 apart meet by a shuffle. A warp has
 // one token: its lanes form the token's angles once (in f64: a position of a million times an f32 frequency has 48 bits), keep
-// the eight pairs of theirs in registers and go over the token's heads, four rows' loads on their way at a time. Where tokens
+// the eight pairs of theirs in registers and go over the token's heads, the next four rows' loads on their way while four are worked on. Where tokens
 // are few, a token's rows are shared among several warps, so that one decode step is one wave of short warps.
 #include <algorithm>
 
@@ -38,7 +38,7 @@ int pool_params(const B200PagedPool &pool, const char *what, PoolParams *p) {
     return B200_OK;
 }
 
-constexpr int PR_WARPS = 8, PR_BATCH = 4;  // warps per block; rows whose loads a lane has on their way
+constexpr int PR_WARPS = 8;  // per block
 
 struct RotaryParams {
     const float *freq;
@@ -64,32 +64,36 @@ struct RowsParams {
     uint32_t tokens, d, parts;  // warps per token
 };
 
-// eight elements as f32
+// eight elements as they are: four words of 16-bit elements, eight of f32
 template <int DT>
-__device__ __forceinline__ void load8(const char *src, bool vec, float (&x)[8]) {
-    if (DT == B200_F32) {
-        if (vec) {
-            const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 16);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
+struct Raw {
+    static constexpr int N = DT == B200_F32 ? 8 : 4;
+    uint32_t w[N];
+};
+template <int DT>
+__device__ __forceinline__ void load8(const char *src, bool vec, Raw<DT> &r) {
+    if (vec) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const float *>(src)[i];
+        for (int i = 0; i < Raw<DT>::N / 4; ++i) {
+            const uint4 a = reinterpret_cast<const uint4 *>(src)[i];
+            r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
         }
+    } else if (DT == B200_F32) {
+#pragma unroll
+        for (int i = 0; i < Raw<DT>::N; ++i) r.w[i] = reinterpret_cast<const uint32_t *>(src)[i];
     } else {
-        uint32_t w[4];
-        if (vec) {
-            const uint4 a = *reinterpret_cast<const uint4 *>(src);
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-        } else {
-            const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(src);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
-        }
+        for (int i = 0; i < Raw<DT>::N; ++i) r.w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void values8(const Raw<DT> &r, float (&x)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = DT == B200_BF16 ? bf16_bits_to_f((uint16_t)w[i]) : f16_bits_to_f((uint16_t)w[i]);
-            x[2 * i + 1] = DT == B200_BF16 ? bf16_bits_to_f((uint16_t)(w[i] >> 16)) : f16_bits_to_f((uint16_t)(w[i] >> 16));
-        }
+    for (int i = 0; i < 8; ++i) {
+        if (DT == B200_F32) x[i] = u2f(r.w[i % Raw<DT>::N]);
+        else if (DT == B200_BF16) x[i] = i & 1 ? u2f(r.w[i / 2] & 0xffff0000u) : u2f(r.w[i / 2] << 16);
+        else x[i] = f16_bits_to_f((uint16_t)(r.w[i / 2] >> (16 * (i & 1))));
     }
 }
 template <int DT>
@@ -155,7 +159,7 @@ __device__ __forceinline__ uint2 mx8(const float (&x)[8], uint32_t &scale) {
 // Measured: see the launcher.
 template <int DT, int TURN, int POOL, int PDT, int LPR>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsParams p, const bool vec) {
-    constexpr int RPW = 32 / LPR;
+    constexpr int RPW = 32 / LPR, PR_BATCH = DT == B200_F32 ? 2 : 4;
     __shared__ float2 s_cs[PR_WARPS][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % LPR, sub = lane / LPR;
     const uint64_t unit = (uint64_t)blockIdx.x * PR_WARPS + warp;
@@ -163,6 +167,23 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsPar
     if (token >= p.tokens) return;  // whole warps; nothing below waits for another warp
     const bool in = (uint32_t)c * 8 < p.d;
     const uint32_t half = p.rot.rot / 2;
+
+    // the token's rows: q's heads, k's, v's; this warp's share of them, a batch's loads ahead of the one that is worked on
+    const uint32_t nqk = p.q.heads + p.k.heads, rows = nqk + p.v.heads, step = p.parts * RPW;
+    auto fetch = [&](uint32_t r0, Raw<DT> &w) {
+        const uint32_t r = r0 + sub;
+        if (r < rows && in) {
+            const HeadsParams &h = r < p.q.heads ? p.q : (r < nqk ? p.k : p.v);
+            const uint32_t hd = r < p.q.heads ? r : (r < nqk ? r - p.q.heads : r - nqk);
+            load8<DT>(h.src + token * h.s_t + hd * h.s_h + (uint64_t)c * 8 * dtype_size(DT), vec, w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Raw<DT>::N; ++i) w.w[i] = 0u;
+        }
+    };
+    Raw<DT> next[PR_BATCH];
+#pragma unroll
+    for (int j = 0; j < PR_BATCH; ++j) fetch(part * RPW + j * step, next[j]);
 
     float co[8], si[8];
     int partner = lane;
@@ -213,51 +234,51 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsPar
         }
     }
 
-    // the token's rows: q's heads, k's, v's; this warp's share of them
-    const uint32_t nqk = p.q.heads + p.k.heads, rows = nqk + p.v.heads;
-    for (uint32_t base = part * RPW; base < rows; base += p.parts * RPW * PR_BATCH) {
-        float x[PR_BATCH][8];
+#pragma unroll 1
+    for (uint32_t base = part * RPW; base < rows; base += step * PR_BATCH) {
+        Raw<DT> raw[PR_BATCH];
+#pragma unroll
+        for (int j = 0; j < PR_BATCH; ++j) raw[j] = next[j];
+#pragma unroll
+        for (int j = 0; j < PR_BATCH; ++j) fetch(base + (PR_BATCH + j) * step, next[j]);
 #pragma unroll
         for (int j = 0; j < PR_BATCH; ++j) {
-            const uint32_t r = base + j * p.parts * RPW + sub;
-            if (r < rows && in) {
-                const HeadsParams &h = r < p.q.heads ? p.q : (r < nqk ? p.k : p.v);
-                const uint32_t hd = r < p.q.heads ? r : (r < nqk ? r - p.q.heads : r - nqk);
-                load8<DT>(h.src + token * h.s_t + hd * h.s_h + (uint64_t)c * 8 * dtype_size(DT), vec, x[j]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < PR_BATCH; ++j) {
-            const uint32_t r0 = base + j * p.parts * RPW, r = r0 + sub;
+            const uint32_t r0 = base + j * step, r = r0 + sub;
             if (r0 >= rows) break;  // the whole warp
             const bool is_v = r >= nqk;
-            if (TURN) {
+            float x[8];
+            values8(raw[j], x);
+            if (TURN && r0 < nqk) {
                 float y[8];
+                if (TURN == 1) {
+                    Raw<DT> other;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = TURN == 1 ? __shfl_sync(0xffffffffu, x[j][i], partner) : x[j][i ^ 1];
+                    for (int i = 0; i < Raw<DT>::N; ++i) other.w[i] = __shfl_sync(0xffffffffu, raw[j].w[i], partner);
+                    values8(other, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+                }
                 if (turned && !is_v) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[j][i] = fmaf(x[j][i], co[i], y[i] * si[i]);
+                    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], co[i], y[i] * si[i]);
                 }
             }
             if (r < p.q.heads || (POOL == 0 && r < rows)) {
                 const HeadsParams &h = r < p.q.heads ? p.q : p.k;
                 const uint32_t hd = r < p.q.heads ? r : r - p.q.heads;
-                if (in) store8<DT>(h.dst + token * h.d_t + hd * h.d_h + (uint64_t)c * 8 * dtype_size(DT), vec, x[j]);
+                if (in) store8<DT>(h.dst + token * h.d_t + hd * h.d_h + (uint64_t)c * 8 * dtype_size(DT), vec, x);
             }
-            if (POOL) {
+            if (POOL && r0 + RPW > p.q.heads) {
                 const bool mine = r >= p.q.heads && r < rows && kept && in;
                 const uint32_t hd = is_v ? r - nqk : r - p.q.heads;
                 const PoolParams &pl = p.pool;
                 char *dst = is_v ? pl.v + blk * pl.v_sb + row * pl.v_sr + hd * pl.v_sh : pl.k + blk * pl.k_sb + row * pl.k_sr + hd * pl.k_sh;
                 if (POOL == 1) {
-                    if (mine) *reinterpret_cast<uint4 *>(dst + c * 16) = pack8<PDT>(x[j]);
+                    if (mine) *reinterpret_cast<uint4 *>(dst + c * 16) = pack8<PDT>(x);
                 } else {
                     uint32_t scale;
-                    const uint2 w = mx8(x[j], scale);
+                    const uint2 w = mx8(x, scale);
                     if (mine) {
                         *reinterpret_cast<uint2 *>(dst + c * 8) = w;
                         if ((c & 3) == 0) (is_v ? pl.vs : pl.ks)[(((uint64_t)blk * pl.hkv + hd) * pl.block_rows + row) * (pl.d / 32) + c / 4] = (uint8_t)scale;
@@ -332,7 +353,7 @@ struct UnpackParams {
 
 template <int DT, int POOL, int PDT, int LPR>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const UnpackParams p) {
-    constexpr int RPW = 32 / LPR;
+    constexpr int RPW = 32 / LPR, PR_BATCH = 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % LPR, sub = lane / LPR;
     const uint64_t unit = (uint64_t)blockIdx.x * PR_WARPS + warp, t = unit / p.parts;
     const uint32_t part = (uint32_t)(unit % p.parts);

@@ -13,7 +13,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _abi as A
-from .turbo_quant import FlashAttnConfig, _call_workspace, _dtype_id, _need_cuda, _stream
+from .turbo_quant import FlashAttnConfig, _DTYPES, _call_workspace, _capturing, _dtype_id, _need_cuda, _stream, _workspace
 
 _E4M3 = getattr(torch, "float8_e4m3fn", None)
 _POOL_DTYPES = {torch.float16: A.F16, torch.bfloat16: A.BF16, _E4M3: A.FP8}
@@ -29,6 +29,7 @@ assert _POOL.size == C.sizeof(A.PagedPool) and _ROTARY_ARGS.size == C.sizeof(A.R
 assert _POOL.size + _APPEND_ARGS.size == C.sizeof(A.PagedAppendArgs) and _POOL.size + _UNPACK_ARGS.size == C.sizeof(A.PagedUnpackArgs)
 assert _POOL.size + _ATTN_ARGS.size == C.sizeof(A.PagedAttnArgs)
 
+_lib = A.lib
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
@@ -49,13 +50,25 @@ def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:
         if t.dtype.is_floating_point or t.dtype == torch.bool:
             raise ValueError(f"{what} must be whole numbers, got {t.dtype}")
         t = t.to(device=device, dtype=dtype)
-    return t if t.stride(-1) == 1 or t.numel() <= 1 else t.contiguous()
+    return t if t.stride()[-1] == 1 or t.numel() <= 1 else t.contiguous()
 
 
-def _heads(t: torch.Tensor, what: str, tokens: Optional[int] = None, d: Optional[int] = None) -> torch.Tensor:
-    if t.dim() != 3 or (tokens is not None and t.shape[0] != tokens) or (d is not None and t.shape[2] != d):
-        raise ValueError(f"{what} must be ({'tokens' if tokens is None else tokens}, heads, {'head_dim' if d is None else d}), got {tuple(t.shape)}")
-    return t if t.stride(2) == 1 else t.contiguous()
+# A decode step's calls are host time before they are anything else, so a tensor is asked for its shape and strides once, and outputs are made
+# the quickest way torch has (empty_like and empty_strided: 1.1 us, empty: 2 to 4).
+def _heads(t: torch.Tensor, what: str, tokens: Optional[int] = None, d: Optional[int] = None):
+    """(the tensor, its shape, its strides) of a (tokens, heads, head_dim) operand, contiguous along the last axis."""
+    shape = t.shape
+    if len(shape) != 3 or (tokens is not None and shape[0] != tokens) or (d is not None and shape[2] != d):
+        raise ValueError(f"{what} must be ({'tokens' if tokens is None else tokens}, heads, {'head_dim' if d is None else d}), got {tuple(shape)}")
+    st = t.stride()
+    if st[2] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, shape, st
+
+
+def _float_id(t: torch.Tensor) -> int:
+    return _DTYPES.get(t.dtype) if t.dtype in _DTYPES else _dtype_id(t)
 
 
 class RotaryAxes:
@@ -88,27 +101,36 @@ class RotaryAxes:
         if len(axes) != half or min(axes) < 0 or self.n_axes > 256:
             raise ValueError(f"rotary: {half} frequencies need an axis from 0 to 255 each")
         self.axis = torch.tensor(axes, dtype=torch.uint8, device=self.freq.device)
+        self.device = self.freq.device
+        self._head = (self.freq.data_ptr(), self.axis.data_ptr())
 
     def fields(self, positions: torch.Tensor, tokens: int, device, inverse: bool):
         """(the values of a B200Rotary, the positions to keep alive)."""
-        pos = positions if positions.dim() == 2 else positions.reshape(1, -1) if positions.dim() == 1 else None
-        if pos is None or tuple(pos.shape) != (self.n_axes, tokens):
+        pos = positions
+        shape = pos.shape
+        if len(shape) == 1:
+            pos = pos.reshape(1, -1)
+            shape = pos.shape
+        if shape != (self.n_axes, tokens):
             raise ValueError(f"rotary: positions must be ({self.n_axes}, {tokens}), got {tuple(positions.shape)}")
-        if self.freq.device != device:
+        if self.device != device:
             raise ValueError("rotary: frequencies live on another device")
         pos = _ints(pos, torch.int64, device, "rotary: positions")
-        return (self.freq.data_ptr(), self.axis.data_ptr(), pos.data_ptr(), pos.stride(0), self.n_axes, self.rot, int(self.interleaved), int(inverse)), pos
+        return (*self._head, pos.data_ptr(), pos.stride()[0], self.n_axes, self.rot, self.interleaved, inverse), pos
 
 
 _NO_ROTARY = (0, 0, 0, 0, 0, 0, 0, 0)
 
 
-def _out_like(t: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
+def _out_like(t: torch.Tensor, out: Optional[torch.Tensor], what: str):
+    """(the output tensor, its strides): `out`, or a new one like `t`."""
     if out is None:
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-    if out.shape != t.shape or out.dtype != t.dtype or out.device != t.device or out.stride(2) != 1:
+        out = torch.empty_like(t)
+        return out, out.stride()
+    st = out.stride()
+    if out.shape != t.shape or out.dtype != t.dtype or out.device != t.device or st[2] != 1:
         raise ValueError(f"{what} must be a {t.dtype} {tuple(t.shape)} tensor on {t.device} with a contiguous head dim")
-    return out
+    return out, st
 
 
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: RotaryAxes, inverse: bool = False,
@@ -118,22 +140,22 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     positions; the elements are turned in f32 and rounded once. `inverse=True` turns back: the gradient with respect to q and
     k of a call's outputs' gradients."""
     _need_cuda(q, "q")
-    q = _heads(q, "rotary: q")
-    tokens, hq, d = q.shape
+    q, (tokens, hq, d), qs = _heads(q, "rotary: q")
+    device = q.device
     if rotary.rot > d:
         raise ValueError(f"rotary: {rotary.rot} turned elements, heads of {d}")
-    qo = _out_like(q, q_out, "rotary: q_out")
-    qs, qos = (q.stride(0), q.stride(1)), (qo.stride(0), qo.stride(1))
+    qo, qos = _out_like(q, q_out, "rotary: q_out")
     if k is not None:
-        k = _heads(k, "rotary: k", tokens, d)
-        if k.dtype != q.dtype or k.device != q.device:
-            raise ValueError(f"rotary: q is {q.dtype} on {q.device}, k is {k.dtype} on {k.device}")
-        ko = _out_like(k, k_out, "rotary: k_out")
-        kp, kop, ks, kos, hkv = k.data_ptr(), ko.data_ptr(), (k.stride(0), k.stride(1)), (ko.stride(0), ko.stride(1)), k.shape[1]
+        k, ksh, ks = _heads(k, "rotary: k", tokens, d)
+        if k.dtype != q.dtype or k.device != device:
+            raise ValueError(f"rotary: q is {q.dtype} on {device}, k is {k.dtype} on {k.device}")
+        ko, kos = _out_like(k, k_out, "rotary: k_out")
+        kp, kop, hkv = k.data_ptr(), ko.data_ptr(), ksh[1]
     else:
         ko, kp, kop, ks, kos, hkv = None, 0, 0, (0, 0), (0, 0), 0
-    fields, pos = rotary.fields(positions, tokens, q.device, inverse)
-    _call(A.lib().b200_rotary_axes, _ROTARY_ARGS.pack(q.data_ptr(), kp, qo.data_ptr(), kop, *qs, *ks, *qos, *kos, tokens, hq, hkv, d, _dtype_id(q), 0, *fields), q.device)
+    fields, pos = rotary.fields(positions, tokens, device, inverse)
+    _call(_lib().b200_rotary_axes, _ROTARY_ARGS.pack(q.data_ptr(), kp, qo.data_ptr(), kop, qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1],
+                                                     tokens, hq, hkv, d, _float_id(q), 0, *fields), device)
     return qo, ko
 
 
@@ -192,38 +214,43 @@ class PagedKvPool:
         is not written; a slot past the pool is not either, and sets `status` (an int32 device tensor) to 3. With `rotary` and
         `positions` (axes, tokens) the keys are turned first, and with `q` (tokens, q_heads, head_dim) the queries
         beside them: returns them in `q_out` (a new tensor unless given; `q` itself: in place)."""
-        dev = self.device
-        k = _heads(k, "paged append: k", None, self.head_dim)
-        tokens = k.shape[0]
-        v = _heads(v, "paged append: v", tokens, self.head_dim)
-        if k.shape[1] != self.kv_heads or v.shape[1] != self.kv_heads or k.dtype != v.dtype or k.device != dev or v.device != dev:
+        dev, d = self.device, self.head_dim
+        k, (tokens, h, _), ks = _heads(k, "paged append: k", None, d)
+        v, vsh, vs = _heads(v, "paged append: v", tokens, d)
+        if h != self.kv_heads or vsh[1] != h or k.dtype != v.dtype or k.device != dev or v.device != dev:
             raise ValueError(f"paged append: k {tuple(k.shape)} {k.dtype} / v {tuple(v.shape)} {v.dtype} do not match {self.kv_heads} kv heads on {dev}")
         slots = _ints(slots, torch.int64, dev, "paged append: slots")
-        if slots.dim() != 1 or slots.shape[0] != tokens:
+        if slots.shape != (tokens,):
             raise ValueError(f"paged append: {tokens} tokens need as many slots, got {tuple(slots.shape)}")
-        if (rotary is None) != (positions is None):
-            raise ValueError("paged append: rotary and positions come together")
-        fields, pos = rotary.fields(positions, tokens, dev, False) if rotary is not None else (_NO_ROTARY, None)
-        if rotary is not None and rotary.rot > self.head_dim:
-            raise ValueError(f"rotary: {rotary.rot} turned elements, heads of {self.head_dim}")
         qo, qp, qop, qs, qos, hq = None, 0, 0, (0, 0), (0, 0), 0
-        if q is not None:
-            if rotary is None:
-                raise ValueError("paged append: queries are turned; without rotary there is nothing to do with them")
-            q = _heads(q, "paged append: q", tokens, self.head_dim)
-            if q.dtype != k.dtype or q.device != dev:
-                raise ValueError(f"paged append: q is {q.dtype} on {q.device}, k {k.dtype} on {dev}")
-            qo = _out_like(q, q_out, "paged append: q_out")
-            qp, qop, qs, qos, hq = q.data_ptr(), qo.data_ptr(), (q.stride(0), q.stride(1)), (qo.stride(0), qo.stride(1)), q.shape[1]
-        _call(A.lib().b200_paged_append, self._packed + _APPEND_ARGS.pack(
-            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), qp, qop, *qs, *qos, tokens, hq, _dtype_id(k), 0,
+        if rotary is not None:
+            if positions is None:
+                raise ValueError("paged append: rotary and positions come together")
+            if rotary.rot > d:
+                raise ValueError(f"rotary: {rotary.rot} turned elements, heads of {d}")
+            fields, pos = rotary.fields(positions, tokens, dev, False)
+            if q is not None:
+                q, qsh, qs = _heads(q, "paged append: q", tokens, d)
+                if q.dtype != k.dtype or q.device != dev:
+                    raise ValueError(f"paged append: q is {q.dtype} on {q.device}, k {k.dtype} on {dev}")
+                qo, qos = _out_like(q, q_out, "paged append: q_out")
+                qp, qop, hq = q.data_ptr(), qo.data_ptr(), qsh[1]
+        elif positions is not None:
+            raise ValueError("paged append: rotary and positions come together")
+        elif q is not None:
+            raise ValueError("paged append: queries are turned; without rotary there is nothing to do with them")
+        else:
+            fields = _NO_ROTARY
+        _call(_lib().b200_paged_append, self._packed + _APPEND_ARGS.pack(
+            k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), qp, qop, qs[0], qs[1], qos[0], qos[1], tokens, hq, _float_id(k), 0,
             *fields, status.data_ptr() if status is not None else 0), dev)
         return qo
 
     def _table(self, table: torch.Tensor, b: int, what: str) -> torch.Tensor:
-        if table.dim() != 2 or table.shape[0] != b:
-            raise ValueError(f"{what}: block_table must have a row for each of {b} sequences, got {tuple(table.shape)}")
-        return _ints(table, torch.int32, self.device, f"{what}: block_table")
+        shape = table.shape
+        if len(shape) != 2 or shape[0] != b:
+            raise ValueError(f"{what}: block_table must have a row for each of {b} sequences, got {tuple(shape)}")
+        return _ints(table, torch.int32, self.device, "block_table")
 
     def keys_values(self, block_table: torch.Tensor, seqlens_k: torch.Tensor, total: int, dtype: Optional[torch.dtype] = None,
                     status: Optional[torch.Tensor] = None):
@@ -231,14 +258,16 @@ class PagedKvPool:
         pool's own, bf16 for MXFP8). `seqlens_k`: cumulative lengths (sequences + 1, on the device, as for the varlen calls); `total`:
         their last (rows behind it are left as allocated). Page numbers outside the pool read as zeros and set `status` to 3."""
         b = seqlens_k.numel() - 1
+        dev = self.device
         table = self._table(block_table, b, "paged keys_values")
-        cu = _ints(seqlens_k, torch.int32, self.device, "paged keys_values: seqlens_k")
+        cu = _ints(seqlens_k, torch.int32, dev, "paged keys_values: seqlens_k")
         dtype = dtype or (torch.bfloat16 if self.dtype == A.FP8 else self.k.dtype)
-        k = torch.empty((int(total), self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        total, h, d = int(total), self.kv_heads, self.head_dim
+        k = torch.empty_strided((total, h, d), (h * d, d, 1), dtype=dtype, device=dev)
         v = torch.empty_like(k)
-        _call(A.lib().b200_paged_unpack, self._packed + _UNPACK_ARGS.pack(
-            table.data_ptr(), table.stride(0), cu.data_ptr(), k.data_ptr(), v.data_ptr(), k.shape[0], b, table.shape[1], _dtype_id(k), 0,
-            status.data_ptr() if status is not None else 0), self.device)
+        _call(_lib().b200_paged_unpack, self._packed + _UNPACK_ARGS.pack(
+            table.data_ptr(), table.stride()[0], cu.data_ptr(), k.data_ptr(), v.data_ptr(), total, b, table.shape[1], _float_id(k), 0,
+            status.data_ptr() if status is not None else 0), dev)
         return k, v
 
     def attention(self, q: torch.Tensor, seqlens_q: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
@@ -250,33 +279,42 @@ class PagedKvPool:
         `max_seqlen_q` and `max_seqlen_k` bound them (longer ones are cut). Rows of `out` (a new tensor unless given) behind the last
         sequence are left as they were. Page numbers outside the pool hold zeros and set `status` (an int32 device tensor) to 3."""
         dev = self.device
-        q = _heads(q, "paged attention: q", None, self.head_dim)
-        total, hq, d = q.shape
+        q, (total, hq, _), qs = _heads(q, "paged attention: q", None, self.head_dim)
         if q.device != dev:
             raise ValueError(f"paged attention: q is on {q.device}, the pool on {dev}")
-        if cfg.softcap is not None and not cfg.softcap > 0.0:
+        softcap = cfg.softcap or 0.0
+        if cfg.softcap is not None and not softcap > 0.0:
             raise ValueError("flash-attn: softcap must be > 0")
         if cfg.k_descale != 1.0 or cfg.v_descale != 1.0:
             raise ValueError("paged attention: a pool's scales are its own; k_descale and v_descale must be 1")
         b = seqlens_q.numel() - 1
         if b < 0 or kv_len.numel() != b:
             raise ValueError(f"paged attention: {seqlens_q.numel()} cumulative lengths do not go with {kv_len.numel()} sequences")
-        out = _out_like(q, out, "paged attention: out")
+        out, os = _out_like(q, out, "paged attention: out")
         table = self._table(block_table, b, "paged attention")
         cu = _ints(seqlens_q, torch.int32, dev, "paged attention: seqlens_q")
         lens = _ints(kv_len, torch.int32, dev, "paged attention: kv_len")
-        alibi, abs_ = None, 0
+        alibi, ap, abs_ = None, 0, 0
         if cfg.alibi_slopes is not None:
             alibi = cfg.alibi_slopes.to(device=dev, dtype=torch.float32).contiguous()
             if alibi.shape not in ((hq,), (b, hq)):
                 raise ValueError(f"flash-attn: alibi slopes must be ({hq}) or ({b}, {hq}), got {tuple(alibi.shape)}")
-            abs_ = hq if alibi.dim() == 2 else 0
+            ap, abs_ = alibi.data_ptr(), hq if alibi.dim() == 2 else 0
         wl, wr = cfg.window_i32()
-        fields = (q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), cu.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0),
-                  b, total, int(max_seqlen_q), int(max_seqlen_k), hq, table.shape[1], _dtype_id(q), cfg.softmax_scale, cfg.softcap or 0.0, wl, wr,
-                  alibi.data_ptr() if alibi is not None else 0, abs_, 0)
+        fields = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], cu.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride()[0],
+                  b, total, int(max_seqlen_q), int(max_seqlen_k), hq, table.shape[1], _float_id(q), cfg.softmax_scale, softcap, wl, wr, ap, abs_, 0)
         st = status.data_ptr() if status is not None else 0
-        lib = A.lib()
+        lib = _lib()
+        if not _capturing():
+            # the stream's scratch as it is; the library says where it is too small
+            ws = _workspace(dev, 1 << 20)
+            args = self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr(), ws.numel(), st)
+            if dev.index == _current_device():
+                rc = lib.b200_paged_attention(args, _stream(dev))
+                if rc == A.OK:
+                    return out
+                if rc != A.ERR_WORKSPACE:
+                    A.check(rc)
         nbytes = lib.b200_paged_attention_workspace_bytes(self._packed + _ATTN_ARGS.pack(*fields, 0, 0, st))
         ws = _call_workspace(dev, nbytes) if nbytes else None
         _call(lib.b200_paged_attention, self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr() if ws is not None else 0, nbytes, st), dev)

@@ -26,6 +26,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "fa_params.cuh"
@@ -1538,33 +1539,52 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                         for (uint32_t i = 0; i < nb; ++i) ks |= (uint32_t)pg.pool.ks[at + i] << (8 * i), vs |= (uint32_t)pg.pool.vs[at + i] << (8 * i);
                     }
                 };
-                // row `key` of a raw tile, or zeros, into the layout of the tensor copies
+                // Row `key` of a raw tile, or zeros, into the layout of the tensor copies. One warp per SM quadrant widens all of a tile's keys while
+                // two others compute exponentials, so it is its instructions that count: four chunks of codes at a time, one multiplier
+                // per 32 elements; rows with a scale outside the type's range (pool_scale2) apart.
                 auto widen = [&](uint32_t raw, uint32_t dst, uint32_t sc, bool zero) {
                     constexpr int CH = HD / 16;  // raw chunks of 16 codes
-                    const uint32_t row = raw + key * HD;
+                    const uint32_t row = raw + key * HD, out = dst + key * 128, sw = HD == 64 ? (key >> 1) & 3 : key & 7;
+                    auto put = [&](int c0, const uint32_t(&o)[4]) {
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(out + (c0 >> 3) * C::T_HALF + (((c0 & 7) ^ (key & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+                    };
+                    if (zero) {
+                        const uint32_t o[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-                    for (int ch = 0; ch < CH; ++ch) {
-                        uint4 w;
-                        const uint32_t sw = HD == 64 ? (ch ^ ((key >> 1) & 3)) : (ch ^ (key & 7));
-                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(row + (sw << 4)));
-                        const uint32_t e = (sc >> (8 * (ch >> 1))) & 0xffu, a[4] = {w.x, w.y, w.z, w.w};
-                        uint32_t rest, o[8];
-                        const uint32_t f = pool_scale2<BF16>(e, e, rest);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            o[2 * i] = pool_mul2<BF16>(pool_pair<BF16, 0>(a[i]), f);
-                            o[2 * i + 1] = pool_mul2<BF16>(pool_pair<BF16, 1>(a[i]), f);
-                        }
-                        if (BF16 ? e > 134u : e < 103u)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = pool_mul2<BF16>(o[i], rest);
-                        if (zero)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) o[i] = 0u;
-                        const uint32_t c0 = 2 * ch, at = dst + (c0 >> 3) * C::T_HALF + key * 128;
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (((c0 & 7) ^ (key & 7)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + ((((c0 + 1) & 7) ^ (key & 7)) << 4)), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                        for (int c0 = 0; c0 < 2 * CH; ++c0) put(c0, o);
+                        return;
                     }
+                    auto chunks = [&](auto far_) {
+                        constexpr bool FAR = far_.value;
+#pragma unroll
+                        for (int q = 0; q < CH; q += 4) {
+                            uint32_t a[4][4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(a[i][0]), "=r"(a[i][1]), "=r"(a[i][2]), "=r"(a[i][3]) : "r"(row + (((q + i) ^ sw) << 4)));
+#pragma unroll
+                            for (int i = 0; i < 4; i += 2) {
+                                const uint32_t e = (sc >> (4 * (q + i))) & 0xffu;
+                                uint32_t rest = 0, f;
+                                if (FAR) f = pool_scale2<BF16>(e, e, rest);
+                                else if (BF16) f = ((e + 120u) << 7) * 0x10001u;
+                                else f = pack_f16x2(u2f(e << 23), u2f(e << 23));
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {  // two chunks of 32 elements' codes, eight elements a store
+                                    const uint32_t w0 = a[i + x / 2][2 * (x & 1)], w1 = a[i + x / 2][2 * (x & 1) + 1];
+                                    uint32_t o[4] = {pool_pair<BF16, 0>(w0), pool_pair<BF16, 1>(w0), pool_pair<BF16, 0>(w1), pool_pair<BF16, 1>(w1)};
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) {
+                                        o[k] = pool_mul2<BF16>(o[k], f);
+                                        if (FAR) o[k] = pool_mul2<BF16>(o[k], rest);
+                                    }
+                                    put(2 * (q + i) + x, o);
+                                }
+                            }
+                        }
+                    };
+                    if (BF16 ? __vcmpgtu4(sc, 0x86868686u) : __vcmpltu4(sc, 0x67676767u)) chunks(std::true_type{});
+                    else chunks(std::false_type{});
                 };
                 for (int k = 0, n; next_item(k, n); ++k) {
                     P3Item it;

@@ -8,8 +8,7 @@
 // other, are cut into equal shares. Every kv head has the same shares, and blocks of neighbouring heads run side by side (two
 // blocks per SM): in a page the heads' rows of a key lie next to one another, so they are read at about the same time. A block that holds all of
 // a column writes its rows; parts of columns go to the workspace, two at most per block (where its share begins and
-// where it ends), and a second grid joins them: it has a block per head and border between shares, and the first border
-// inside a column belongs to that column.
+// where it ends), and a second grid joins them, its blocks told by the first's in which share a column begins that goes on behind it.
 // In a block each warp has keys of its own, K and V in a ring of stages that it fills ahead of the column it is working on,
 // across columns too; scores and sums run on mma.sync m16n8k16, and the warps' partial results meet in shared memory at a
 // column's end.
@@ -41,6 +40,7 @@ struct PaParams {
     int32_t *status;
     float *part_o;    // [blocks][2][16][d]
     float2 *part_ml;  // [blocks][2][16]: maximum (log 2), sum
+    int4 *part_col;   // [blocks]: a column that begins in this share and goes on behind it (sequence, pack, parts, slot of the first); parts 0: none
     uint32_t b, hq, hkv, group, d, total_q, max_q, max_k, table_cols, alibi_bs;
     float scale, softcap;
     int32_t wl, wr;
@@ -100,15 +100,15 @@ __device__ __forceinline__ uint64_t pa_seq(const PaParams &p, uint32_t b, int un
     return (uint64_t)(uint32_t)(s.uhi - s.ulo) * s.packs;
 }
 
-// Where the block (all of its threads; a multiple of 32, 512 at most) finds unit `target(total)` of all: the sequence and the unit
-// within it. Every thread sums a run of sequences. `scratch`: 18 words of shared memory.
+// Where the block (all of its threads; a multiple of 32, 256 at most) finds unit `target(total)` of all: the sequence and the unit
+// within it. Every thread sums a run of sequences. `scratch`: ten words of shared memory.
 struct PaPlace {
     uint64_t total, per, off;
     uint32_t seq;
 };
 template <typename F>
 __device__ __forceinline__ PaPlace pa_place(const PaParams &p, int unit, uint64_t *scratch, F target) {
-    uint64_t *const s_sum = scratch, *const s_at = scratch + 16;
+    uint64_t *const s_sum = scratch, *const s_at = scratch + 8;
     const uint32_t n = (p.b + blockDim.x - 1) / blockDim.x, first = min(threadIdx.x * n, p.b), last = min(first + n, p.b);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     uint64_t sum = 0;
@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     const uint32_t share = column / p.hkv, hk = column - share * p.hkv;
     PaCursor cur, lead;  // the unit being worked on, and the one to be asked for next
     int nu;
+    uint32_t share_units = 0;
     if (CLUSTER) {
         cur.seq = share;
         cur.pack = 0;
@@ -272,8 +273,10 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     } else {
         const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return share * per; });
         const uint64_t u0 = share * place.per;
+        if (tid == 0 && p.shares > 1) p.part_col[blockIdx.x] = make_int4(0, 0, 0, 0);
         if (u0 >= place.total) return;
         nu = (int)min(place.per, place.total - u0);
+        share_units = (uint32_t)place.per;
         cur.start(p, UNIT, place.seq, place.off);
     }
     lead = cur;
@@ -753,6 +756,9 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         // ---- the end of the column, or of the block's share
         if (!CLUSTER && (cur.u + 1 == cur.s.uhi || t + 1 == nu)) {
             finish(cur, seg_u == cur.s.ulo && cur.u + 1 == cur.s.uhi, 2ull * blockIdx.x + (seg ? 1 : 0));
+            const uint32_t rest = (uint32_t)(cur.s.uhi - cur.u - 1);
+            if (tid == 0 && rest && seg_u == cur.s.ulo)
+                p.part_col[blockIdx.x] = make_int4((int)cur.seq, (int)cur.pack, (int)((rest - 1) / share_units) + 2, (int)(2 * blockIdx.x + (seg ? 1 : 0)));
             ++seg;
             begin = true;
         }
@@ -798,32 +804,23 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     }
 }
 
-// Joins the parts of columns that lie in several shares. Blocks (i, head) stand at the border in front of share i + 1; the first border inside a
-// column is the one that joins it. Its sixteen warps take rows and parts; a row's parts meet in shared memory.
+// Joins the parts of columns that lie in several shares: the block of the share in which a column begins (part_col). Its warps take rows and
+// parts; a row's parts meet in shared memory.
 template <bool BF16>
-__global__ void __launch_bounds__(512) paged_join_kernel(const PaParams p, const int unit) {
+__global__ void __launch_bounds__(512) paged_join_kernel(const PaParams p) {
     __shared__ float s_o[16][256];
     __shared__ float s_l[16], s_m[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    __shared__ uint64_t s_place[18];
-    const uint32_t share = blockIdx.x / p.hkv, hk = blockIdx.x - share * p.hkv;
-    uint64_t border = 0;
-    const PaPlace place = pa_place(p, unit, s_place, [&](uint64_t per) { return border = (share + 1) * per; });
-    PaCursor at;
-    uint64_t first = border, last = border;
-    if (border < place.total) {
-        at.start(p, unit, place.seq, place.off);
-        first = border - (uint64_t)(at.u - at.s.ulo), last = first + (uint64_t)(at.s.uhi - at.s.ulo) - 1;
-    }
-    if (first == border || share * place.per > first) {  // behind the last unit, between two columns, or not the column's first
-        if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid does not end before the one it follows
-        return;
-    }
-    const uint32_t parts = (uint32_t)(last / place.per) - share + 1;
-    const uint32_t row0 = at.pack * PA_ROWS, rows = min((uint32_t)PA_ROWS, at.s.rows - row0);
-    // warps per row, a power of two
-    const uint32_t per_row = rows > 8 ? 1 : (rows > 4 ? 2 : (rows > 2 ? 4 : (rows > 1 ? 8 : 16))), step = 16 / per_row;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 col = p.part_col[blockIdx.x];
+    const uint32_t parts = (uint32_t)col.z, hk = blockIdx.x % p.hkv, row0 = (uint32_t)col.y * PA_ROWS;
+    if (parts == 0) return;
+    const uint32_t q0 = min(p.cu_q[col.x], p.total_q), all = min(min(p.cu_q[col.x + 1], p.total_q) - q0, p.max_q) * p.group, rows = min((uint32_t)PA_ROWS, all - row0);
+    // warps per row, a power of two
+    const uint32_t warps = blockDim.x >> 5;
+    uint32_t per_row = warps;
+    while (per_row > 1 && per_row * rows > warps) per_row /= 2;
+    const uint32_t step = warps / per_row;
     for (uint32_t base = 0; base < rows; base += step) {
         const uint32_t row = base + warp / per_row, sub = warp % per_row;
         float M = -INFINITY, L = 0.0f, o[8];
@@ -836,8 +833,8 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const PaParams p, const
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint32_t part = k0 + k * per_row;
-                    // a share's first segment is in its first slot; the column's first part is that only where column and share begin alike
-                    const uint64_t slot = 2ull * ((share + part) * (uint64_t)p.hkv + hk) + (part == 0 && first != share * place.per ? 1 : 0);
+                    // a share's first segment is in its first slot; the column's first part has the slot that it says
+                    const uint64_t slot = part == 0 ? (uint64_t)col.w : 2ull * (blockIdx.x + part * (uint64_t)p.hkv);
                     const bool in = part < parts;
                     ml[k] = in ? p.part_ml[slot * PA_ROWS + row] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
@@ -890,7 +887,7 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const PaParams p, const
         }
         if (sub == 0 && row < rows) {
             const uint32_t r = row0 + row, tok = r / p.group;
-            char *const orow = p.out + (at.s.q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
+            char *const orow = p.out + (q0 + tok) * p.o_st + (hk * p.group + r - tok * p.group) * p.o_sh;
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
@@ -951,7 +948,7 @@ struct PaPlan {
     int hd, kind, unit;
     uint32_t box;  // rows of a tensor copy, 0: 16-byte chunks
     uint32_t cluster;  // blocks of a cluster per column, 0: shares
-    size_t ws_bytes, off_ml;
+    size_t ws_bytes, off_ml, off_col;
     // the tcgen05 tiles: sequences of more than 16 packed rows
     bool tiles, steps;  // they are launched; the kernel of this file is
     FaParams fa;
@@ -1036,7 +1033,8 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     }
     const size_t slots = (size_t)2 * p.shares * p.hkv;
     pl.off_ml = (slots * PA_ROWS * p.d * 4 + 255) / 256 * 256;
-    pl.ws_bytes = pl.steps && p.shares > 1 ? pl.off_ml + slots * PA_ROWS * 8 : 0;
+    pl.off_col = pl.off_ml + slots * PA_ROWS * 8;
+    pl.ws_bytes = pl.steps && p.shares > 1 ? pl.off_col + slots * 8 : 0;
     if (pl.tiles && pl.fa.n_splits > 1) {
         pl.off_split = (pl.ws_bytes + 255) / 256 * 256;
         pl.off_lse = pl.off_split + (pl.fa.n_splits * pl.fa.rows_total * p.d * 4 + 255) / 256 * 256;
@@ -1080,14 +1078,14 @@ static int pa_launch(const PaPlan &pl, cudaStream_t stream) {
     if (rc || pl.p.shares == 1) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((pl.p.shares - 1) * pl.p.hkv);
-    cfg.blockDim = dim3(512);
+    cfg.blockDim = dim3(pl.p.b * 8 < pl.p.shares ? 512 : 256);  // columns over many shares: more warps for their parts
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<PA<HD, KIND>::BF16>, pl.p, PA<HD, KIND>::UNIT);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<PA<HD, KIND>::BF16>, pl.p);
     if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention (join): %s", cudaGetErrorString(e));
     return check_launch("paged_attention (join)");
 }
@@ -1161,6 +1159,7 @@ extern "C" int b200_paged_attention(const B200PagedAttnArgs *a, b200_stream_t st
             char *ws = static_cast<char *>(a->workspace);
             pl.p.part_o = reinterpret_cast<float *>(ws);
             pl.p.part_ml = reinterpret_cast<float2 *>(ws + pl.off_ml);
+            pl.p.part_col = reinterpret_cast<int4 *>(ws + pl.off_col);
             pl.fa.part_o = reinterpret_cast<float *>(ws + pl.off_split);
             pl.fa.part_lse = reinterpret_cast<float *>(ws + pl.off_lse);
         }

@@ -8,9 +8,10 @@
 // All three kernels are bound by memory: every element is read once and written once, in 16-byte pieces (8 elements a lane), a
 // head's row by neighbouring lanes of one warp. The two elements of a pair that lie rot / 2 apart meet by a shuffle. A warp has
 // one token: its lanes form the token's angles once (in f64: a position of a million times an f32 frequency has 48 bits), keep
-// the eight pairs of theirs in registers and go over the token's heads, the next four rows' loads on their way while four are worked on. Where tokens
+// the eight pairs of theirs in registers and go over the token's heads, four rows' loads on their way at a time. Where tokens
 // are few, a token's rows are shared among several warps, so that one decode step is one wave of short warps.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -38,7 +39,7 @@ int pool_params(const B200PagedPool &pool, const char *what, PoolParams *p) {
     return B200_OK;
 }
 
-constexpr int PR_WARPS = 8;  // per block
+constexpr int PR_WARPS = 4;  // per block
 
 struct RotaryParams {
     const float *freq;
@@ -87,34 +88,53 @@ __device__ __forceinline__ void load8(const char *src, bool vec, Raw<DT> &r) {
         for (int i = 0; i < Raw<DT>::N; ++i) r.w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
     }
 }
+// two elements as a pair of f32: the row kernels are bound by their instructions where rows are many, and multiply two at a time
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float lo2(f32x2 v) { return u2f((uint32_t)v); }
+__device__ __forceinline__ float hi2(f32x2 v) { return u2f((uint32_t)(v >> 32)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
 template <int DT>
-__device__ __forceinline__ void values8(const Raw<DT> &r, float (&x)[8]) {
+__device__ __forceinline__ void values8(const Raw<DT> &r, f32x2 (&x)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (DT == B200_F32) x[i] = u2f(r.w[i % Raw<DT>::N]);
-        else if (DT == B200_BF16) x[i] = i & 1 ? u2f(r.w[i / 2] & 0xffff0000u) : u2f(r.w[i / 2] << 16);
-        else x[i] = f16_bits_to_f((uint16_t)(r.w[i / 2] >> (16 * (i & 1))));
+    for (int i = 0; i < 4; ++i) {
+        if (DT == B200_F32) x[i] = pair2(u2f(r.w[2 * i % Raw<DT>::N]), u2f(r.w[(2 * i + 1) % Raw<DT>::N]));
+        else if (DT == B200_BF16) x[i] = pair2(u2f(r.w[i] << 16), u2f(r.w[i] & 0xffff0000u));
+        else x[i] = pair2(f16_bits_to_f((uint16_t)r.w[i]), f16_bits_to_f((uint16_t)(r.w[i] >> 16)));
     }
 }
 template <int DT>
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+__device__ __forceinline__ uint4 pack8(const f32x2 (&x)[4]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if (DT == B200_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
-        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+        if (DT == B200_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(hi2(x[i])), "f"(lo2(x[i])));
+        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(hi2(x[i])), "f"(lo2(x[i])));
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <int DT>
-__device__ __forceinline__ void store8(char *dst, bool vec, const float (&x)[8]) {
+__device__ __forceinline__ void store8(char *dst, bool vec, const f32x2 (&x)[4]) {
     if (DT == B200_F32) {
         if (vec) {
-            *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4 *>(dst + 16) = make_float4(x[4], x[5], x[6], x[7]);
+            *reinterpret_cast<float4 *>(dst) = make_float4(lo2(x[0]), hi2(x[0]), lo2(x[1]), hi2(x[1]));
+            *reinterpret_cast<float4 *>(dst + 16) = make_float4(lo2(x[2]), hi2(x[2]), lo2(x[3]), hi2(x[3]));
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) reinterpret_cast<float *>(dst)[i] = x[i];
+            for (int i = 0; i < 4; ++i) reinterpret_cast<float *>(dst)[2 * i] = lo2(x[i]), reinterpret_cast<float *>(dst)[2 * i + 1] = hi2(x[i]);
         }
     } else {
         const uint4 w = pack8<DT>(x);
@@ -129,37 +149,41 @@ __device__ __forceinline__ void store8(char *dst, bool vec, const float (&x)[8])
     }
 }
 // eight elements of a block of 32 (four lanes) -> codes and the block's scale; every lane of the row takes part
-__device__ __forceinline__ uint2 mx8(const float (&x)[8], uint32_t &scale) {
-    float m = fabsf(x[0]), z = x[0] * 0.0f;
+__device__ __forceinline__ uint2 mx8(const f32x2 (&x)[4], uint32_t &scale) {
+    float m = 0.0f;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(x[i])), z = fmaf(x[i], 0.0f, z);
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(lo2(x[i])), fabsf(hi2(x[i]))));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     scale = mx_scale_code(m, 8);
-    uint32_t w[2] = {0u, 0u};
-    if (scale != 0) {  // a block of zeros (or with an infinity) has codes of zero
-        const float r = e8m0_recip(scale);
-        if (z != z) {  // a NaN keeps its sign
+    if (scale == 0) return make_uint2(0u, 0u);  // a block of zeros (or with an infinity) has codes of zero
+    const float r = e8m0_recip(scale);
+    uint32_t w[2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i >> 2] |= f_to_e4m3(__fmul_rn(x[i], r)) << (8 * (i & 3));
-        } else {
+    for (int i = 0; i < 2; ++i) {
+        const f32x2 a = mul2(x[2 * i], pair2(r, r)), b = mul2(x[2 * i + 1], pair2(r, r));
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(hi2(a)), "f"(lo2(a)));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(hi2(b)), "f"(lo2(b)));
+        w[i] = lo | (uint32_t)hi << 16;
+    }
+    // a magnitude of 0x7f is a NaN, which keeps its sign
+    if ((((w[0] & 0x7f7f7f7fu) + 0x01010101u) | ((w[1] & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint16_t h;
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(__fmul_rn(x[2 * i + 1], r)), "f"(__fmul_rn(x[2 * i], r)));
-                w[i >> 1] |= (uint32_t)h << (16 * (i & 1));
-            }
-        }
+        for (int i = 0; i < 2; ++i)
+            w[i] = f_to_e4m3(__fmul_rn(lo2(x[2 * i]), r)) | f_to_e4m3(__fmul_rn(hi2(x[2 * i]), r)) << 8 | f_to_e4m3(__fmul_rn(lo2(x[2 * i + 1]), r)) << 16 |
+                   f_to_e4m3(__fmul_rn(hi2(x[2 * i + 1]), r)) << 24;
     }
     return make_uint2(w[0], w[1]);
 }
 
 // TURN: 0 nothing is turned, 1 pairs rot / 2 apart, 2 neighbouring pairs. POOL: 0 none (rotary_axes), 1 16-bit elements, 2 MXFP8;
 // PDT: the 16-bit pool's type. LPR: lanes per row (8, 16 or 32).
-// Measured: see the launcher.
+// Bound by bytes and by latency alike, so the warps that fit count: 64 registers, eight blocks of four warps per SM (three of eight with 80: 46.2 us for
+// 40.0, 8 191 tokens turned and written as MXFP8), and short blocks, since a token or half of one is all that a warp does.
 template <int DT, int TURN, int POOL, int PDT, int LPR>
-__global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsParams p, const bool vec) {
-    constexpr int RPW = 32 / LPR, PR_BATCH = DT == B200_F32 ? 2 : 4;
+__global__ void __launch_bounds__(PR_WARPS * 32, 8) paged_rows_kernel(const RowsParams p, const bool vec) {
+    constexpr int RPW = 32 / LPR, PR_BATCH = 4;
     __shared__ float2 s_cs[PR_WARPS][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % LPR, sub = lane / LPR;
     const uint64_t unit = (uint64_t)blockIdx.x * PR_WARPS + warp;
@@ -168,24 +192,8 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsPar
     const bool in = (uint32_t)c * 8 < p.d;
     const uint32_t half = p.rot.rot / 2;
 
-    // the token's rows: q's heads, k's, v's; this warp's share of them, a batch's loads ahead of the one that is worked on
-    const uint32_t nqk = p.q.heads + p.k.heads, rows = nqk + p.v.heads, step = p.parts * RPW;
-    auto fetch = [&](uint32_t r0, Raw<DT> &w) {
-        const uint32_t r = r0 + sub;
-        if (r < rows && in) {
-            const HeadsParams &h = r < p.q.heads ? p.q : (r < nqk ? p.k : p.v);
-            const uint32_t hd = r < p.q.heads ? r : (r < nqk ? r - p.q.heads : r - nqk);
-            load8<DT>(h.src + token * h.s_t + hd * h.s_h + (uint64_t)c * 8 * dtype_size(DT), vec, w);
-        } else {
-#pragma unroll
-            for (int i = 0; i < Raw<DT>::N; ++i) w.w[i] = 0u;
-        }
-    };
-    Raw<DT> next[PR_BATCH];
-#pragma unroll
-    for (int j = 0; j < PR_BATCH; ++j) fetch(part * RPW + j * step, next[j]);
-
-    float co[8], si[8];
+    const uint32_t step = p.parts * RPW, mine = part * RPW;
+    f32x2 co[4], si[4];
     int partner = lane;
     bool turned = false;
     if (TURN) {
@@ -205,17 +213,17 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsPar
                 const uint32_t f0 = (uint32_t)c * 8 - (second ? half : 0u);
                 partner = second ? lane - (int)(half / 8) : lane + (int)(half / 8);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 cs = s_cs[warp][f0 + i];
-                    co[i] = cs.x;
-                    si[i] = second ? cs.y : -cs.y;
+                for (int i = 0; i < 4; ++i) {
+                    const float2 a = s_cs[warp][f0 + 2 * i], b = s_cs[warp][f0 + 2 * i + 1];
+                    co[i] = pair2(a.x, b.x);
+                    si[i] = second ? pair2(a.y, b.y) : pair2(-a.y, -b.y);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 cs = s_cs[warp][c * 4 + i];
-                    co[2 * i] = co[2 * i + 1] = cs.x;
-                    si[2 * i] = -cs.y, si[2 * i + 1] = cs.y;
+                    co[i] = pair2(cs.x, cs.x);
+                    si[i] = pair2(-cs.y, cs.y);
                 }
             }
         }
@@ -234,58 +242,81 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_rows_kernel(const RowsPar
         }
     }
 
+    // The token's rows, q's heads, then k's, then v's, are dealt out to its warps RPW at a time. One operand's: a batch of loads, then the elements.
+    auto operand = [&](uint32_t first, const HeadsParams &h, auto turn, auto store) {
+        uint32_t r0 = mine;
+        if (first >= r0 + RPW) r0 += (first - r0 - RPW + step) / step * step;  // the first of the warp's that reaches into the operand
+        const char *src = h.src + token * h.s_t + (uint64_t)c * 8 * dtype_size(DT);
 #pragma unroll 1
-    for (uint32_t base = part * RPW; base < rows; base += step * PR_BATCH) {
-        Raw<DT> raw[PR_BATCH];
+        for (; r0 < first + h.heads; r0 += PR_BATCH * step) {
+            Raw<DT> raw[PR_BATCH];
 #pragma unroll
-        for (int j = 0; j < PR_BATCH; ++j) raw[j] = next[j];
+            for (int j = 0; j < PR_BATCH; ++j) {
+                const uint32_t hd = r0 + j * step + sub - first;  // (a row of the operand in front: out of range)
+                if (hd < h.heads && in) load8<DT>(src + hd * h.s_h, vec, raw[j]);
+                else
 #pragma unroll
-        for (int j = 0; j < PR_BATCH; ++j) fetch(base + (PR_BATCH + j) * step, next[j]);
-#pragma unroll
-        for (int j = 0; j < PR_BATCH; ++j) {
-            const uint32_t r0 = base + j * step, r = r0 + sub;
-            if (r0 >= rows) break;  // the whole warp
-            const bool is_v = r >= nqk;
-            float x[8];
-            values8(raw[j], x);
-            if (TURN && r0 < nqk) {
-                float y[8];
-                if (TURN == 1) {
-                    Raw<DT> other;
-#pragma unroll
-                    for (int i = 0; i < Raw<DT>::N; ++i) other.w[i] = __shfl_sync(0xffffffffu, raw[j].w[i], partner);
-                    values8(other, y);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-                }
-                if (turned && !is_v) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], co[i], y[i] * si[i]);
-                }
+                    for (int i = 0; i < Raw<DT>::N; ++i) raw[j].w[i] = 0u;
             }
-            if (r < p.q.heads || (POOL == 0 && r < rows)) {
-                const HeadsParams &h = r < p.q.heads ? p.q : p.k;
-                const uint32_t hd = r < p.q.heads ? r : r - p.q.heads;
-                if (in) store8<DT>(h.dst + token * h.d_t + hd * h.d_h + (uint64_t)c * 8 * dtype_size(DT), vec, x);
+#pragma unroll
+            for (int j = 0; j < PR_BATCH; ++j) {
+                if (r0 + j * step >= first + h.heads) break;  // the whole warp
+                const uint32_t hd = r0 + j * step + sub - first;
+                f32x2 x[4];
+                values8(raw[j], x);
+                if (turn.value) {
+                    f32x2 y[4];
+                    if (TURN == 1) {
+                        Raw<DT> other;
+#pragma unroll
+                        for (int i = 0; i < Raw<DT>::N; ++i) other.w[i] = __shfl_sync(0xffffffffu, raw[j].w[i], partner);
+                        values8(other, y);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = pair2(hi2(x[i]), lo2(x[i]));
+                    }
+                    if (turned) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = fma2(x[i], co[i], mul2(y[i], si[i]));
+                    }
+                }
+                store(hd, hd < h.heads && in, x);
             }
-            if (POOL && r0 + RPW > p.q.heads) {
-                const bool mine = r >= p.q.heads && r < rows && kept && in;
-                const uint32_t hd = is_v ? r - nqk : r - p.q.heads;
-                const PoolParams &pl = p.pool;
-                char *dst = is_v ? pl.v + blk * pl.v_sb + row * pl.v_sr + hd * pl.v_sh : pl.k + blk * pl.k_sb + row * pl.k_sr + hd * pl.k_sh;
-                if (POOL == 1) {
-                    if (mine) *reinterpret_cast<uint4 *>(dst + c * 16) = pack8<PDT>(x);
+        }
+    };
+    using Turn = std::bool_constant<TURN != 0>;
+    auto dense = [&](const HeadsParams &h) {
+        char *dst = h.dst + token * h.d_t + (uint64_t)c * 8 * dtype_size(DT);
+        const uint64_t d_h = h.d_h;
+        return [dst, d_h, vec](uint32_t hd, bool there, const f32x2(&x)[4]) {
+            if (there) store8<DT>(dst + hd * d_h, vec, x);
+        };
+    };
+    if (p.q.heads) operand(0, p.q, Turn{}, dense(p.q));
+    if constexpr (POOL == 0) {
+        if (p.k.heads) operand(p.q.heads, p.k, Turn{}, dense(p.k));
+    } else {
+        auto pool = [&](char *plane, uint64_t sb, uint64_t sr, uint64_t sh, uint8_t *scales) {
+            const uint32_t nb = p.pool.d / 32;
+            char *dst = plane + blk * sb + row * sr + c * (POOL == 1 ? 16 : 8);
+            uint8_t *sc = POOL == 2 ? scales + ((uint64_t)blk * p.pool.hkv * p.pool.block_rows + row) * nb + c / 4 : nullptr;
+            const uint32_t sc_h = p.pool.block_rows * nb;
+            const bool put = kept, first = (c & 3) == 0;
+            return [=](uint32_t hd, bool there, const f32x2(&x)[4]) {
+                if constexpr (POOL == 1) {
+                    if (there && put) *reinterpret_cast<uint4 *>(dst + hd * sh) = pack8<PDT>(x);
                 } else {
                     uint32_t scale;
                     const uint2 w = mx8(x, scale);
-                    if (mine) {
-                        *reinterpret_cast<uint2 *>(dst + c * 8) = w;
-                        if ((c & 3) == 0) (is_v ? pl.vs : pl.ks)[(((uint64_t)blk * pl.hkv + hd) * pl.block_rows + row) * (pl.d / 32) + c / 4] = (uint8_t)scale;
+                    if (there && put) {
+                        *reinterpret_cast<uint2 *>(dst + hd * sh) = w;
+                        if (first) sc[(uint64_t)hd * sc_h] = (uint8_t)scale;
                     }
                 }
-            }
-        }
+            };
+        };
+        operand(p.q.heads, p.k, Turn{}, pool(p.pool.k, p.pool.k_sb, p.pool.k_sr, p.pool.k_sh, p.pool.ks));
+        operand(p.q.heads + p.k.heads, p.v, std::false_type{}, pool(p.pool.v, p.pool.v_sb, p.pool.v_sr, p.pool.v_sh, p.pool.vs));
     }
 }
 
@@ -293,9 +324,10 @@ template <int DT, int TURN, int POOL, int PDT>
 static int rows_launch(const RowsParams &p, bool vec, cudaStream_t stream, const char *what) {
     const uint32_t chunks = p.d / 8, lpr = chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32), rows = p.q.heads + p.k.heads + p.v.heads;
     RowsParams r = p;
-    // a warp goes over a whole token where tokens fill the device; fewer tokens are shared among warps, down to one load a lane
+    // Two waves of warps and more: a warp goes over a whole token. Fewer tokens are shared among warps, down to one load a lane (8 191 tokens: 41.9 us whole,
+    // 40.0 in halves).
     const uint32_t most = std::max(1u, (rows * lpr + 31) / 32);
-    r.parts = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, 148ull * 32 / std::max(p.tokens, 1u)));
+    r.parts = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, 148ull * 32 * 2 / std::max(p.tokens, 1u)));
     const uint64_t blocks = ((uint64_t)p.tokens * r.parts + PR_WARPS - 1) / PR_WARPS;
     if (blocks >= (1ull << 31)) return set_error(B200_ERR_UNSUPPORTED_SHAPE, "%s: %u tokens", what, p.tokens);
     if (lpr == 8) paged_rows_kernel<DT, TURN, POOL, PDT, 8><<<(unsigned)blocks, PR_WARPS * 32, 0, stream>>>(r, vec);
@@ -351,6 +383,7 @@ struct UnpackParams {
     int32_t *status;
 };
 
+// LPR lanes per row, eight elements each (sixteen codes a lane, and with them two stores of every other 16 bytes, took 48.9 us for 45).
 template <int DT, int POOL, int PDT, int LPR>
 __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const UnpackParams p) {
     constexpr int RPW = 32 / LPR, PR_BATCH = 4;
@@ -365,60 +398,68 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const Unpac
     const bool there = id >= 0 && (uint32_t)id < pl.n_blocks, in = (uint32_t)c * 8 < pl.d;
     if (!there && p.status && lane == 0 && part == 0) atomicExch(p.status, 3);
     const uint64_t blk = there ? (uint64_t)id : 0;
-    const uint32_t rows = pl.hkv * (p.v ? 2u : 1u);
-    for (uint32_t base = part * RPW; base < rows; base += p.parts * RPW * PR_BATCH) {
+    // the token's rows, k's heads, then v's
+    const uint32_t nb = pl.d / 32, rows = pl.hkv * (p.v ? 2u : 1u), step = p.parts * RPW;
+    constexpr int PIECE = POOL == 2 ? 8 : 16;
+    const char *k_src = pl.k + blk * pl.k_sb + row * pl.k_sr + c * PIECE, *v_src = pl.v + blk * pl.v_sb + row * pl.v_sr + c * PIECE;
+    const uint64_t sc_at = POOL == 2 ? (blk * pl.hkv * pl.block_rows + row) * nb + c / 4 : 0, to = (t * pl.hkv * pl.d + c * 8) * dtype_size(DT);
+#pragma unroll 1
+    for (uint32_t r0 = part * RPW; r0 < rows; r0 += PR_BATCH * step) {
         uint4 w[PR_BATCH];
         uint32_t e[PR_BATCH];
 #pragma unroll
         for (int i = 0; i < PR_BATCH; ++i) {
-            const uint32_t r = base + i * p.parts * RPW + sub;
-            const bool is_v = r >= pl.hkv;
-            const uint32_t hd = is_v ? r - pl.hkv : r;
+            const uint32_t r = r0 + i * step + sub, hd = r >= pl.hkv ? r - pl.hkv : r;
             w[i] = make_uint4(0u, 0u, 0u, 0u);
-            e[i] = 0;
+            e[i] = 127;
             if (r < rows && in && there) {
-                const char *src = is_v ? pl.v + blk * pl.v_sb + row * pl.v_sr + hd * pl.v_sh : pl.k + blk * pl.k_sb + row * pl.k_sr + hd * pl.k_sh;
+                const char *src = r >= pl.hkv ? v_src + hd * pl.v_sh : k_src + hd * pl.k_sh;
                 if (POOL == 1) {
-                    w[i] = *reinterpret_cast<const uint4 *>(src + c * 16);
+                    w[i] = *reinterpret_cast<const uint4 *>(src);
                 } else {
-                    const uint2 a = *reinterpret_cast<const uint2 *>(src + c * 8);
+                    const uint2 a = *reinterpret_cast<const uint2 *>(src);
                     w[i].x = a.x, w[i].y = a.y;
-                    e[i] = (is_v ? pl.vs : pl.ks)[((blk * pl.hkv + hd) * pl.block_rows + row) * (pl.d / 32) + c / 4];
                 }
+                if (POOL == 2) e[i] = (r >= pl.hkv ? pl.vs : pl.ks)[sc_at + (uint64_t)hd * pl.block_rows * nb];
             }
         }
 #pragma unroll
         for (int i = 0; i < PR_BATCH; ++i) {
-            const uint32_t r = base + i * p.parts * RPW + sub;
+            const uint32_t r = r0 + i * step + sub, hd = r >= pl.hkv ? r - pl.hkv : r;
             if (r >= rows || !in) continue;
-            const bool is_v = r >= pl.hkv;
-            const uint32_t hd = is_v ? r - pl.hkv : r;
-            char *dst = (is_v ? p.v : p.k) + ((t * pl.hkv + hd) * pl.d + c * 8) * dtype_size(DT);
-            if (POOL == 1 && DT == PDT) {
-                *reinterpret_cast<uint4 *>(dst) = w[i];
-                continue;
-            }
-            float x[8];
-            if (POOL == 1) {
-                const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            char *out = (r >= pl.hkv ? p.v : p.k) + to + (uint64_t)hd * pl.d * dtype_size(DT);
+            const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            if constexpr (POOL == 1 && DT == PDT) {
+                *reinterpret_cast<uint4 *>(out) = w[i];
+            } else if constexpr (POOL == 1) {
+                f32x2 x[4];
+                Raw<PDT> raw;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[2 * k] = PDT == B200_BF16 ? bf16_bits_to_f((uint16_t)a[k]) : f16_bits_to_f((uint16_t)a[k]);
-                    x[2 * k + 1] = PDT == B200_BF16 ? bf16_bits_to_f((uint16_t)(a[k] >> 16)) : f16_bits_to_f((uint16_t)(a[k] >> 16));
-                }
+                for (int k = 0; k < 4; ++k) raw.w[k] = a[k];
+                values8<PDT>(raw, x);
+                store8<DT>(out, true, x);
+            } else if (DT != B200_F32 && (DT == B200_BF16 ? e[i] <= 134u : e[i] - 112u <= 30u)) {
+                // a power of two that the type has: the product is exact, or rounded once
+                constexpr bool B = DT == B200_BF16;
+                uint32_t rest;
+                const uint32_t f = pool_scale2<B>(e[i], e[i], rest);
+                uint4 o;
+                o.x = pool_mul2<B>(pool_pair<B, 0>(a[0]), f);
+                o.y = pool_mul2<B>(pool_pair<B, 1>(a[0]), f);
+                o.z = pool_mul2<B>(pool_pair<B, 0>(a[1]), f);
+                o.w = pool_mul2<B>(pool_pair<B, 1>(a[1]), f);
+                *reinterpret_cast<uint4 *>(out) = o;
             } else {
-                const float s = e8m0_to_f(e[i]);
-                const uint32_t a[2] = {w[i].x, w[i].y};
+                const f32x2 s = pair2(e8m0_to_f(e[i]), e8m0_to_f(e[i]));
+                f32x2 x[4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t lo = cvt_e4m3x2_f16x2(a[k]), hi = cvt_e4m3x2_hi_f16x2(a[k]);  // exact
-                    x[4 * k] = f16_bits_to_f((uint16_t)lo) * s;
-                    x[4 * k + 1] = f16_bits_to_f((uint16_t)(lo >> 16)) * s;
-                    x[4 * k + 2] = f16_bits_to_f((uint16_t)hi) * s;
-                    x[4 * k + 3] = f16_bits_to_f((uint16_t)(hi >> 16)) * s;
+                for (int y = 0; y < 2; ++y) {
+                    const uint32_t lo = cvt_e4m3x2_f16x2(a[y]), hi = cvt_e4m3x2_hi_f16x2(a[y]);  // exact
+                    x[2 * y] = mul2(pair2(f16_bits_to_f((uint16_t)lo), f16_bits_to_f((uint16_t)(lo >> 16))), s);
+                    x[2 * y + 1] = mul2(pair2(f16_bits_to_f((uint16_t)hi), f16_bits_to_f((uint16_t)(hi >> 16))), s);
                 }
+                store8<DT>(out, true, x);
             }
-            store8<DT>(dst, true, x);
         }
     }
 }

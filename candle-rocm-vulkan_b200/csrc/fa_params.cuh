@@ -55,6 +55,7 @@ struct FaPages {
     uint32_t tile_rows;  // whole tokens' rows among 256
     uint32_t g_mul, g_shr;  // n / group
     uint32_t box;           // rows of a page that are copied at a time
+    uint32_t classes;       // of sequences by their keys, the longest first
 };
 // Tensor maps of a pool's K and V: boxes of 128-byte columns (64 where a row of codes is no longer) x `rows` rows of a page, swizzled over that
 // width; what lies past the head dim or outside the pool reads as zeros. `order` as in fa_kv_maps. k == null: only whether maps can describe them.

@@ -1124,17 +1124,23 @@ __device__ __forceinline__ void p3_paged_item(const FaParams &p, const FaPages &
     }
 }
 // Owner warp: the sequence, kv head, row tile and key split of item n, counted over the sequences whose rows are this kernel's (a row tile's
-// heads and splits next to one another, the tiles with the most keys first). `base`, `before`: where the last search ended; items
-// mostly come in ascending order. False: there are no more than n.
-__device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, uint32_t n, uint32_t &base, uint32_t &before, int lane, int4 &w) {
-    if (n < before) base = before = 0;
-    for (; base < p.b; base += 32) {
-        const uint32_t seq = base + lane;
+// heads and splits next to one another, the tiles with the most keys first), those of more than half of the bound on the keys first, then of
+// more than a quarter, then the rest (pg.classes 3): an item that starts late should be short. `at`, `before`: where the last search
+// ended (32 sequences of a class); items mostly come in ascending order. False: there are no more than n.
+__device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, uint32_t n, uint32_t &at, uint32_t &before, int lane, int4 &w) {
+    if (n < before) at = before = 0;
+    const uint32_t runs = (p.b + 31) / 32;
+    for (; at < runs * pg.classes; ++at) {
+        const uint32_t cls = at / runs, base = (at - cls * runs) * 32, seq = base + lane;
         uint32_t tiles = 0;
         if (seq < p.b) {
             const uint32_t q0 = min(p.cu_q[seq], pg.total_q), q1 = min(p.cu_q[seq + 1], pg.total_q);
             const uint32_t rows = q1 > q0 ? min(q1 - q0, p.lq) * p.group : 0u;
             if (rows > pg.row_cap) tiles = (rows + pg.tile_rows - 1) / pg.tile_rows;
+            if (pg.classes > 1) {
+                const uint32_t keys = (uint32_t)max(pg.kv_len[seq], 0), mine = keys > p.lk / 2 ? 0u : (keys > p.lk / 4 ? 1u : 2u);
+                if (mine != cls) tiles = 0;
+            }
         }
         const uint32_t per = p.hkv * p.n_splits;
         uint32_t upto = tiles * per;
@@ -1145,9 +1151,9 @@ __device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, ui
         }
         const uint32_t hit = __ballot_sync(0xffffffffu, n - before < upto);
         if (hit) {
-            const int at = __ffs(hit) - 1;
-            const uint32_t rest = n - before - (__shfl_sync(0xffffffffu, upto, at) - __shfl_sync(0xffffffffu, tiles, at) * per), rank = rest / per, hs = rest - rank * per;
-            w = make_int4((int)(base + at), (int)(hs / p.n_splits), (int)(__shfl_sync(0xffffffffu, tiles, at) - 1 - rank), (int)(hs % p.n_splits));
+            const int who = __ffs(hit) - 1;
+            const uint32_t rest = n - before - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, tiles, who) * per), rank = rest / per, hs = rest - rank * per;
+            w = make_int4((int)(base + who), (int)(hs / p.n_splits), (int)(__shfl_sync(0xffffffffu, tiles, who) - 1 - rank), (int)(hs % p.n_splits));
             return true;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -1450,11 +1456,11 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
             // tile of an item has been requested: the answer comes while the tiles in flight are worked on (asked for at an item's
             // start, the early blocks claim too much: 181 against 142 us for 512 items of 1 to 32 tiles).
             const uint64_t k_total = KV == 0 && p.varlen ? p.cu_k[p.b] : 0;
-            uint32_t base = 0, before = 0;  // where the search among the sequences ended
+            uint32_t at = 0, before = 0;  // where the search among the sequences ended
             auto resolve = [&](int n, P3Item &x) {
                 if constexpr (KV == 0) return p3_item(p, gr, (uint32_t)n, x);
                 else {
-                    if (!p3_find(p, pg, (uint32_t)n, base, before, lane, found)) return false;
+                    if (!p3_find(p, pg, (uint32_t)n, at, before, lane, found)) return false;
                     p3_paged_item(p, pg, found, x);
                     return true;
                 }
@@ -1992,6 +1998,7 @@ template <int HD, bool BF16, int KV>
 __global__ void __launch_bounds__(P3<HD, KV>::THREADS, 1) fa_paged_tma_kernel(const FaParams p, const __grid_constant__ CUtensorMap tm_k,
                                                                               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_q,
                                                                               const P3Grid gr, const FaPages pg) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the steps' kernel takes the places that this one leaves
     p3_body<HD, BF16, KV>(p, tm_k, tm_v, tm_q, gr, pg);
 }
 
@@ -2224,10 +2231,11 @@ uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sm
     return (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::min<uint64_t>(sms / paged_items(p, pg), keys / (4 * P3_BN)), 64), 1);
 }
 template <int HD, bool BF16, int KV>
-static int fa_paged_launch_as(const FaParams &p, const FaPages &pg, const P3Grid &gr, const CUtensorMap &tm_k, const CUtensorMap &tm_v, const CUtensorMap &tm_q, cudaStream_t stream) {
+static int fa_paged_launch_as(const FaParams &p, FaPages pg, const P3Grid &gr, const CUtensorMap &tm_k, const CUtensorMap &tm_v, const CUtensorMap &tm_q, cudaStream_t stream) {
     static thread_local bool done[16] = {};
     const int rc = pf_opt_in(fa_paged_tma_kernel<HD, BF16, KV>, P3<HD, KV>::SMEM, done);
     if (rc) return rc;
+    pg.classes = gr.items > 148 ? 3 : 1;  // one wave starts at once
     fa_paged_tma_kernel<HD, BF16, KV><<<gr.items, P3<HD, KV>::THREADS, P3<HD, KV>::SMEM, stream>>>(p, tm_k, tm_v, tm_q, gr, pg);
     return check_launch("paged_attention (tcgen05 tiles)");
 }

@@ -256,6 +256,8 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     }
     if (!CLUSTER && p.shares > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining grid may get ready
     const PoolParams &pl = p.pool;
+    // Behind the tiles' kernel this grid may start before that one has ended (it needs nothing of it): the first block sees that it does not end before.
+    auto in_order = [&]() { if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory"); };
     // which head, and which units: nu of them, every stride-th
     const uint32_t ranks = CLUSTER ? pa_cluster_size() : 1, rank = CLUSTER ? pa_cluster_rank() : 0, column = blockIdx.x / ranks;
     const uint32_t share = column / p.hkv, hk = column - share * p.hkv;
@@ -266,7 +268,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         cur.seq = share;
         cur.pack = 0;
         const int n = (int)pa_seq(p, share, UNIT, cur.s);
-        if (n == 0) return;  // the whole cluster
+        if (n == 0) return in_order();  // the whole cluster
         cur.u = cur.s.ulo + (int)rank;
         cur.enter(p);
         nu = (int)rank < n ? (n - (int)rank - 1) / (int)ranks + 1 : 0;
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         const PaPlace place = pa_place(p, UNIT, reinterpret_cast<uint64_t *>(mg), [&](uint64_t per) { return share * per; });
         const uint64_t u0 = share * place.per;
         if (tid == 0 && p.shares > 1) p.part_col[blockIdx.x] = make_int4(0, 0, 0, 0);
-        if (u0 >= place.total) return;
+        if (u0 >= place.total) return in_order();
         nu = (int)min(place.per, place.total - u0);
         share_units = (uint32_t)place.per;
         cur.start(p, UNIT, place.seq, place.off);
@@ -802,6 +804,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         for (int i = 0; i < C::NS; ++i) mbar_wait_bounded(&bars[i], 0, 1u << 12), mbar_wait_bounded(&bars[i], 1, 1u << 12);  // copies in flight land first
         atomicExch(&g_paged_wait_failed, 1);
     }
+    in_order();
 }
 
 // Joins the parts of columns that lie in several shares: the block of the share in which a column begins (part_col). Its warps take rows and
@@ -1058,11 +1061,17 @@ static int pa_launch_as(const PaPlan &pl, const CUtensorMap &tm_k, const CUtenso
     cfg.blockDim = dim3(PA_THREADS);
     cfg.dynamicSmemBytes = PA<HD, KIND>::SMEM;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = pl.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    if (pl.tiles) {  // behind the tiles' kernel, which reads and writes nothing of this one's
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (MODE == PA_CLUSTER) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = pl.cluster, attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = MODE == PA_CLUSTER ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<HD, KIND, MODE>, pl.p, tm_k, tm_v, order, pl.box);
     if (e != cudaSuccess) return set_error(B200_ERR_LAUNCH, "paged_attention: %s", cudaGetErrorString(e));
     return check_launch("paged_attention");

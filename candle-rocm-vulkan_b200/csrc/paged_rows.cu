@@ -398,75 +398,80 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const Unpac
     const bool there = id >= 0 && (uint32_t)id < pl.n_blocks, in = (uint32_t)c * 8 < pl.d;
     if (!there && p.status && lane == 0 && part == 0) atomicExch(p.status, 3);
     const uint64_t blk = there ? (uint64_t)id : 0;
-    // the token's rows, k's heads, then v's
-    const uint32_t nb = pl.d / 32, rows = pl.hkv * (p.v ? 2u : 1u), step = p.parts * RPW;
-    constexpr int PIECE = POOL == 2 ? 8 : 16;
-    const char *k_src = pl.k + blk * pl.k_sb + row * pl.k_sr + c * PIECE, *v_src = pl.v + blk * pl.v_sb + row * pl.v_sr + c * PIECE;
-    const uint64_t sc_at = POOL == 2 ? (blk * pl.hkv * pl.block_rows + row) * nb + c / 4 : 0, to = (t * pl.hkv * pl.d + c * 8) * dtype_size(DT);
+    // heads part x RPW + sub, and on by the step: k's and v's rows of each, addresses moved by sums alone
+    constexpr int PIECE = POOL == 2 ? 8 : 16, ES = DT == B200_F32 ? 4 : 2;
+    const uint32_t nb = pl.d / 32, step = p.parts * RPW, h0 = part * RPW + sub;
+    const char *k_src = pl.k + blk * pl.k_sb + row * pl.k_sr + h0 * pl.k_sh + c * PIECE, *v_src = pl.v + blk * pl.v_sb + row * pl.v_sr + h0 * pl.v_sh + c * PIECE;
+    const uint64_t k_step = step * pl.k_sh, v_step = step * pl.v_sh;
+    uint64_t sc_at = POOL == 2 ? ((blk * pl.hkv + h0) * pl.block_rows + row) * nb + c / 4 : 0, to = ((t * pl.hkv + h0) * pl.d + c * 8) * ES;
+    const uint32_t sc_step = step * pl.block_rows * nb, to_step = step * pl.d * ES;
+    auto out = [&](char *dst, const uint4 &w, uint32_t e) {
+        if constexpr (POOL == 1 && DT == PDT) {
+            *reinterpret_cast<uint4 *>(dst) = w;
+        } else if constexpr (POOL == 1) {
+            f32x2 x[4];
+            Raw<PDT> raw;
+            raw.w[0] = w.x, raw.w[1] = w.y, raw.w[2] = w.z, raw.w[3] = w.w;
+            values8<PDT>(raw, x);
+            store8<DT>(dst, true, x);
+        } else if (DT != B200_F32 && (DT == B200_BF16 ? e <= 134u : e - 112u <= 30u)) {
+            // a power of two that the type has: the product is exact, or rounded once
+            constexpr bool B = DT == B200_BF16;
+            uint32_t rest;
+            const uint32_t f = pool_scale2<B>(e, e, rest);
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(pool_mul2<B>(pool_pair<B, 0>(w.x), f), pool_mul2<B>(pool_pair<B, 1>(w.x), f), pool_mul2<B>(pool_pair<B, 0>(w.y), f),
+                                                         pool_mul2<B>(pool_pair<B, 1>(w.y), f));
+        } else {
+            const f32x2 s = pair2(e8m0_to_f(e), e8m0_to_f(e));
+            const uint32_t a[2] = {w.x, w.y};
+            f32x2 x[4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const uint32_t lo = cvt_e4m3x2_f16x2(a[y]), hi = cvt_e4m3x2_hi_f16x2(a[y]);  // exact
+                x[2 * y] = mul2(pair2(f16_bits_to_f((uint16_t)lo), f16_bits_to_f((uint16_t)(lo >> 16))), s);
+                x[2 * y + 1] = mul2(pair2(f16_bits_to_f((uint16_t)hi), f16_bits_to_f((uint16_t)(hi >> 16))), s);
+            }
+            store8<DT>(dst, true, x);
+        }
+    };
+    const bool any_v = p.v != nullptr;
 #pragma unroll 1
-    for (uint32_t r0 = part * RPW; r0 < rows; r0 += PR_BATCH * step) {
-        uint4 w[PR_BATCH];
-        uint32_t e[PR_BATCH];
+    for (uint32_t h = h0; h < pl.hkv + sub; h += PR_BATCH * step) {  // (the whole warp)
+        uint4 w[PR_BATCH][2];
+        uint32_t e[PR_BATCH][2];
 #pragma unroll
         for (int i = 0; i < PR_BATCH; ++i) {
-            const uint32_t r = r0 + i * step + sub, hd = r >= pl.hkv ? r - pl.hkv : r;
-            w[i] = make_uint4(0u, 0u, 0u, 0u);
-            e[i] = 127;
-            if (r < rows && in && there) {
-                const char *src = r >= pl.hkv ? v_src + hd * pl.v_sh : k_src + hd * pl.k_sh;
+            const bool load = h + i * step < pl.hkv && in && there;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                w[i][x] = make_uint4(0u, 0u, 0u, 0u);
+                e[i][x] = 127;
+                if (!load || (x && !any_v)) continue;
+                const char *src = x ? v_src : k_src;
                 if (POOL == 1) {
-                    w[i] = *reinterpret_cast<const uint4 *>(src);
+                    w[i][x] = *reinterpret_cast<const uint4 *>(src);
                 } else {
                     const uint2 a = *reinterpret_cast<const uint2 *>(src);
-                    w[i].x = a.x, w[i].y = a.y;
+                    w[i][x].x = a.x, w[i][x].y = a.y;
+                    e[i][x] = (x ? pl.vs : pl.ks)[sc_at];
                 }
-                if (POOL == 2) e[i] = (r >= pl.hkv ? pl.vs : pl.ks)[sc_at + (uint64_t)hd * pl.block_rows * nb];
             }
+            k_src += k_step, v_src += v_step, sc_at += sc_step;
         }
 #pragma unroll
         for (int i = 0; i < PR_BATCH; ++i) {
-            const uint32_t r = r0 + i * step + sub, hd = r >= pl.hkv ? r - pl.hkv : r;
-            if (r >= rows || !in) continue;
-            char *out = (r >= pl.hkv ? p.v : p.k) + to + (uint64_t)hd * pl.d * dtype_size(DT);
-            const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-            if constexpr (POOL == 1 && DT == PDT) {
-                *reinterpret_cast<uint4 *>(out) = w[i];
-            } else if constexpr (POOL == 1) {
-                f32x2 x[4];
-                Raw<PDT> raw;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) raw.w[k] = a[k];
-                values8<PDT>(raw, x);
-                store8<DT>(out, true, x);
-            } else if (DT != B200_F32 && (DT == B200_BF16 ? e[i] <= 134u : e[i] - 112u <= 30u)) {
-                // a power of two that the type has: the product is exact, or rounded once
-                constexpr bool B = DT == B200_BF16;
-                uint32_t rest;
-                const uint32_t f = pool_scale2<B>(e[i], e[i], rest);
-                uint4 o;
-                o.x = pool_mul2<B>(pool_pair<B, 0>(a[0]), f);
-                o.y = pool_mul2<B>(pool_pair<B, 1>(a[0]), f);
-                o.z = pool_mul2<B>(pool_pair<B, 0>(a[1]), f);
-                o.w = pool_mul2<B>(pool_pair<B, 1>(a[1]), f);
-                *reinterpret_cast<uint4 *>(out) = o;
-            } else {
-                const f32x2 s = pair2(e8m0_to_f(e[i]), e8m0_to_f(e[i]));
-                f32x2 x[4];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint32_t lo = cvt_e4m3x2_f16x2(a[y]), hi = cvt_e4m3x2_hi_f16x2(a[y]);  // exact
-                    x[2 * y] = mul2(pair2(f16_bits_to_f((uint16_t)lo), f16_bits_to_f((uint16_t)(lo >> 16))), s);
-                    x[2 * y + 1] = mul2(pair2(f16_bits_to_f((uint16_t)hi), f16_bits_to_f((uint16_t)(hi >> 16))), s);
-                }
-                store8<DT>(out, true, x);
+            if (h + i * step < pl.hkv && in) {
+                out(p.k + to, w[i][0], e[i][0]);
+                if (any_v) out(p.v + to, w[i][1], e[i][1]);
             }
+            to += to_step;
         }
     }
 }
 
 template <int DT, int POOL, int PDT>
 static int unpack_launch(const UnpackParams &p, cudaStream_t stream) {
-    const uint32_t chunks = p.pool.d / 8, lpr = chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32), rows = p.pool.hkv * (p.v ? 2u : 1u);
+    const uint32_t chunks = p.pool.d / 8, lpr = chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32), rows = p.pool.hkv;
     UnpackParams r = p;
     const uint32_t most = std::max(1u, (rows * lpr + 31) / 32);
     r.parts = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, 148ull * 32 / p.total));

@@ -46,6 +46,7 @@ struct PaParams {
     int32_t wl, wr;
     uint32_t shares;  // per kv head; blocks = shares x hkv
     uint32_t row_cap;  // sequences of more packed rows are on the tcgen05 tiles; 0: all are here
+    uint32_t packs;    // the most groups of 16 rows that a sequence has here
 };
 
 // KIND: 0 f16, 1 bf16, 2 MXFP8 under f16 queries, 3 MXFP8 under bf16 queries
@@ -265,10 +266,10 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
     int nu;
     uint32_t share_units = 0;
     if (CLUSTER) {
-        cur.seq = share;
-        cur.pack = 0;
-        const int n = (int)pa_seq(p, share, UNIT, cur.s);
-        if (n == 0) return in_order();  // the whole cluster
+        cur.seq = share / p.packs;
+        cur.pack = share - cur.seq * p.packs;
+        const int n = pa_seq(p, cur.seq, UNIT, cur.s) ? cur.s.uhi - cur.s.ulo : 0;
+        if (n == 0 || cur.pack >= cur.s.packs) return in_order();  // the whole cluster
         cur.u = cur.s.ulo + (int)rank;
         cur.enter(p);
         nu = (int)rank < n ? (n - (int)rank - 1) / (int)ranks + 1 : 0;
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         // the block's rows into its shared memory (the rings: every copy has been waited for), then the cluster's blocks share the outputs
         finish(cur, false, 0);
         pa_cluster_sync();
-        const uint32_t at = smem_u32(smem), pairs = cur.s.rows * (p.d / 2);
+        const uint32_t at = smem_u32(smem), row0 = cur.pack * PA_ROWS, pairs = min((uint32_t)PA_ROWS, cur.s.rows - row0) * (p.d / 2);
         for (uint32_t i = rank * PA_THREADS + tid; i < pairs; i += ranks * PA_THREADS) {
             const uint32_t row = i / (p.d / 2), dd = 2 * (i - row * (p.d / 2));
             float2 ml[8], o[8];
@@ -794,8 +795,8 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                     o1 = fmaf(f, o[k].y, o1);
                 }
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            const uint32_t tok = row / p.group;
-            *reinterpret_cast<uint32_t *>(p.out + (cur.s.q0 + tok) * p.o_st + (hk * p.group + row - tok * p.group) * p.o_sh + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
+            const uint32_t tok = (row0 + row) / p.group;
+            *reinterpret_cast<uint32_t *>(p.out + (cur.s.q0 + tok) * p.o_st + (hk * p.group + row0 + row - tok * p.group) * p.o_sh + dd * 2) = pa_pack2<BF16>(o0 * inv, o1 * inv);
         }
         pa_cluster_sync();  // a block's shared memory is there until all have read it
     }
@@ -992,10 +993,28 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     if (pl.box < 8 || (mx && (p.d != (uint32_t)pl.hd || pl.box * (p.d / 32) % 16)) || !may_map || !fa_pool_maps(p.pool, a->pool.dtype, false, pl.box, nullptr, nullptr, nullptr)) pl.box = 0;
     int sms = 148, dev = 0;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    // Sequences of up to 16 packed rows (one group of mma.sync) are bound by their keys' bytes and stay here, longer ones by products:
-    // the tcgen05 tiles, where these take the call at all. Where all lengths are alike as far as the bounds tell, one kernel has all.
+    const uint64_t rows_max = (uint64_t)a->max_q * p.group, blocks = (uint64_t)sms * (pl.hd == 256 ? 1 : 2);
+    // Columns over few keys: a cluster of up to eight blocks each, as many as are resident at once (clusters do not fill every place: 37 of eight
+    // blocks took two waves, 32 one), up to 1152 keys a block, or 576 where the clusters leave half of the places empty. us, shares
+    // and clusters, 32 / 8 heads of 128 over bf16 (lengths alike; spread evenly up to the longest): 1 x 300 keys 10.2, 7.1; 1 x 2000 14.7,
+    // 10.8; 1 x 4000 16.3, 16.0; 1 x 8000 19.1, 25.9; 8 x 2000 24.2, 17.9 (18.0, 17.0); 8 x 4000 36.5, 30.7 (25.8, 27.3); 16 x 2000 36.7, 30.3
+    // (29.5, 27.1); 16 x 4000 57.3, 52.2 (41.6, 50.9); 37 x 1000 35.7, 31.9 (39.5, 27.2). MXFP8: 8 x 4000 31.5, 26.3 (22.1, 24.3).
+    auto cluster = [&](uint64_t packs, uint32_t keys_half) -> uint32_t {
+        const uint64_t columns = (uint64_t)a->b * p.hkv * packs;
+        if (!pl.box || columns == 0 || columns > blocks) return 0;
+        uint32_t n = 8;
+        while (n > 1 && columns * n > blocks / 8 * 7) n /= 2;
+        return p.max_k <= (uint64_t)(columns * n * 2 > blocks ? keys_half : 576) * n ? n : 0;
+    };
+    // Short sequences stay here, long ones are on the tcgen05 tiles, where these take the call at all: one group of 16 packed rows (of
+    // mma.sync) is bound by its keys' bytes, and so are two under MXFP8, whose tiles are bound by what widens them; small calls of up to four
+    // in clusters (a tile is 23 us from end to end). us, here and there, 32 / 8 heads of 128 over 48 x 4000 keys: bf16 16 rows 138, 215;
+    // 20 rows 254, 215; MXFP8 16 rows 122, 339; 32 rows 220, 340; 64 rows 415, 340. Over 1 x 1000: bf16 16 rows 8.8, 24.0; 64 rows 11.1, 24.3. Where all
+    // lengths are alike as far as the bounds tell, one kernel has all.
+    const uint32_t few = rows_max <= 64 ? cluster((rows_max + PA_ROWS - 1) / PA_ROWS, 576) : 0;
+    const uint32_t cap = few ? 64 : (mx ? 2 * PA_ROWS : PA_ROWS);
     pl.tiles = false, pl.steps = true;
-    if (may_map && (uint64_t)a->max_q * p.group > PA_ROWS) {
+    if (may_map && rows_max > cap) {
         FaParams &f = pl.fa;
         FaPages &g = pl.pg;
         memset(&f, 0, sizeof(f));
@@ -1010,30 +1029,20 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
         g.table = a->table, g.kv_len = a->kv_len, g.status = a->status, g.table_stride = a->table_stride, g.table_cols = a->table_cols;
         g.o_ss = a->out_strides[0], g.o_sh = a->out_strides[1], g.total_q = a->total_q;
         const bool alike = (uint64_t)a->b * a->max_q == a->total_q;
-        g.row_cap = alike ? 0 : PA_ROWS;
+        g.row_cap = alike ? 0 : cap;
         pl.tiles = fa_paged_tiles_take(f, g, a->pool.dtype);
         if (pl.tiles) {
             f.n_splits = fa_paged_tiles_splits(f, g, (uint32_t)sms);
             pl.steps = !alike;
-            p.row_cap = PA_ROWS;
+            p.row_cap = cap;
         }
     }
     // as many shares as two blocks per SM (one at head dim 256), no more than there can be units
-    const uint64_t rows = pl.tiles ? PA_ROWS : (uint64_t)a->max_q * p.group, packs = (rows + PA_ROWS - 1) / PA_ROWS;
+    const uint64_t packs = ((pl.tiles ? cap : rows_max) + PA_ROWS - 1) / PA_ROWS;
     const uint64_t most = std::max<uint64_t>((uint64_t)a->b * packs * ((p.max_k + pl.unit - 1) / pl.unit + 1), 1);
-    p.shares = (uint32_t)std::min<uint64_t>(std::max<uint64_t>((uint64_t)sms * (pl.hd == 256 ? 1 : 2) / p.hkv, 1), most);
-    // Columns over few keys: a cluster of up to eight blocks each, as many as are resident at once (clusters do not fill every place: 37 of eight
-    // blocks took two waves, 32 one), up to 1152 keys a block, or 576 where the clusters leave half of the places empty. us, shares
-    // and clusters, 32 / 8 heads of 128 over bf16 (lengths alike; spread evenly up to the longest): 1 x 300 keys 10.2, 7.1; 1 x 2000 14.7,
-    // 10.8; 1 x 4000 16.3, 16.0; 1 x 8000 19.1, 25.9; 8 x 2000 24.2, 17.9 (18.0, 17.0); 8 x 4000 36.5, 30.7 (25.8, 27.3); 16 x 2000 36.7, 30.3
-    // (29.5, 27.1); 16 x 4000 57.3, 52.2 (41.6, 50.9); 37 x 1000 35.7, 31.9 (39.5, 27.2). MXFP8: 8 x 4000 31.5, 26.3 (22.1, 24.3).
-    const uint64_t blocks = (uint64_t)sms * (pl.hd == 256 ? 1 : 2), columns = (uint64_t)a->b * p.hkv;
-    pl.cluster = 0;
-    if (pl.box && packs == 1 && columns > 0 && columns <= blocks) {
-        uint32_t n = 8;
-        while (n > 1 && columns * n > blocks / 8 * 7) n /= 2;
-        if (p.max_k <= (uint64_t)(columns * n * 2 > blocks ? 1152 : 576) * n) pl.cluster = n;
-    }
+    p.shares = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(blocks / p.hkv, 1), most);
+    p.packs = (uint32_t)packs;
+    pl.cluster = packs == 1 ? cluster(1, 1152) : few;
     const size_t slots = (size_t)2 * p.shares * p.hkv;
     pl.off_ml = (slots * PA_ROWS * p.d * 4 + 255) / 256 * 256;
     pl.off_col = pl.off_ml + slots * PA_ROWS * 8;
@@ -1057,7 +1066,7 @@ static int pa_launch_as(const PaPlan &pl, const CUtensorMap &tm_k, const CUtenso
         if (dev >= 0 && dev < 16) done[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(MODE == PA_CLUSTER ? pl.p.b * pl.p.hkv * pl.cluster : pl.p.shares * pl.p.hkv);
+    cfg.gridDim = dim3(MODE == PA_CLUSTER ? pl.p.b * pl.p.packs * pl.p.hkv * pl.cluster : pl.p.shares * pl.p.hkv);
     cfg.blockDim = dim3(PA_THREADS);
     cfg.dynamicSmemBytes = PA<HD, KIND>::SMEM;
     cfg.stream = stream;

@@ -394,3 +394,91 @@ def test_against_the_gathering_call(P):
     old = P.flash_attn.flash_attn_varlen_paged_windowed(b.q, b.pool.k, b.pool.v, b.cu, cuk, b.table.clamp_min(0), None, 64, 300, 128 ** -0.5, None, 0, 16)
     b.check(b.run(c), c)
     b.check(old, c)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05])
+@pytest.mark.parametrize("lq", [1, 90])
+def test_scales_of_the_scores_that_are_not_positive(P, scale, lq):
+    for form in (None, "mxfp8"):
+        b = Batch(P, [lq, 1], [200, 333], form=form, seed=13)
+        c = P.FlashAttnConfig(scale).causal()
+        b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("n,lq,hq,hkv", [(150, 6, 8, 2), (40, 9, 8, 2), (5, 16, 8, 2), (3, 13, 10, 2), (70, 30, 4, 4)])
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+def test_batches_of_short_chunks(P, n, lq, hq, hkv, form):
+    """Two to four groups of 16 packed rows per sequence, alike and not: the steps' kernel, clusters and tiles by the rule between them."""
+    g = torch.Generator().manual_seed(n)
+    lk = torch.randint(lq, 700, (n,), generator=g).tolist()
+    lens = [lq] * n if n != 40 else [1 + i % lq for i in range(n)]
+    b = Batch(P, lens, lk, hq=hq, hkv=hkv, form=form, seed=n)
+    c = cfg(P, 128)
+    b.check(b.run(c), c)
+
+
+def test_many_chunks_of_all_lengths(P):
+    """More row tiles than the device has places, sequences of each length class, empty ones between."""
+    g = torch.Generator().manual_seed(3)
+    lk = torch.randint(300, 2000, (41,), generator=g).tolist()
+    lq = [0 if i % 7 == 3 else min(k, 40 + 13 * i) for i, k in enumerate(lk)]
+    for form in (None, "mxfp8"):
+        b = Batch(P, lq, lk, hq=16, hkv=4, form=form, dt="f16", page=64, seed=14)
+        c = cfg(P, 128)
+        b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+@pytest.mark.parametrize("lq,lk", [([1] * 3, [700, 90, 400]), ([1] * 60, [2500] * 60), ([300, 1, 40], [900, 800, 3000])])
+def test_the_same_call_gives_the_same_bits(P, form, lq, lk):
+    b = Batch(P, lq, lk, form=form, seed=15)
+    c = cfg(P, 128)
+    want = b.run(c).clone()
+    for _ in range(3):
+        assert torch.equal(b.run(c), want)
+
+
+def test_keys_past_32_bit_offsets(P):
+    """Planes of more than 4 GiB: the last pages' keys are attended over like the first ones'."""
+    n, page, h, d = 2300, 1024, 8, 128
+    k, v = (torch.empty((n, page, h, d), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    pool = P.PagedKvPool.from_tensors(k, v)
+    x = [torch.randn((2, page, h, d), device="cuda").bfloat16() for _ in range(2)]
+    small = P.PagedKvPool.from_tensors(*x)
+    for t, y in zip((k, v), x):
+        t[n - 1], t[n - 2] = y[0], y[1]
+    c = cfg(P, 128)
+    for lq in (1, 200):
+        q = torch.randn((lq, 32, d), device="cuda").bfloat16()
+        cu, lens = torch.tensor([0, lq], device="cuda").int(), torch.tensor([1500], device="cuda").int()
+        far = pool.attention(q, cu, torch.tensor([[n - 1, n - 2]], device="cuda").int(), lens, lq, 1500, c)
+        near = small.attention(q, cu, torch.tensor([[0, 1]], device="cuda").int(), lens, lq, 1500, c)
+        assert torch.equal(far, near)
+
+
+def test_host_refusals(P):
+    b = Batch(P, [1, 2], [20, 40], seed=16)
+    c = cfg(P, 128)
+    run = lambda q=b.q, cu=b.cu, table=b.table, lens=b.kv_len, cfg=c, **k: b.pool.attention(q, cu, table, lens, 2, 40, cfg, **k)
+    run()
+    for bad in (dict(q=b.q[..., :64]), dict(q=b.q[0]), dict(lens=b.kv_len[:1]), dict(table=b.table[:1]), dict(table=b.table[0]), dict(lens=b.kv_len.float()),
+                dict(out=b.q.float()), dict(out=b.q[:2]), dict(out=b.q.transpose(1, 2).contiguous().transpose(1, 2)), dict(cfg=P.FlashAttnConfig(0.1, softcap=0.0)),
+                dict(cfg=P.FlashAttnConfig(0.1, k_descale=2.0)), dict(cfg=P.FlashAttnConfig(0.1, alibi_slopes=torch.ones(3)))):
+        with pytest.raises(ValueError):
+            run(**bad)
+    with pytest.raises(P._abi.B200Error, match="under queries"):
+        run(q=b.q.half())
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        run(q=b.q.to(torch.float64))
+    with pytest.raises(P._abi.B200Error, match="multiple"):
+        run(q=b.q[:, :3].contiguous())
+    p = b.pool
+    k = torch.zeros((4, 2, 128), device="cuda", dtype=torch.bfloat16)
+    slots = torch.arange(4, device="cuda")
+    r = P.RotaryAxes(torch.ones(64))
+    for bad in (dict(k=k[:, :1]), dict(k=k.half()), dict(slots=slots[:3]), dict(slots=slots.float()), dict(rotary=r), dict(q=k), dict(rotary=r, positions=slots[:2]),
+                dict(rotary=P.RotaryAxes(torch.ones(128)), positions=slots), dict(rotary=r, positions=slots, q=k.half())):
+        a = dict(k=k, v=k, slots=slots)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            p.append(**a)

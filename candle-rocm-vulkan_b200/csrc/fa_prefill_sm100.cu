@@ -2226,9 +2226,19 @@ static uint64_t paged_items(const FaParams &p, const FaPages &pg) {
     return std::max<uint64_t>(std::min<uint64_t>(big * tiles, (uint64_t)pg.total_q * p.group / pg.tile_rows + big), 1) * p.hkv;
 }
 uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sms) {
-    // as fa_prefill_sm100_splits; the lengths are bounds here, and splits that find no keys cost a partial result of nothing
-    const uint64_t keys = p.wl >= 0 ? std::min<uint64_t>(p.lk, (uint64_t)p.wl + P3_ROWS) : p.lk;
-    return (uint32_t)std::max<uint64_t>(std::min<uint64_t>(std::min<uint64_t>(sms / paged_items(p, pg), keys / (4 * P3_BN)), 64), 1);
+    // Where the items leave SMs idle: the number of key splits with the least time, a tile at 1.6 us, 3.5 us for the grid that joins them, and the partial rows
+    // written and read (mostly in L2) at 10 TB/s. The lengths are bounds here; splits that find no keys cost a partial result of nothing. us, at least four
+    // tiles a split and this rule, 32 / 8 heads of 128: 20 tokens over 1000 keys 24.2, 14.3; 64 over 2000 25.9, 20.5; 4 x 64 over 1000 27.4, 21.7; 200
+    // over 1000 25.1, 20.6.
+    const uint64_t keys = p.wl >= 0 ? std::min<uint64_t>(p.lk, (uint64_t)p.wl + P3_ROWS) : p.lk, tiles = (keys + P3_BN - 1) / P3_BN;
+    const uint64_t most = std::min<uint64_t>(sms / paged_items(p, pg), 64);
+    uint32_t best = 1;
+    double least = 1.6 * tiles;
+    for (uint32_t n = 2; n <= most; ++n) {
+        const double t = 1.6 * ((tiles + n - 1) / n) + 3.5 + 0.05 * n + (double)p.rows_total * n * p.d * 8 / 1e7;
+        if (t < least) least = t, best = n;
+    }
+    return best;
 }
 template <int HD, bool BF16, int KV>
 static int fa_paged_launch_as(const FaParams &p, FaPages pg, const P3Grid &gr, const CUtensorMap &tm_k, const CUtensorMap &tm_v, const CUtensorMap &tm_q, cudaStream_t stream) {

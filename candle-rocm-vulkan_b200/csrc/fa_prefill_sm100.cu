@@ -1560,8 +1560,9 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                         for (int c0 = 0; c0 < 2 * CH; ++c0) put(c0, o);
                         return;
                     }
-                    auto chunks = [&](auto far_) {
+                    auto chunks = [&](auto far_) {  // true: a NaN among the codes that the short way took for a number
                         constexpr bool FAR = far_.value;
+                        uint32_t most = 0;
 #pragma unroll
                         for (int q = 0; q < CH; q += 4) {
                             uint32_t a[4][4];
@@ -1578,9 +1579,11 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
 #pragma unroll
                                 for (int x = 0; x < 4; ++x) {  // two chunks of 32 elements' codes, eight elements a store
                                     const uint32_t w0 = a[i + x / 2][2 * (x & 1)], w1 = a[i + x / 2][2 * (x & 1) + 1];
-                                    uint32_t o[4] = {pool_pair<BF16, 0>(w0), pool_pair<BF16, 1>(w0), pool_pair<BF16, 0>(w1), pool_pair<BF16, 1>(w1)};
+                                    uint32_t mag[4] = {}, o[4] = {pool_pair<BF16, 0>(w0, mag[0]), pool_pair<BF16, 1>(w0, mag[1]), pool_pair<BF16, 0>(w1, mag[2]), pool_pair<BF16, 1>(w1, mag[3])};
+                                    if (BF16 && !FAR) most = __vimax3_u16x2(__vimax3_u16x2(most, mag[0], mag[1]), mag[2], mag[3]);
 #pragma unroll
                                     for (int k = 0; k < 4; ++k) {
+                                        if (BF16 && FAR && pool_nan(mag[k])) o[k] = pool_nans(o[k], mag[k]);
                                         o[k] = pool_mul2<BF16>(o[k], f);
                                         if (FAR) o[k] = pool_mul2<BF16>(o[k], rest);
                                     }
@@ -1588,9 +1591,9 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                                 }
                             }
                         }
+                        return BF16 && !FAR && pool_nan(most);
                     };
-                    if (BF16 ? __vcmpgtu4(sc, 0x86868686u) : __vcmpltu4(sc, 0x67676767u)) chunks(std::true_type{});
-                    else chunks(std::false_type{});
+                    if ((BF16 ? __vcmpgtu4(sc, 0x86868686u) : __vcmpltu4(sc, 0x67676767u)) || chunks(std::false_type{})) chunks(std::true_type{});
                 };
                 for (int k = 0, n; next_item(k, n); ++k) {
                     P3Item it;

@@ -30,14 +30,22 @@ __device__ __forceinline__ uint32_t pool_mul2(uint32_t a, uint32_t b) {
     return d;
 }
 // E4M3 codes as pairs of values: f16, or bf16 times 2^-120 (a code's exponent and mantissa in the places of a bf16's, its subnormals
-// among that type's). pool_codes4: the bytes of two words, pair by pair; pool_pair: bytes 2 I and 2 I + 1 of one.
+// among that type's). A NaN is the code 0x7f, which the move makes 480: pool_codes4 puts a NaN there, pool_pair leaves the codes' magnitudes in
+// `mag` for a look at all of a row at once (pool_nan). pool_codes4: the bytes of two words, pair by pair; pool_pair: bytes 2 I and 2 I + 1 of one.
+// whether the magnitudes (or their maximum, lane by lane) are a NaN's; the pair x with NaNs where they are
+__device__ __forceinline__ bool pool_nan(uint32_t mag) { return ((mag + 0x00100010u) & 0x08000800u) != 0; }
+__device__ __forceinline__ uint32_t pool_nans(uint32_t x, uint32_t mag) {
+    const uint32_t nan = (mag + 0x00100010u) & 0x08000800u;
+    return x | ((nan << 4) - (nan >> 4));
+}
 template <bool BF16>
 __device__ __forceinline__ void pool_codes4(uint32_t lo, uint32_t hi, uint32_t (&x)[4]) {
     if (BF16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t t = __byte_perm(lo, hi, (4u + i) << 12 | i << 4);
-            x[i] = (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+            const uint32_t mag = (t >> 4) & 0x07f007f0u;
+            x[i] = pool_nans((t & 0x80008000u) | mag, mag);
         }
     } else {
         const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);
@@ -46,10 +54,11 @@ __device__ __forceinline__ void pool_codes4(uint32_t lo, uint32_t hi, uint32_t (
     }
 }
 template <bool BF16, int I>
-__device__ __forceinline__ uint32_t pool_pair(uint32_t w) {
+__device__ __forceinline__ uint32_t pool_pair(uint32_t w, uint32_t &mag) {
     if (BF16) {
         const uint32_t t = __byte_perm(w, w, (2u * I + 1u) << 12 | (2u * I) << 4);
-        return (t & 0x80008000u) | ((t >> 4) & 0x07f007f0u);
+        mag = (t >> 4) & 0x07f007f0u;
+        return (t & 0x80008000u) | mag;
     }
     return I ? cvt_e4m3x2_hi_f16x2(w) : cvt_e4m3x2_f16x2(w);
 }
@@ -59,7 +68,7 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t pool_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
     if (BF16) {
         const uint32_t m0 = min(e0, 134u), m1 = min(e1, 134u);
-        rest = (e0 - m0 + 127u) << 7 | (e1 - m1 + 127u) << 23;
+        rest = (e0 == 255u ? 255u : e0 - m0 + 127u) << 7 | (e1 == 255u ? 255u : e1 - m1 + 127u) << 23;  // (255 is an infinity, as for e8m0_to_f)
         return (m0 + 120u) << 7 | (m1 + 120u) << 23;
     }
     const uint32_t m0 = max(e0, 103u), m1 = max(e1, 103u);

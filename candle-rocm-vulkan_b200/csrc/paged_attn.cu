@@ -370,6 +370,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                 } else {
                     if (p.status) atomicExch(p.status, 3);
                     for (uint32_t i = 0; i < box * C::NB; ++i) at[i] = at[KEYS * C::NB + i] = 127;  // zeros times one
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a later copy goes over them
                 }
             } else if (id < 0 && p.status) {
                 atomicExch(p.status, 3);
@@ -1044,6 +1045,7 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
     p.packs = (uint32_t)packs;
     pl.cluster = packs == 1 ? cluster(1, 1152) : few;
     const size_t slots = (size_t)2 * p.shares * p.hkv;
+    pl.off_split = pl.off_lse = 0;
     pl.off_ml = (slots * PA_ROWS * p.d * 4 + 255) / 256 * 256;
     pl.off_col = pl.off_ml + slots * PA_ROWS * 8;
     pl.ws_bytes = pl.steps && p.shares > 1 ? pl.off_col + slots * 8 : 0;

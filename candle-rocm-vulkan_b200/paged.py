@@ -53,6 +53,14 @@ def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:
     return t if t.stride()[-1] == 1 or t.numel() <= 1 else t.contiguous()
 
 
+def _word(status: Optional[torch.Tensor], device) -> int:
+    if status is None:
+        return 0
+    if status.dtype != torch.int32 or status.device != device or status.numel() == 0:
+        raise ValueError(f"status must be an int32 tensor on {device}, got {status.dtype} {tuple(status.shape)} on {status.device}")
+    return status.data_ptr()
+
+
 # A decode step's calls are host time before they are anything else, so a tensor is asked for its shape and strides once, and outputs are made
 # the quickest way torch has (empty_like and empty_strided: 1.1 us, empty: 2 to 4).
 def _heads(t: torch.Tensor, what: str, tokens: Optional[int] = None, d: Optional[int] = None):
@@ -243,7 +251,7 @@ class PagedKvPool:
             fields = _NO_ROTARY
         _call(_lib().b200_paged_append, self._packed + _APPEND_ARGS.pack(
             k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), qp, qop, qs[0], qs[1], qos[0], qos[1], tokens, hq, _float_id(k), 0,
-            *fields, status.data_ptr() if status is not None else 0), dev)
+            *fields, _word(status, dev)), dev)
         return qo
 
     def _table(self, table: torch.Tensor, b: int, what: str) -> torch.Tensor:
@@ -267,7 +275,7 @@ class PagedKvPool:
         v = torch.empty_like(k)
         _call(_lib().b200_paged_unpack, self._packed + _UNPACK_ARGS.pack(
             table.data_ptr(), table.stride()[0], cu.data_ptr(), k.data_ptr(), v.data_ptr(), total, b, table.shape[1], _float_id(k), 0,
-            status.data_ptr() if status is not None else 0), dev)
+            _word(status, dev)), dev)
         return k, v
 
     def attention(self, q: torch.Tensor, seqlens_q: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
@@ -277,7 +285,8 @@ class PagedKvPool:
         chunk of a prompt; its keys are the first kv_len[i] of its pages, the new tokens' (written before) among them. Masks are
         bottom-right aligned as for `flash_attn_varlen`; rows without a visible key give zeros. The lengths are read on the device;
         `max_seqlen_q` and `max_seqlen_k` bound them (longer ones are cut). Rows of `out` (a new tensor unless given) behind the last
-        sequence are left as they were. Page numbers outside the pool hold zeros and set `status` (an int32 device tensor) to 3."""
+        sequence are left as they were; `out` must not overlap `q`. Page numbers outside the pool hold zeros and set `status` (an int32 device
+        tensor) to 3. MXFP8 values count as q's type holds them (f16: up to 65504, as far as sums of weights with them go)."""
         dev = self.device
         q, (total, hq, _), qs = _heads(q, "paged attention: q", None, self.head_dim)
         if q.device != dev:
@@ -303,7 +312,7 @@ class PagedKvPool:
         wl, wr = cfg.window_i32()
         fields = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], cu.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride()[0],
                   b, total, int(max_seqlen_q), int(max_seqlen_k), hq, table.shape[1], _float_id(q), cfg.softmax_scale, softcap, wl, wr, ap, abs_, 0)
-        st = status.data_ptr() if status is not None else 0
+        st = _word(status, dev)
         lib = _lib()
         if not _capturing():
             # the stream's scratch as it is; the library says where it is too small

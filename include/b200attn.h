@@ -563,7 +563,8 @@ int b200_paged_unpack(const B200PagedUnpackArgs *args, b200_stream_t stream);
  * without a visible key give zeros; scores scale * q . k, then softcap (> 0) and ALiBi. All lengths are read on the
  * device: nothing synchronises, and a captured call follows them. max_q, max_k and the table's columns bound the lengths (longer
  * ones are cut) and size the launches; total_q bounds cu_q[b], and rows of `out` behind cu_q[b] are left as they were. q and out of q_dtype
- * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows.
+ * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows; out does not overlap q. An MXFP8
+ * pool's values count as q_dtype holds them (f16: an infinity above 65504).
  * The reference gathers the pages on the host (candle-flash-attn/src/lib.rs:341-420). */
 typedef struct B200PagedAttnArgs {
     B200PagedPool pool;

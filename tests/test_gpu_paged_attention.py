@@ -482,3 +482,30 @@ def test_host_refusals(P):
         a.update(bad)
         with pytest.raises(ValueError):
             p.append(**a)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("lq", [1, 40, 300])
+@pytest.mark.parametrize("far", [False, True])
+def test_a_nan_among_codes_shows(P, dt, lq, far):
+    """A code of NaN (and, under bf16 queries, one behind a scale that takes two factors) is a NaN to every row that sees it."""
+    b = Batch(P, [lq], [700], dt=dt, form="mxfp8")
+    c = cfg(P, b.d, wr=None)
+    clean = b.run(c)
+    page, row = int(b.table[0, 333 // b.page]), 333 % b.page
+    b.pool.v.view(torch.uint8)[page, row, 1, 37] = 0xff
+    if far:
+        e = 140 if dt == "bf16" else 90
+        b.pool.v.view(torch.uint8)[page, row, 1, 32:64] = torch.where(torch.arange(32, device="cuda") == 5, 0xff, 0).to(torch.uint8)
+        b.pool.v_scale[page, 1, row, 1] = e
+    out = b.run(c)
+    assert bool(out[:, 4:, 37].isnan().all())
+    assert int(out.isnan().sum()) == 4 * lq
+    assert bool((out[:, :4] == clean[:, :4]).all())
+    b.pool.k.view(torch.uint8)[page, row, 0, 0] = 0x7f
+    if far:
+        b.pool.k_scale[page, 0, row, 0] = 140 if dt == "bf16" else 90
+    out = b.run(c)
+    assert bool(out[:, :4].isnan().all())
+    assert bool(out[:, 4:, 37].isnan().all())
+    assert int(out.isnan().sum()) == lq * (4 * b.d + 4)

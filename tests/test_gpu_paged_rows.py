@@ -307,3 +307,17 @@ def test_rows_in_a_graph_and_on_another_stream(P):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0][slots], want[0][slots - 1])
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("e", [0, 60, 104, 112, 127, 134, 135, 142, 143, 200, 254])
+def test_every_code_reads_as_its_value(P, dt, e):
+    """All 256 codes, NaNs (0x7f and 0xff) among them, behind a scale: rounded once to the output's type."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").repeat(2).reshape(2, 1, 2, 128)
+    scale = torch.full((2, 2, 1, 4), e, dtype=torch.uint8, device="cuda")
+    pool = P.PagedKvPool.from_tensors(codes.view(torch.float8_e4m3fn), codes.flip(-1).contiguous().view(torch.float8_e4m3fn), scale, scale)
+    k, v = pool.keys_values(torch.tensor([[1, 0]], dtype=torch.int32, device="cuda"), torch.tensor([0, 2], dtype=torch.int32, device="cuda"), 2, DT[dt])
+    for x, plane in ((k, pool.k), (v, pool.v)):
+        want = (plane.float().double() * 2.0 ** (e - 127)).to(DT[dt]).flatten(0, 1)
+        assert bool(((x == want) | (x.isnan() & want.isnan())).all())
+        assert int(x.isnan().sum()) == 4

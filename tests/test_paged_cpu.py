@@ -193,3 +193,15 @@ def test_attention_workspace(P):
     assert 0 < need() <= need(b=500, total_q=500, max_k=1 << 20) <= 64 << 20
     assert need(hq=7) == 0 and A.lib().b200_paged_attention_workspace_bytes(None) == 0
     assert A.lib().b200_paged_attention(C.byref(attn(A, b=0, q=None)), None) == 0 and A.lib().b200_paged_attention(None, None) == -1
+
+
+def test_status_words(P):
+    """A status word that the kernels could not write is refused before any launch."""
+    from candle_rocm_vulkan_b200 import paged
+    cpu = torch.device("cpu")
+    assert paged._word(None, cpu) == 0
+    ok = torch.zeros(1, dtype=torch.int32)
+    assert paged._word(ok, cpu) == ok.data_ptr()
+    for bad, dev in ((ok.long(), cpu), (ok, torch.device("cuda:0")), (ok[:0], cpu)):
+        with pytest.raises(ValueError, match="status"):
+            paged._word(bad, dev)

@@ -1,8 +1,9 @@
 // Prefill attention tiles on the 5th generation tensor cores (tcgen05, accumulators in tensor memory), f16 or bf16. Query
 // rows are packed (row = token * group + head in group, so the heads that share a kv head also share every K / V tile).
-// Three kernels:
+// Four kernels:
 //   fa_prefill_tma_kernel<64 | 128>  head dims up to 128, any tensors that tensor maps describe (groups of a power of two):
 //              256 rows per work item, tiles by tensor copies. Everything usual runs here.
+//   fa_paged_tma_kernel<64 | 128>    the same over a pool of cache pages, 16-bit or MXFP8.
 //   fa_prefill_sm100_kernel2         head dim 128, 1024 rows and more that no map describes: 16-byte chunk copies.
 //   fa_prefill_sm100_kernel          the same from 512 rows on: 128 rows per block.
 //
@@ -977,7 +978,9 @@ __global__ void __launch_bounds__(P2_THREADS, 1) fa_prefill_sm100_kernel2(const 
 // ---------------------------------------------------------------------------------------------
 constexpr int P3_THREADS = 384, P3_ROWS = 256, P3_BN = 128, P3_LOADER = 8, P3_ISSUER = 9, P3_OWNER = 11;
 // KV, where keys and values come from: 0 tensors, 1 pages of 16-bit elements, 2 MXFP8 pages (fa_paged_tma_kernel). Warps 12-15 of
-// the last widen the codes: one stage of raw tiles lies where the others stage their output rows.
+// the last widen the codes: one stage of raw tiles lies where the others stage their output rows. Measured, 2048 tokens over 16384 keys, 32 / 8 heads of
+// 128, TFLOP/s: tensors 1 029; pages of 128 rows 1 027, of 16 rows 1 000; MXFP8 under f16 queries 937, under bf16 886. What bounds MXFP8 beside what bounds the
+// others: the widening warps share the SM's schedulers with the exponentials.
 template <int HD, int KV = 0>
 struct P3 {
     static constexpr int THREADS = KV == 2 ? 512 : P3_THREADS;
@@ -1546,8 +1549,9 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                     }
                 };
                 // Row `key` of a raw tile, or zeros, into the layout of the tensor copies. One warp per SM quadrant widens all of a tile's keys while
-                // two others compute exponentials, so it is its instructions that count: four chunks of codes at a time, one multiplier
-                // per 32 elements; rows with a scale outside the type's range (pool_scale2) apart.
+                // two others compute exponentials, so its instructions count, and more than they the places that they take in the instruction cache:
+                // short loops over four chunks of codes, one body for K and V, are faster than straight code (2048 tokens over 16384 keys, 32 / 8 heads
+                // of 128: f16 907 -> 942 TFLOP/s, bf16 740 -> 886). One multiplier per 32 elements; f16 rows with a scale below 2^-24 apart.
                 auto widen = [&](uint32_t raw, uint32_t dst, uint32_t sc, bool zero) {
                     constexpr int CH = HD / 16;  // raw chunks of 16 codes
                     const uint32_t row = raw + key * HD, out = dst + key * 128, sw = HD == 64 ? (key >> 1) & 3 : key & 7;
@@ -1560,10 +1564,23 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                         for (int c0 = 0; c0 < 2 * CH; ++c0) put(c0, o);
                         return;
                     }
-                    auto chunks = [&](auto far_) {  // true: a NaN among the codes that the short way took for a number
-                        constexpr bool FAR = far_.value;
-                        uint32_t most = 0;
+                    auto far = [&]() {  // two factors
+#pragma unroll 1
+                        for (int q = 0; q < CH; ++q) {
+                            uint32_t a[4], rest;
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(row + ((q ^ sw) << 4)));
+                            const uint32_t e = (sc >> (4 * (q & ~1))) & 0xffu, f = pool_scale2<BF16>(e, e, rest);
 #pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                uint32_t o[4] = {pool_pair<BF16, 0>(a[2 * x]), pool_pair<BF16, 1>(a[2 * x]), pool_pair<BF16, 0>(a[2 * x + 1]), pool_pair<BF16, 1>(a[2 * x + 1])};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) o[k] = pool_mul2<BF16>(pool_mul2<BF16>(o[k], f), rest);
+                                put(2 * q + x, o);
+                            }
+                        }
+                    };
+                    auto chunks = [&]() {
+#pragma unroll 1
                         for (int q = 0; q < CH; q += 4) {
                             uint32_t a[4][4];
 #pragma unroll
@@ -1572,28 +1589,21 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
 #pragma unroll
                             for (int i = 0; i < 4; i += 2) {
                                 const uint32_t e = (sc >> (4 * (q + i))) & 0xffu;
-                                uint32_t rest = 0, f;
-                                if (FAR) f = pool_scale2<BF16>(e, e, rest);
-                                else if (BF16) f = ((e + 120u) << 7) * 0x10001u;
-                                else f = pack_f16x2(u2f(e << 23), u2f(e << 23));
+                                uint32_t rest;
+                                const uint32_t f = BF16 ? pool_scale2<BF16>(e, e, rest) : pack_f16x2(u2f(e << 23), u2f(e << 23));
 #pragma unroll
                                 for (int x = 0; x < 4; ++x) {  // two chunks of 32 elements' codes, eight elements a store
                                     const uint32_t w0 = a[i + x / 2][2 * (x & 1)], w1 = a[i + x / 2][2 * (x & 1) + 1];
-                                    uint32_t mag[4] = {}, o[4] = {pool_pair<BF16, 0>(w0, mag[0]), pool_pair<BF16, 1>(w0, mag[1]), pool_pair<BF16, 0>(w1, mag[2]), pool_pair<BF16, 1>(w1, mag[3])};
-                                    if (BF16 && !FAR) most = __vimax3_u16x2(__vimax3_u16x2(most, mag[0], mag[1]), mag[2], mag[3]);
+                                    uint32_t o[4] = {pool_pair<BF16, 0>(w0), pool_pair<BF16, 1>(w0), pool_pair<BF16, 0>(w1), pool_pair<BF16, 1>(w1)};
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k) {
-                                        if (BF16 && FAR && pool_nan(mag[k])) o[k] = pool_nans(o[k], mag[k]);
-                                        o[k] = pool_mul2<BF16>(o[k], f);
-                                        if (FAR) o[k] = pool_mul2<BF16>(o[k], rest);
-                                    }
+                                    for (int k = 0; k < 4; ++k) o[k] = pool_mul2<BF16>(o[k], f);
                                     put(2 * (q + i) + x, o);
                                 }
                             }
                         }
-                        return BF16 && !FAR && pool_nan(most);
                     };
-                    if ((BF16 ? __vcmpgtu4(sc, 0x86868686u) : __vcmpltu4(sc, 0x67676767u)) || chunks(std::false_type{})) chunks(std::true_type{});
+                    if (!BF16 && __vcmpltu4(sc, 0x67676767u)) far();
+                    else chunks();
                 };
                 for (int k = 0, n; next_item(k, n); ++k) {
                     P3Item it;
@@ -1605,7 +1615,7 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                         const uint32_t ph = ((kv / NS) - 1) & 1;
                         if (t + 1 < it.ntiles) scales(it, j0 + P3_BN, ks1, vs1);
                         const bool hidden = j0 + key < it.v_lo || j0 + key >= it.t_hi;
-#pragma unroll
+#pragma unroll 1
                         for (int x = 0; x < 2; ++x) {
                             if (!(ok = p3_wait(bar0 + 8 * (C::RF + x), kv & 1, abort_flag))) break;
                             if (kv >= NS && !(ok = p3_wait(bar0 + 8 * ((x ? C::VE : C::KE) + st), ph, abort_flag))) break;

@@ -29,47 +29,32 @@ __device__ __forceinline__ uint32_t pool_mul2(uint32_t a, uint32_t b) {
     else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-// E4M3 codes as pairs of values: f16, or bf16 times 2^-120 (a code's exponent and mantissa in the places of a bf16's, its subnormals
-// among that type's). A NaN is the code 0x7f, which the move makes 480: pool_codes4 puts a NaN there, pool_pair leaves the codes' magnitudes in
-// `mag` for a look at all of a row at once (pool_nan). pool_codes4: the bytes of two words, pair by pair; pool_pair: bytes 2 I and 2 I + 1 of one.
-// whether the magnitudes (or their maximum, lane by lane) are a NaN's; the pair x with NaNs where they are
-__device__ __forceinline__ bool pool_nan(uint32_t mag) { return ((mag + 0x00100010u) & 0x08000800u) != 0; }
-__device__ __forceinline__ uint32_t pool_nans(uint32_t x, uint32_t mag) {
-    const uint32_t nan = (mag + 0x00100010u) & 0x08000800u;
-    return x | ((nan << 4) - (nan >> 4));
+// E4M3 codes as pairs of values, exact, NaNs among them. pool_codes4: the bytes of two words, pair by pair; pool_pair: bytes 2 I and 2 I + 1 of one.
+// To bf16 by way of f16 and f32, whose instructions are spread over the pipes (the code's bits moved to a bf16's places, with a look for NaNs: 638 for 740
+// TFLOP/s of fa_paged_tma_kernel).
+template <bool BF16>
+__device__ __forceinline__ uint32_t pool_f16_as(uint32_t h) {
+    if (!BF16) return h;
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(f16_bits_to_f((uint16_t)(h >> 16))), "f"(f16_bits_to_f((uint16_t)h)));
+    return d;
 }
 template <bool BF16>
 __device__ __forceinline__ void pool_codes4(uint32_t lo, uint32_t hi, uint32_t (&x)[4]) {
-    if (BF16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t t = __byte_perm(lo, hi, (4u + i) << 12 | i << 4);
-            const uint32_t mag = (t >> 4) & 0x07f007f0u;
-            x[i] = pool_nans((t & 0x80008000u) | mag, mag);
-        }
-    } else {
-        const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);
-        x[0] = cvt_e4m3x2_f16x2(a), x[1] = cvt_e4m3x2_hi_f16x2(a);
-        x[2] = cvt_e4m3x2_f16x2(b), x[3] = cvt_e4m3x2_hi_f16x2(b);
-    }
+    const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);
+    x[0] = pool_f16_as<BF16>(cvt_e4m3x2_f16x2(a)), x[1] = pool_f16_as<BF16>(cvt_e4m3x2_hi_f16x2(a));
+    x[2] = pool_f16_as<BF16>(cvt_e4m3x2_f16x2(b)), x[3] = pool_f16_as<BF16>(cvt_e4m3x2_hi_f16x2(b));
 }
 template <bool BF16, int I>
-__device__ __forceinline__ uint32_t pool_pair(uint32_t w, uint32_t &mag) {
-    if (BF16) {
-        const uint32_t t = __byte_perm(w, w, (2u * I + 1u) << 12 | (2u * I) << 4);
-        mag = (t >> 4) & 0x07f007f0u;
-        return (t & 0x80008000u) | mag;
-    }
-    return I ? cvt_e4m3x2_hi_f16x2(w) : cvt_e4m3x2_f16x2(w);
+__device__ __forceinline__ uint32_t pool_pair(uint32_t w) {
+    return pool_f16_as<BF16>(I ? cvt_e4m3x2_hi_f16x2(w) : cvt_e4m3x2_f16x2(w));
 }
-// The multiplier that takes such a pair to its values, for the scales e0 and e1: f16 2^(e - 127), bf16 2^(e - 127 + 120). Scales outside the
-// type's range (f16 e < 103, bf16 e > 134) go in two steps: `rest` is the second.
+// The multiplier 2^(e - 127) of such a pair, for the scales e0 and e1. bf16 has all of them; f16's below e = 103 go in two steps: `rest` is the second.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pool_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
     if (BF16) {
-        const uint32_t m0 = min(e0, 134u), m1 = min(e1, 134u);
-        rest = (e0 == 255u ? 255u : e0 - m0 + 127u) << 7 | (e1 == 255u ? 255u : e1 - m1 + 127u) << 23;  // (255 is an infinity, as for e8m0_to_f)
-        return (m0 + 120u) << 7 | (m1 + 120u) << 23;
+        rest = 0x3f803f80u;
+        return (e0 ? e0 << 7 : 0x40u) | (e1 ? e1 << 7 : 0x40u) << 16;
     }
     const uint32_t m0 = max(e0, 103u), m1 = max(e1, 103u);
     rest = pack_f16x2(e8m0_to_f(e0 + 127u - m0), e8m0_to_f(e1 + 127u - m1));

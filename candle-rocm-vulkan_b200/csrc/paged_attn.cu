@@ -13,6 +13,11 @@
 // across columns too; scores and sums run on mma.sync m16n8k16, and the warps' partial results meet in shared memory at a
 // column's end.
 //
+// Measured (32 / 8 heads of 128; copy bandwidth 6 470 GB/s): 64 sequences of 500 to 8192 keys, bf16, 185 us, 0.95 of the copy; 48 x 4 tokens over
+// 4000 to 30000 keys, MXFP8, 387 us, 0.69: there the loads alone take 281 and the instructions alone 278, on two blocks of four warps per SM, which is
+// what the registers hold. A fifth warp per block for the copies (463: its registers come from the others), E4M3 operands for the scores with q in two parts
+// (477) and the code without its rare forms (380) were tried.
+//
 // MXFP8 keys and values stay codes up to the registers. Scores: the codes are exact in f16; q is taken to f16 behind a power of
 // two per row (a bf16 element keeps its eight bits unless it is 2^28 below the row's largest), and a block of 32 elements adds its
 // sum times its scale in f32. Values and weights: see the products. Weights are rounded to 16 bits (f16 2^-11, bf16 2^-8 at most each, and these
@@ -689,7 +694,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
         } else {
             // Column n = g of the products' tile i is element g HD / 8 + i: a lane reads the same bytes of its four keys. Values and weights in f16, also
             // under bf16 queries (the codes times 2^k with k from -22 to 7 are within 2^-11 of a block's largest there, and weights have three bits
-            // more); tiles with scales outside that take the second form: two factors, and bf16 under bf16 queries.
+            // more); tiles with scales outside that take the second form: two factors, or bf16 under bf16 queries.
             constexpr int W = HD / 32;  // words of a lane's elements
             const uint32_t vsc = tsc + KEYS * C::NB + g * (HD / 8) / 32;
             uint32_t e[KG][4], off = 0;
@@ -727,7 +732,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
 #pragma unroll
                                 for (int y = 0; y < 4; ++y) {
                                     b[k][y] = pool_mul2<B>(b[k][y], f[k]);
-                                    if (FAR) b[k][y] = pool_mul2<B>(b[k][y], rest[k]);
+                                    if (FAR && !B) b[k][y] = pool_mul2<B>(b[k][y], rest[k]);
                                 }
                             }
 #pragma unroll
@@ -1008,9 +1013,9 @@ static int pa_plan(const B200PagedAttnArgs *a, PaPlan &pl, bool may_map = true) 
         return p.max_k <= (uint64_t)(columns * n * 2 > blocks ? keys_half : 576) * n ? n : 0;
     };
     // Short sequences stay here, long ones are on the tcgen05 tiles, where these take the call at all: one group of 16 packed rows (of
-    // mma.sync) is bound by its keys' bytes, and so are two under MXFP8, whose tiles are bound by what widens them; small calls of up to four
-    // in clusters (a tile is 23 us from end to end). us, here and there, 32 / 8 heads of 128 over 48 x 4000 keys: bf16 16 rows 138, 215;
-    // 20 rows 254, 215; MXFP8 16 rows 122, 339; 32 rows 220, 340; 64 rows 415, 340. Over 1 x 1000: bf16 16 rows 8.8, 24.0; 64 rows 11.1, 24.3. Where all
+    // mma.sync) is bound by its keys' bytes, and two under MXFP8 are as fast as tiles whose codes are widened; small calls of up to four
+    // in clusters (a tile is 23 us from end to end). us, here and there, 32 / 8 heads of 128 over 48 x 4000 keys: bf16 16 rows 139, 213;
+    // 20 rows 251, 214; MXFP8 16 rows 122, 243; 32 rows 231, 244 (f16 221, 238); 48 rows 330, 244. Over 1 x 1000: bf16 16 rows 8.8, 24.0; 64 rows 11.1, 24.3. Where all
     // lengths are alike as far as the bounds tell, one kernel has all.
     const uint32_t few = rows_max <= 64 ? cluster((rows_max + PA_ROWS - 1) / PA_ROWS, 576) : 0;
     const uint32_t cap = few ? 64 : (mx ? 2 * PA_ROWS : PA_ROWS);

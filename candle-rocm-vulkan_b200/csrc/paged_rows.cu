@@ -415,18 +415,14 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const Unpac
             raw.w[0] = w.x, raw.w[1] = w.y, raw.w[2] = w.z, raw.w[3] = w.w;
             values8<PDT>(raw, x);
             store8<DT>(dst, true, x);
+        } else if (DT == B200_BF16 || (DT == B200_F16 && e - 112u <= 30u)) {
+            // a power of two that the type has: the product is exact, or rounded once
+            constexpr bool B = DT == B200_BF16;
+            uint32_t rest;
+            const uint32_t f = pool_scale2<B>(e, e, rest);
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(pool_mul2<B>(pool_pair<B, 0>(w.x), f), pool_mul2<B>(pool_pair<B, 1>(w.x), f), pool_mul2<B>(pool_pair<B, 0>(w.y), f),
+                                                         pool_mul2<B>(pool_pair<B, 1>(w.y), f));
         } else {
-            if (DT != B200_F32 && (DT == B200_BF16 ? e <= 134u : e - 112u <= 30u)) {
-                // a power of two that the type has: the product is exact, or rounded once
-                constexpr bool B = DT == B200_BF16;
-                uint32_t rest, mag[4];
-                const uint32_t f = pool_scale2<B>(e, e, rest);
-                const uint32_t x[4] = {pool_pair<B, 0>(w.x, mag[0]), pool_pair<B, 1>(w.x, mag[1]), pool_pair<B, 0>(w.y, mag[2]), pool_pair<B, 1>(w.y, mag[3])};
-                if (!B || !pool_nan(__vimax3_u16x2(__vmaxu2(mag[0], mag[1]), mag[2], mag[3]))) {
-                    *reinterpret_cast<uint4 *>(dst) = make_uint4(pool_mul2<B>(x[0], f), pool_mul2<B>(x[1], f), pool_mul2<B>(x[2], f), pool_mul2<B>(x[3], f));
-                    return;
-                }
-            }
             const f32x2 s = pair2(e8m0_to_f(e), e8m0_to_f(e));
             const uint32_t a[2] = {w.x, w.y};
             f32x2 x[4];

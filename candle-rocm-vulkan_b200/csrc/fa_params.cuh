@@ -56,13 +56,15 @@ struct FaPages {
     uint32_t g_mul, g_shr;  // n / group
     uint32_t box;           // rows of a page that are copied at a time
     uint32_t classes;       // of sequences by their keys, the longest first
+    uint32_t whole;         // the items in front that are not split along the keys
 };
 // Tensor maps of a pool's K and V: boxes of 128-byte columns (64 where a row of codes is no longer) x `rows` rows of a page, swizzled over that
 // width; what lies past the head dim or outside the pool reads as zeros. `order` as in fa_kv_maps. k == null: only whether maps can describe them.
 bool fa_pool_maps(const PoolParams &pl, int pool_dtype, bool bf16, uint32_t rows, CUtensorMap_st *k, CUtensorMap_st *v, uint32_t *order);
-// whether the tiles take the call, and in how many key splits (part_o and part_lse, [splits][token x head], for paged_split_join)
+// whether the tiles take the call, and in how many key splits (part_o and part_lse, [splits][token x head], for paged_split_join; an infinity in the first of a
+// row's part_lse: its item was not split, `whole`)
 bool fa_paged_tiles_take(const FaParams &p, FaPages &pg, int pool_dtype);
-uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sms);
+uint32_t fa_paged_tiles_splits(const FaParams &p, FaPages &pg, uint32_t sms);
 int fa_paged_tiles_launch(const FaParams &p, const FaPages &pg, int pool_dtype, cudaStream_t stream);
 
 // decode over 16-bit K / V by tensor copies (fa_decode_tma.cu): grid (1, hkv, b * n_splits)

@@ -1098,7 +1098,7 @@ __device__ __forceinline__ bool p3_clears(const FaParams &p, const P3ItemOf<KV> 
 }
 template <int KV>
 __device__ __forceinline__ bool p3_low(const P3ItemOf<KV> &it) { return KV == 1 && (it.v_lo & 15) != 0; }
-// The same for pages. `w`: sequence, kv head, row tile, key split, as the owner warp found them.
+// The same for pages. `w`: sequence, kv head, row tile, key split (-1: all keys), as the owner warp found them.
 template <int KV>
 __device__ __forceinline__ void p3_paged_item(const FaParams &p, const FaPages &pg, const int4 &w, P3ItemOf<KV> &it) {
     it.b = (uint32_t)w.x, it.hk = (uint32_t)w.y, it.split = (uint32_t)w.w;
@@ -1118,7 +1118,7 @@ __device__ __forceinline__ void p3_paged_item(const FaParams &p, const FaPages &
     it.t_hi = max(it.t_hi, it.v_lo);
     it.t_lo = it.v_lo / P3_BN * P3_BN;
     it.ntiles = it.t_hi > it.v_lo ? (it.t_hi - it.t_lo + P3_BN - 1) / P3_BN : 0;
-    if (p.n_splits > 1) {  // whole tiles
+    if (w.w >= 0 && p.n_splits > 1) {  // whole tiles
         const int per = (it.ntiles + (int)p.n_splits - 1) / (int)p.n_splits, first = min((int)it.split * per, it.ntiles);
         it.ntiles = min(per, it.ntiles - first);
         it.t_lo += first * P3_BN;
@@ -1126,11 +1126,17 @@ __device__ __forceinline__ void p3_paged_item(const FaParams &p, const FaPages &
         it.t_hi = max(min(it.t_hi, it.t_lo + it.ntiles * P3_BN), it.t_lo);
     }
 }
-// Owner warp: the sequence, kv head, row tile and key split of item n, counted over the sequences whose rows are this kernel's (a row tile's
-// heads and splits next to one another, the tiles with the most keys first), those of more than half of the bound on the keys first, then of
+// Owner warp: the sequence, kv head, row tile and key split of item n (the first pg.whole are not split), counted over the sequences whose rows are this
+// kernel's (a row tile's heads and splits next to one another, the tiles with the most keys first), those of more than half of the bound on the keys first, then of
 // more than a quarter, then the rest (pg.classes 3): an item that starts late should be short. `at`, `before`: where the last search
 // ended (32 sequences of a class); items mostly come in ascending order. False: there are no more than n.
 __device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, uint32_t n, uint32_t &at, uint32_t &before, int lane, int4 &w) {
+    int split = -1;
+    if (n >= pg.whole) {
+        const uint32_t rest = n - pg.whole;
+        n = pg.whole + rest / p.n_splits;
+        split = (int)(rest % p.n_splits);
+    }
     if (n < before) at = before = 0;
     const uint32_t runs = (p.b + 31) / 32;
     for (; at < runs * pg.classes; ++at) {
@@ -1145,7 +1151,7 @@ __device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, ui
                 if (mine != cls) tiles = 0;
             }
         }
-        const uint32_t per = p.hkv * p.n_splits;
+        const uint32_t per = p.hkv;
         uint32_t upto = tiles * per;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -1155,13 +1161,23 @@ __device__ __forceinline__ bool p3_find(const FaParams &p, const FaPages &pg, ui
         const uint32_t hit = __ballot_sync(0xffffffffu, n - before < upto);
         if (hit) {
             const int who = __ffs(hit) - 1;
-            const uint32_t rest = n - before - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, tiles, who) * per), rank = rest / per, hs = rest - rank * per;
-            w = make_int4((int)(base + who), (int)(hs / p.n_splits), (int)(__shfl_sync(0xffffffffu, tiles, who) - 1 - rank), (int)(hs % p.n_splits));
+            const uint32_t rest = n - before - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, tiles, who) * per), rank = rest / per;
+            w = make_int4((int)(base + who), (int)(rest - rank * per), (int)(__shfl_sync(0xffffffffu, tiles, who) - 1 - rank), split);
             return true;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
     return false;
+}
+// Two neighbouring lanes, each with 16-byte pieces x and y of its own row: afterwards the even lane has x of both rows, the odd one y, so that a store
+// of both fills whole sectors of 32 bytes.
+__device__ __forceinline__ void p3_pairs(uint32_t (&x)[4], uint32_t (&y)[4], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x[i] : y[i], 1);
+        if (lane & 1) x[i] = other;
+        else y[i] = other;
+    }
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t e;
@@ -1908,13 +1924,18 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
             // 64 elements of the warp's 32 rows at a time through shared memory, so that eight lanes write 128 bytes of a row
             // (a lane that writes its own row leaves every store in 32 lines)
             uint8_t *const stage = smem + C::SM_OUT + warp * 4096;
-            if (p.n_splits > 1 || p.o_f32) {
+            const bool parts = p.n_splits > 1 && (KV == 0 || cur.split != ~0u);
+            if (KV && p.n_splits > 1 && !parts) {
+                const uint32_t r = cur.row0 + g * PF_BM + w4 * 32 + lane;
+                if (r < cur.R) p.part_lse[(cur.q0 + cur.tok(r)) * p.hq + cur.head(r)] = INFINITY;  // nothing to join
+            }
+            if (parts || p.o_f32) {
                 // f32 rows, 32 elements at a time: outputs, or a key split with the logarithm of the row's sum for fa_combine_kernel
-                float *const dst = p.n_splits > 1 ? p.part_o : reinterpret_cast<float *>(p.o);
+                float *const dst = parts ? p.part_o : reinterpret_cast<float *>(p.o);
                 const uint64_t part = (uint64_t)cur.split * p.rows_total;
                 auto out_row = [&](uint32_t rr) { return (cur.q0 + cur.tok(rr)) * p.hq + cur.head(rr); };
                 const uint32_t r = cur.row0 + g * PF_BM + w4 * 32 + lane;
-                if (p.n_splits > 1 && r < cur.R) p.part_lse[part + out_row(r)] = l == 0.0f ? -INFINITY : mref * 0.6931471805599453f + logf(l);  // a NaN stays one
+                if (parts && r < cur.R) p.part_lse[part + out_row(r)] = l == 0.0f ? -INFINITY : mref * 0.6931471805599453f + logf(l);  // a NaN stays one
 #pragma unroll 1
                 for (uint32_t c0 = 0; c0 < p.d; c0 += 32) {
                     uint32_t o[32];
@@ -1926,12 +1947,18 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                         for (int i = 0; i < 32; ++i) o[i] = 0u;
                     }
                     if constexpr (KV == 2) {  // (the stage holds codes)
-                        if (r < cur.R)
 #pragma unroll
-                            for (int v4 = 0; v4 < 8; ++v4)
-                                if (c0 + 4 * v4 < p.d)
-                                    *reinterpret_cast<float4 *>(dst + (part + out_row(r)) * p.d + c0 + 4 * v4) =
-                                        make_float4(u2f(o[4 * v4]) * inv, u2f(o[4 * v4 + 1]) * inv, u2f(o[4 * v4 + 2]) * inv, u2f(o[4 * v4 + 3]) * inv);
+                        for (int i = 0; i < 32; ++i) o[i] = f2u(u2f(o[i]) * inv);
+#pragma unroll
+                        for (int v4 = 0; v4 < 8; v4 += 2) {
+                            uint32_t(&x)[4] = reinterpret_cast<uint32_t(&)[4]>(o[4 * v4]), (&y)[4] = reinterpret_cast<uint32_t(&)[4]>(o[4 * v4 + 4]);
+                            p3_pairs(x, y, lane);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t rr = r - (lane & 1) + e, at = c0 + 4 * (v4 + (lane & 1));
+                                if (rr < cur.R && at < p.d) *reinterpret_cast<uint4 *>(dst + (part + out_row(rr)) * p.d + at) = e ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(x[0], x[1], x[2], x[3]);
+                            }
+                        }
                     } else {
 #pragma unroll
                     for (int v4 = 0; v4 < 8; ++v4)
@@ -2238,18 +2265,28 @@ static uint64_t paged_items(const FaParams &p, const FaPages &pg) {
     const uint64_t tiles = ((uint64_t)p.lq * p.group + pg.tile_rows - 1) / pg.tile_rows, big = std::min<uint64_t>(p.b, pg.total_q / (pg.row_cap / p.group + 1));
     return std::max<uint64_t>(std::min<uint64_t>(big * tiles, (uint64_t)pg.total_q * p.group / pg.tile_rows + big), 1) * p.hkv;
 }
-uint32_t fa_paged_tiles_splits(const FaParams &p, const FaPages &pg, uint32_t sms) {
-    // Where the items leave SMs idle: the number of key splits with the least time, a tile at 1.6 us, 3.5 us for the grid that joins them, and the partial rows
-    // written and read (mostly in L2) at 10 TB/s. The lengths are bounds here; splits that find no keys cost a partial result of nothing. us, at least four
-    // tiles a split and this rule, 32 / 8 heads of 128: 20 tokens over 1000 keys 24.2, 14.3; 64 over 2000 25.9, 20.5; 4 x 64 over 1000 27.4, 21.7; 200
-    // over 1000 25.1, 20.6.
+uint32_t fa_paged_tiles_splits(const FaParams &p, FaPages &pg, uint32_t sms) {
+    // Whole items for a number of full waves, and the rest in n key splits: the pair with the least time. A tile takes 2.1 us, 1.6 for one group of rows; splits
+    // 3.5 us for the grid that joins them, and the partial rows written and read: 0.1 us a MB, and 0.4 more from 30 MB on. The lengths are bounds here; splits
+    // that find no keys cost a partial result of nothing. Few items, us, at least four tiles a split and this rule, 32 / 8 heads of 128: 20 tokens over 1000 keys
+    // 24.2, 14.3; 64 over 2000 25.9, 20.5; 4 x 64 over 1000 27.4, 21.7; 200 over 1000 25.1, 20.6. Items that fill a wave or two by half, unsplit and so: 700
+    // over 12000 keys 221, 184; 1300 over 4000 129, 123; MXFP8 237, 199; 139, 130. That only for one sequence: several of uneven
+    // lengths balance one another (1000 over 5000 and 600 over 3000: 148, 162).
     const uint64_t keys = p.wl >= 0 ? std::min<uint64_t>(p.lk, (uint64_t)p.wl + P3_ROWS) : p.lk, tiles = (keys + P3_BN - 1) / P3_BN;
-    const uint64_t most = std::min<uint64_t>(sms / paged_items(p, pg), 64);
+    const uint64_t items = paged_items(p, pg), waves = items / sms;
+    const double tile = (uint64_t)p.lq * p.group > PF_BM ? 2.1 : 1.6;
     uint32_t best = 1;
-    double least = 1.6 * tiles;
-    for (uint32_t n = 2; n <= most; ++n) {
-        const double t = 1.6 * ((tiles + n - 1) / n) + 3.5 + 0.05 * n + (double)p.rows_total * n * p.d * 8 / 1e7;
-        if (t < least) least = t, best = n;
+    double least = tile * tiles * ((items + sms - 1) / sms) * (waves ? 0.97 : 1.0);
+    pg.whole = 0;
+    if (waves && p.b > 1) return 1;
+    for (uint64_t k = waves ? waves - 1 : 0; k <= waves; ++k) {
+        const uint64_t rest = items - k * sms, rows = std::min<uint64_t>(p.rows_total, rest * pg.tile_rows);
+        for (uint32_t n = 2; rest && n <= 64 && (uint64_t)n * p.rows_total * p.d * 4 <= (512u << 20); ++n) {
+            const uint64_t turns = (rest * n + sms - 1) / sms;
+            if (turns > 1 && p.b > 1) break;
+            const double mb = (double)rows * n * p.d * 8e-6, t = tile * (k * tiles + turns * ((tiles + n - 1) / n)) + (turns - 1) + 3.5 + 0.05 * n + 0.1 * mb + 0.4 * std::max(0.0, mb - 30.0);
+            if (t < least) least = t, best = n, pg.whole = (uint32_t)(k * sms);
+        }
     }
     return best;
 }
@@ -2264,7 +2301,7 @@ static int fa_paged_launch_as(const FaParams &p, FaPages pg, const P3Grid &gr, c
 }
 int fa_paged_tiles_launch(const FaParams &p, const FaPages &pg, int pool_dtype, cudaStream_t stream) {
     const bool mx = pool_dtype == B200_FP8, bf16 = p.q_dtype == B200_BF16;
-    const uint64_t items = paged_items(p, pg) * p.n_splits;
+    const uint64_t items = pg.whole + (paged_items(p, pg) - pg.whole) * p.n_splits;
     CUtensorMap tm_k, tm_v, tm_q;
     P3Grid gr = {};
     if (items >= (1ull << 31) || !fa_pool_maps(pg.pool, pool_dtype, bf16, pg.box, &tm_k, &tm_v, &gr.tm_order)) return FA_NO_MAP;

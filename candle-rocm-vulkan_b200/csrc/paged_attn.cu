@@ -909,7 +909,8 @@ __global__ void __launch_bounds__(512) paged_join_kernel(const PaParams p) {
     }
 }
 
-// Key splits of the tcgen05 tiles: one warp per token and head of the sequences that are theirs, as fa_combine_kernel.
+// Key splits of the tcgen05 tiles: one warp per token and head of the sequences that are theirs, as fa_combine_kernel. Rows whose item was not split
+// say so in their first split's sum. (Four heads a warp, with fewer warps: 217 for 185 us, 700 tokens over 12000 keys.)
 template <bool BF16>
 __global__ void __launch_bounds__(128) paged_split_join(const PaParams p, const uint32_t row_cap, const float *__restrict__ part_o, const float *__restrict__ part_lse,
                                                         const uint32_t n_splits) {
@@ -922,6 +923,7 @@ __global__ void __launch_bounds__(128) paged_split_join(const PaParams p, const 
         const uint32_t seq = pool_seq(p.cu_q, p.b, tok, lane), q0 = p.cu_q[seq], lq = p.cu_q[seq + 1] - q0;
         if (tok < q0 || tok - q0 >= min(lq, p.max_q) || min(lq, p.max_q) * p.group <= row_cap) continue;
         float e0 = (uint32_t)lane < n_splits ? part_lse[(uint64_t)lane * rows + row] : -INFINITY;
+        if (__shfl_sync(0xffffffffu, e0, 0) == INFINITY) continue;  // not split
         float e1 = (uint32_t)lane + 32 < n_splits ? part_lse[(uint64_t)(lane + 32) * rows + row] : -INFINITY;
         float mx = fmaxf(e0, e1);
 #pragma unroll

@@ -509,3 +509,14 @@ def test_a_nan_among_codes_shows(P, dt, lq, far):
     assert bool(out[:, :4].isnan().all())
     assert bool(out[:, 4:, 37].isnan().all())
     assert int(out.isnan().sum()) == lq * (4 * b.d + 4)
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+@pytest.mark.parametrize("lq,lk,opt,pad", [([1300], [1500], {}, 3), ([1300], [1500], dict(wl=200), 0), ([900, 500], [1700, 600], {}, 0), ([1251], [1251], dict(wr=None), 2)])
+def test_whole_items_and_a_rest_in_key_splits(P, form, lq, lk, opt, pad):
+    """Just over a wave of row tiles: the first are taken whole, the others in splits of their keys."""
+    b = Batch(P, lq, lk, hq=32, hkv=8, d=64, form=form, pad=pad)
+    c = cfg(P, b.d, **opt)
+    out = torch.full_like(b.q, 7.0)
+    b.check(b.run(c, out=out), c)
+    assert bool((out[sum(lq):] == 7.0).all())

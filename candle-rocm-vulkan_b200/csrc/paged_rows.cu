@@ -324,10 +324,10 @@ template <int DT, int TURN, int POOL, int PDT>
 static int rows_launch(const RowsParams &p, bool vec, cudaStream_t stream, const char *what) {
     const uint32_t chunks = p.d / 8, lpr = chunks <= 8 ? 8 : (chunks <= 16 ? 16 : 32), rows = p.q.heads + p.k.heads + p.v.heads;
     RowsParams r = p;
-    // Two waves of warps and more: a warp goes over a whole token. Fewer tokens are shared among warps, down to one load a lane (8 191 tokens: 41.9 us whole,
-    // 40.0 in halves).
+    // Two waves of warps and more (four where there is no pool): a warp goes over a whole token. Fewer tokens are shared among warps, down to one load a lane
+    // (8 191 tokens into an MXFP8 pool: 40.0 us whole, 44.6 in halves; 5 003 turned alone, f32: 19.3 whole, 18.4 in thirds).
     const uint32_t most = std::max(1u, (rows * lpr + 31) / 32);
-    r.parts = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, 148ull * 32 * 2 / std::max(p.tokens, 1u)));
+    r.parts = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(1, 148ull * 32 * (POOL ? 2 : 4) / std::max(p.tokens, 1u)));
     const uint64_t blocks = ((uint64_t)p.tokens * r.parts + PR_WARPS - 1) / PR_WARPS;
     if (blocks >= (1ull << 31)) return set_error(B200_ERR_UNSUPPORTED_SHAPE, "%s: %u tokens", what, p.tokens);
     if (lpr == 8) paged_rows_kernel<DT, TURN, POOL, PDT, 8><<<(unsigned)blocks, PR_WARPS * 32, 0, stream>>>(r, vec);

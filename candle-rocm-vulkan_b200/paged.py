@@ -258,6 +258,8 @@ class PagedKvPool:
         shape = table.shape
         if len(shape) != 2 or shape[0] != b:
             raise ValueError(f"{what}: block_table must have a row for each of {b} sequences, got {tuple(shape)}")
+        if shape[1] == 0:  # nobody has a page
+            return torch.full((b, 1), -1, dtype=torch.int32, device=self.device)
         return _ints(table, torch.int32, self.device, "block_table")
 
     def keys_values(self, block_table: torch.Tensor, seqlens_k: torch.Tensor, total: int, dtype: Optional[torch.dtype] = None,

@@ -520,3 +520,37 @@ def test_whole_items_and_a_rest_in_key_splits(P, form, lq, lk, opt, pad):
     out = torch.full_like(b.q, 7.0)
     b.check(b.run(c, out=out), c)
     assert bool((out[sum(lq):] == 7.0).all())
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+@pytest.mark.parametrize("hq,hkv", [(71, 1), (128, 1), (256, 1), (300, 1), (600, 3)])
+def test_groups_of_many_heads(P, hq, hkv, form):
+    b = Batch(P, [1, 3, 20], [100, 600, 333], hq=hq, hkv=hkv, d=64, form=form)
+    c = cfg(P, b.d)
+    b.check(b.run(c), c)
+
+
+def test_a_table_without_columns(P):
+    b = Batch(P, [2, 3], [0, 0])
+    b.table = b.table[:, :0]
+    out = b.run(cfg(P, b.d))
+    assert bool((out == 0).all())
+    k, v = b.pool.keys_values(b.table, torch.zeros(3, dtype=torch.int32, device="cuda"), 0)
+    assert k.shape == v.shape == (0, 2, 128)
+
+
+def test_calls_on_two_streams_at_once(P):
+    """Steps, chunks and both, each with scratch, side by side on two streams: the results of calls alone."""
+    batches = [Batch(P, [1] * 30, [300 + 100 * i for i in range(30)], form="mxfp8", seed=1), Batch(P, [500], [3000], seed=2), Batch(P, [1, 300, 2, 40], [2000, 900, 50, 1500], seed=3)]
+    c = cfg(P, 128)
+    want = [b.run(c) for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(10):
+        for i, b in enumerate(batches):
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append((i, b.run(c)))
+    torch.cuda.synchronize()
+    assert all(bool((o == want[i]).all()) for i, o in got)

@@ -316,16 +316,15 @@ class PagedKvPool:
                   b, total, int(max_seqlen_q), int(max_seqlen_k), hq, table.shape[1], _float_id(q), cfg.softmax_scale, softcap, wl, wr, ap, abs_, 0)
         st = _word(status, dev)
         lib = _lib()
-        if not _capturing():
+        if dev.index == _current_device() and not _capturing():
             # the stream's scratch as it is; the library says where it is too small
-            ws = _workspace(dev, 1 << 20)
-            args = self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr(), ws.numel(), st)
-            if dev.index == _current_device():
-                rc = lib.b200_paged_attention(args, _stream(dev))
-                if rc == A.OK:
-                    return out
-                if rc != A.ERR_WORKSPACE:
-                    A.check(rc)
+            stream = _stream(dev)
+            ws = _workspace(dev, 1 << 20, stream)
+            rc = lib.b200_paged_attention(self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr(), ws.numel(), st), stream)
+            if rc == A.OK:
+                return out
+            if rc != A.ERR_WORKSPACE:
+                A.check(rc)
         nbytes = lib.b200_paged_attention_workspace_bytes(self._packed + _ATTN_ARGS.pack(*fields, 0, 0, st))
         ws = _call_workspace(dev, nbytes) if nbytes else None
         _call(lib.b200_paged_attention, self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr() if ws is not None else 0, nbytes, st), dev)

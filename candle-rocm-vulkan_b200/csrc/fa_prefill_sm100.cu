@@ -2276,7 +2276,7 @@ uint32_t fa_paged_tiles_splits(const FaParams &p, FaPages &pg, uint32_t sms) {
     const uint64_t items = paged_items(p, pg), waves = items / sms;
     const double tile = (uint64_t)p.lq * p.group > PF_BM ? 2.1 : 1.6;
     uint32_t best = 1;
-    double least = tile * tiles * ((items + sms - 1) / sms) * (waves ? 0.97 : 1.0);
+    double least = tile * tiles * ((items + sms - 1) / sms) * (waves ? 0.95 : 1.0);  // (full waves: not for less than a twentieth)
     pg.whole = 0;
     if (waves && p.b > 1) return 1;
     for (uint64_t k = waves ? waves - 1 : 0; k <= waves; ++k) {

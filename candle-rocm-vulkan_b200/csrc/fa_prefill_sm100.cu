@@ -1567,7 +1567,8 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                 // Row `key` of a raw tile, or zeros, into the layout of the tensor copies. One warp per SM quadrant widens all of a tile's keys while
                 // two others compute exponentials, so its instructions count, and more than they the places that they take in the instruction cache:
                 // short loops over four chunks of codes, one body for K and V, are faster than straight code (2048 tokens over 16384 keys, 32 / 8 heads
-                // of 128: f16 907 -> 942 TFLOP/s, bf16 740 -> 886). One multiplier per 32 elements; f16 rows with a scale below 2^-24 apart.
+                // of 128: f16 907 -> 942 TFLOP/s, bf16 740 -> 886). One multiplier per 32 elements; f16 rows with a scale that f16 does not have (below 2^-24,
+                // above 2^15) apart.
                 auto widen = [&](uint32_t raw, uint32_t dst, uint32_t sc, bool zero) {
                     constexpr int CH = HD / 16;  // raw chunks of 16 codes
                     const uint32_t row = raw + key * HD, out = dst + key * 128, sw = HD == 64 ? (key >> 1) & 3 : key & 7;
@@ -1618,7 +1619,7 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                             }
                         }
                     };
-                    if (!BF16 && __vcmpltu4(sc, 0x67676767u)) far();
+                    if (!BF16 && (__vcmpltu4(sc, 0x67676767u) | __vcmpgtu4(sc, 0x8e8e8e8eu))) far();
                     else chunks();
                 };
                 for (int k = 0, n; next_item(k, n); ++k) {

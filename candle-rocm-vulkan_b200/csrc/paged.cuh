@@ -49,15 +49,16 @@ template <bool BF16, int I>
 __device__ __forceinline__ uint32_t pool_pair(uint32_t w) {
     return pool_f16_as<BF16>(I ? cvt_e4m3x2_hi_f16x2(w) : cvt_e4m3x2_f16x2(w));
 }
-// The multiplier 2^(e - 127) of such a pair, for the scales e0 and e1. bf16 has all of them; f16's below e = 103 go in two steps: `rest` is the second.
+// The multiplier 2^(e - 127) of such a pair, for the scales e0 and e1. bf16 has all of them; f16's outside 103 .. 142 go in two steps: `rest` is the second. A
+// large one ends at 2^15, which with the first 2^15 takes the smallest code, 2^-9, past f16's largest number; neither is infinite, so a code of zero stays zero.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pool_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
     if (BF16) {
         rest = 0x3f803f80u;
         return (e0 ? e0 << 7 : 0x40u) | (e1 ? e1 << 7 : 0x40u) << 16;
     }
-    const uint32_t m0 = max(e0, 103u), m1 = max(e1, 103u);
-    rest = pack_f16x2(e8m0_to_f(e0 + 127u - m0), e8m0_to_f(e1 + 127u - m1));
+    const uint32_t m0 = min(max(e0, 103u), 142u), m1 = min(max(e1, 103u), 142u);
+    rest = pack_f16x2(e8m0_to_f(min(e0 + 127u - m0, 142u)), e8m0_to_f(min(e1 + 127u - m1, 142u)));
     return pack_f16x2(e8m0_to_f(m0), e8m0_to_f(m1));
 }
 

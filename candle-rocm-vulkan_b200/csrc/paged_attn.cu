@@ -693,9 +693,11 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
             }
         } else {
             // Column n = g of the products' tile i is element g HD / 8 + i: a lane reads the same bytes of its four keys. Values and weights in f16, also
-            // under bf16 queries (the codes times 2^k with k from -22 to 7 are within 2^-11 of a block's largest there, and weights have three bits
-            // more); tiles with scales outside that take the second form: two factors, or bf16 under bf16 queries.
+            // under bf16 queries, where f16 holds every code times the scale exactly: 2^-9 2^-15 is its smallest number, 448 2^7 is below its largest, so scale
+            // bytes from 112 to 134 (weights have three bits more there). f16 queries round values to f16 in any case and go down to byte 105, whose power
+            // of two f16 still has. Tiles with scales outside that take the second form: two factors, or bf16 under bf16 queries.
             constexpr int W = HD / 32;  // words of a lane's elements
+            constexpr uint32_t E_LO = BF16 ? 112 : 105, E_HI = 134;
             const uint32_t vsc = tsc + KEYS * C::NB + g * (HD / 8) / 32;
             uint32_t e[KG][4], off = 0;
 #pragma unroll
@@ -703,7 +705,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     e[kk][k] = pa_lds8(vsc + (kk * 16 + 2 * c + (k & 1) + (k >> 1) * 8) * C::NB);
-                    off = __viaddmax_u32(e[kk][k], 0u - 105u, off);
+                    off = __viaddmax_u32(e[kk][k], 0u - E_LO, off);
                 }
             auto products = [&](auto bf, auto far) {
                 constexpr bool B = bf.value, FAR = far.value;
@@ -741,7 +743,7 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                     }
                 }
             };
-            if (__any_sync(0xffffffffu, off > 29u)) products(std::bool_constant<BF16>{}, std::true_type{});
+            if (__any_sync(0xffffffffu, off > E_HI - E_LO)) products(std::bool_constant<BF16>{}, std::true_type{});
             else products(std::false_type{}, std::false_type{});
         }
         __syncwarp();  // the stage has been read

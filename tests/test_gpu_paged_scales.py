@@ -77,3 +77,18 @@ def test_f16_over_scales_past_its_range(P, lq, d, e):
         assert bool((out[:, 4:, 37] == math.inf).all()) and bool((out[:, 4:, 41] == -math.inf).all())
         out[:, 4:, 37], out[:, 4:, 41] = got[:, 4:, 37], got[:, 4:, 41]
         assert torch.equal(out, got)
+
+
+@pytest.mark.parametrize("lq", [1, 5, 60])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lo,hi", [(100, 112), (105, 106), (108, 109), (111, 112), (112, 135), (133, 137)])
+def test_bf16_holds_every_code(P, lq, d, lo, hi):
+    """Values beside one that is a thousand times larger, behind small and large powers of two: under bf16 queries none of them loses a digit."""
+    b = Apart(P, [lq, lq], [100, 333], form="mxfp8", d=d, seed=lo)
+    v = b.pool.v.view(torch.uint8)
+    codes = torch.randint(0, 0x28, v.shape, generator=b.g, device="cuda")  # up to 2^-2, most below the normal ones
+    codes[..., 3::32] = torch.randint(0x70, 0x7f, codes[..., 3::32].shape, generator=b.g, device="cuda")
+    v.copy_(codes | torch.randint(0, 2, v.shape, generator=b.g, device="cuda") << 7)
+    b.pool.v_scale.copy_(torch.randint(lo, hi, b.pool.v_scale.shape, generator=b.g, device="cuda"))
+    c = cfg(P, d)
+    b.check(b.run(c), c)

@@ -1591,7 +1591,7 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                             for (int x = 0; x < 2; ++x) {
                                 uint32_t o[4] = {pool_pair<BF16, 0>(a[2 * x]), pool_pair<BF16, 1>(a[2 * x]), pool_pair<BF16, 0>(a[2 * x + 1]), pool_pair<BF16, 1>(a[2 * x + 1])};
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) o[k] = pool_mul2<BF16>(pool_mul2<BF16>(o[k], f), rest);
+                                for (int k = 0; k < 4; ++k) o[k] = pool_mul2<BF16>(pool_mul2<BF16>(o[k], rest), f);
                                 put(2 * q + x, o);
                             }
                         }

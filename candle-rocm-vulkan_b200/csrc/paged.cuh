@@ -49,8 +49,9 @@ template <bool BF16, int I>
 __device__ __forceinline__ uint32_t pool_pair(uint32_t w) {
     return pool_f16_as<BF16>(I ? cvt_e4m3x2_hi_f16x2(w) : cvt_e4m3x2_f16x2(w));
 }
-// The multiplier 2^(e - 127) of such a pair, for the scales e0 and e1. bf16 has all of them; f16's outside 103 .. 142 go in two steps: `rest` is the second. A
-// large one ends at 2^15, which with the first 2^15 takes the smallest code, 2^-9, past f16's largest number; neither is infinite, so a code of zero stays zero.
+// The multiplier 2^(e - 127) of such a pair, for the scales e0 and e1. bf16 has all of them; f16's outside 103 .. 142 go in two steps, `rest` first: a small
+// one is exact there (or the value less than half of f16's smallest number in any case), so that the second step rounds once, as a conversion would. A large
+// one ends at 2^15, which with the second's 2^15 takes the smallest code, 2^-9, past f16's largest number; neither is infinite, so a code of zero stays zero.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pool_scale2(uint32_t e0, uint32_t e1, uint32_t &rest) {
     if (BF16) {

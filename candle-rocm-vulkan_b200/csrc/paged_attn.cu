@@ -733,8 +733,8 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                                 pool_codes4<B>(w[2 * k][x], w[2 * k + 1][x], b[k]);
 #pragma unroll
                                 for (int y = 0; y < 4; ++y) {
-                                    b[k][y] = pool_mul2<B>(b[k][y], f[k]);
                                     if (FAR && !B) b[k][y] = pool_mul2<B>(b[k][y], rest[k]);
+                                    b[k][y] = pool_mul2<B>(b[k][y], f[k]);
                                 }
                             }
 #pragma unroll

@@ -92,3 +92,21 @@ def test_bf16_holds_every_code(P, lq, d, lo, hi):
     b.pool.v_scale.copy_(torch.randint(lo, hi, b.pool.v_scale.shape, generator=b.g, device="cuda"))
     c = cfg(P, d)
     b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("e", [100, 105, 108, 111, 112, 134])
+@pytest.mark.parametrize("form", ["bf16", "f16"])
+def test_a_step_a_chunk_and_the_rows_have_the_same_values(P, form, e):
+    """One key alone is its value: by the kernel of steps, by the tiles, and read back."""
+    b = Apart(P, [1, 1], [1, 1], dt=form, form="mxfp8", seed=e)
+    b.pool.v_scale.fill_(e)
+    v = b.pool.v.view(torch.uint8)
+    v.copy_(torch.arange(v.numel(), device="cuda").view(v.shape) % 127)
+    c = cfg(P, 128)
+    step = b.run(c).clone()
+    _, rows = b.pool.keys_values(b.table, torch.tensor([0, 1, 2], device="cuda"), 2, dtype=b.q.dtype)
+    assert torch.equal(step, rows.repeat_interleave(4, 1))
+    q = torch.randn((40, 8, 128), generator=b.g, device="cuda").to(b.q.dtype)
+    one = torch.tensor([1], device="cuda").int()
+    chunk = b.pool.attention(q, torch.tensor([0, 40], device="cuda").int(), b.table[:1], one, 40, 1, cfg(P, 128, wr=None))
+    assert torch.equal(chunk, rows[:1].repeat_interleave(4, 1).expand(40, 8, 128))

@@ -603,9 +603,9 @@ __global__ void __launch_bounds__(PA_THREADS, HD == 256 ? 1 : 2) paged_decode_ke
                     float z[4];
                     mma_f16_16816_z(z, q0[0], q0[1], q0[2], q0[3], cvt_e4m3x2_f16x2(w.x), cvt_e4m3x2_hi_f16x2(w.x));
                     mma_f16_16816(z, q1[0], q1[1], q1[2], q1[3], cvt_e4m3x2_f16x2(w.y), cvt_e4m3x2_hi_f16x2(w.y));
-                    // (the smallest scale, 2^-127, counts as nothing here)
-                    const float s0 = u2f(C::NB == 4 ? (i < 3 ? sw[n].x << (23 - 8 * (i & 3)) : sw[n].x >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i) << 23);
-                    const float s1 = u2f(C::NB == 4 ? (i < 3 ? sw[n].y << (23 - 8 * (i & 3)) : sw[n].y >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i) << 23);
+                    // (the smallest scale, 2^-127, is half of the smallest normal number)
+                    const float s0 = u2f(max(C::NB == 4 ? (i < 3 ? sw[n].x << (23 - 8 * (i & 3)) : sw[n].x >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c) * C::NB + i) << 23, 0x00400000u));
+                    const float s1 = u2f(max(C::NB == 4 ? (i < 3 ? sw[n].y << (23 - 8 * (i & 3)) : sw[n].y >> 1) & 0x7f800000u : pa_lds8(tsc + (8 * n + 2 * c + 1) * C::NB + i) << 23, 0x00400000u));
                     s[n][0] = fmaf(z[0], s0, s[n][0]);
                     s[n][1] = fmaf(z[1], s1, s[n][1]);
                     s[n][2] = fmaf(z[2], s0, s[n][2]);

@@ -110,3 +110,16 @@ def test_a_step_a_chunk_and_the_rows_have_the_same_values(P, form, e):
     one = torch.tensor([1], device="cuda").int()
     chunk = b.pool.attention(q, torch.tensor([0, 40], device="cuda").int(), b.table[:1], one, 40, 1, cfg(P, 128, wr=None))
     assert torch.equal(chunk, rows[:1].repeat_interleave(4, 1).expand(40, 8, 128))
+
+
+@pytest.mark.parametrize("lq", [1, 5, 60])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_keys_behind_the_smallest_scale_count(P, lq, d):
+    """2^-127, scale byte 0, under queries that are as large as the keys are small."""
+    b = Apart(P, [lq, lq], [100, 333], form="mxfp8", d=d, seed=d)
+    k = b.pool.k.view(torch.uint8)
+    k.copy_(torch.randint(0x40, 0x7f, k.shape, generator=b.g, device="cuda") | torch.randint(0, 2, k.shape, generator=b.g, device="cuda") << 7)  # 2 to 448
+    b.pool.k_scale.zero_()
+    b.q = (b.q.float() * 2.0 ** 100).bfloat16()
+    c = P.FlashAttnConfig(2.0 ** 16).causal()
+    b.check(b.run(c), c)

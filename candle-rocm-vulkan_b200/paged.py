@@ -8,12 +8,13 @@ where the pool holds MXFP8) and `attention` (every sequence's new tokens over it
 """
 import ctypes as C
 import struct
+import threading
 from typing import Optional, Sequence
 
 import torch
 
 from . import _abi as A
-from .turbo_quant import FlashAttnConfig, _DTYPES, _call_workspace, _capturing, _dtype_id, _need_cuda, _stream, _workspace
+from .turbo_quant import FlashAttnConfig, _DTYPES, _capturing, _dtype_id, _need_cuda, _stream, _workspace
 
 _E4M3 = getattr(torch, "float8_e4m3fn", None)
 _POOL_DTYPES = {torch.float16: A.F16, torch.bfloat16: A.BF16, _E4M3: A.FP8}
@@ -42,6 +43,15 @@ def _call(fn, args: bytes, device):
             rc = fn(args, _stream(device))
     if rc:
         A.check(rc)
+
+
+_this_thread = threading.get_ident
+
+
+def _scratch(device, nbytes: int, stream: int) -> torch.Tensor:
+    """`_workspace` of this thread on this stream. An attention call is up to three launches that hand partial results on, and threads that share a
+    stream may come in between one another's: each has scratch of its own."""
+    return _workspace(device, nbytes, (stream, _this_thread()))
 
 
 def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:
@@ -317,15 +327,17 @@ class PagedKvPool:
         st = _word(status, dev)
         lib = _lib()
         if dev.index == _current_device() and not _capturing():
-            # the stream's scratch as it is; the library says where it is too small
+            # the scratch as it is; the library says where it is too small
             stream = _stream(dev)
-            ws = _workspace(dev, 1 << 20, stream)
+            ws = _scratch(dev, 1 << 20, stream)
             rc = lib.b200_paged_attention(self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr(), ws.numel(), st), stream)
             if rc == A.OK:
                 return out
             if rc != A.ERR_WORKSPACE:
                 A.check(rc)
         nbytes = lib.b200_paged_attention_workspace_bytes(self._packed + _ATTN_ARGS.pack(*fields, 0, 0, st))
-        ws = _call_workspace(dev, nbytes) if nbytes else None
+        ws = None
+        if nbytes:  # a call that is being captured has scratch of its own, in its graph's memory pool
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if _capturing() else _scratch(dev, nbytes, _stream(dev))
         _call(lib.b200_paged_attention, self._packed + _ATTN_ARGS.pack(*fields, ws.data_ptr() if ws is not None else 0, nbytes, st), dev)
         return out

@@ -565,6 +565,8 @@ int b200_paged_unpack(const B200PagedUnpackArgs *args, b200_stream_t stream);
  * ones are cut) and size the launches; total_q bounds cu_q[b], and rows of `out` behind cu_q[b] are left as they were. q and out of q_dtype
  * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows; out does not overlap q. An MXFP8
  * pool's values count as q_dtype holds them (f16: an infinity above 65504).
+ * A call is up to three launches that hand partial results on in the workspace: calls that may come in between one another, on
+ * different streams or from threads that share one, need different workspaces.
  * The reference gathers the pages on the host (candle-flash-attn/src/lib.rs:341-420). */
 typedef struct B200PagedAttnArgs {
     B200PagedPool pool;

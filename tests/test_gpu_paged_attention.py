@@ -554,3 +554,26 @@ def test_calls_on_two_streams_at_once(P):
                     got.append((i, b.run(c)))
     torch.cuda.synchronize()
     assert all(bool((o == want[i]).all()) for i, o in got)
+
+
+def test_two_threads_on_one_stream(P):
+    """Calls of two threads whose launches alternate on the default stream: steps in many shares, chunks in key splits, both."""
+    import threading
+    batches = [Batch(P, [1] * 30, [300 + 100 * i for i in range(30)], form="mxfp8", seed=1), Batch(P, [64], [3000], seed=2), Batch(P, [1, 300, 2, 40], [2000, 900, 50, 1500], seed=3)]
+    c = cfg(P, 128)
+    want = [b.run(c) for b in batches]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(2)
+
+    def work(turn):
+        start.wait(60)
+        got = [((i + turn) % 3, batches[(i + turn) % 3].run(c)) for i in range(150)]
+        torch.cuda.synchronize()
+        wrong.extend(i for i, o in got if not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

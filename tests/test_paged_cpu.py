@@ -205,3 +205,26 @@ def test_status_words(P):
     for bad, dev in ((ok.long(), cpu), (ok, torch.device("cuda:0")), (ok[:0], cpu)):
         with pytest.raises(ValueError, match="status"):
             paged._word(bad, dev)
+
+
+def test_threads_that_share_a_stream_have_scratch_of_their_own(P):
+    """Launches of two threads on one stream may alternate: neither's partial results lie where the other's are, or the other calls'."""
+    import threading
+    from candle_rocm_vulkan_b200 import paged
+    from candle_rocm_vulkan_b200.turbo_quant import _workspace
+    cpu = torch.device("cpu")
+    got, meet = [_workspace(cpu, 100, 7)], threading.Barrier(3)
+
+    def work():
+        mine = paged._scratch(cpu, 1 << 20, 7)
+        meet.wait(60)  # both live
+        got.extend([mine, paged._scratch(cpu, 100, 7), paged._scratch(cpu, 100, 8)])
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    meet.wait(60)
+    for t in threads:
+        t.join()
+    places = [x.data_ptr() for x in got]
+    assert len(places) == 7 and len(set(places)) == 5  # one thread's calls on one stream share theirs

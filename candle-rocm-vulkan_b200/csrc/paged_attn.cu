@@ -922,7 +922,7 @@ __global__ void __launch_bounds__(128) paged_split_join(const PaParams p, const 
     for (uint64_t row = (uint64_t)blockIdx.x * 4 + warp; row < rows; row += (uint64_t)gridDim.x * 4) {
         const uint32_t tok = (uint32_t)(row / p.hq), h = (uint32_t)(row - (uint64_t)tok * p.hq);
         if (tok >= p.cu_q[p.b]) return;
-        const uint32_t seq = pool_seq(p.cu_q, p.b, tok, lane), q0 = p.cu_q[seq], lq = p.cu_q[seq + 1] - q0;
+        const uint32_t seq = pool_seq(p.cu_q, p.b, tok, lane), q0 = p.cu_q[seq], lq = min(p.cu_q[seq + 1], p.total_q) - q0;  // (cut as in pa_seq)
         if (tok < q0 || tok - q0 >= min(lq, p.max_q) || min(lq, p.max_q) * p.group <= row_cap) continue;
         float e0 = (uint32_t)lane < n_splits ? part_lse[(uint64_t)lane * rows + row] : -INFINITY;
         if (__shfl_sync(0xffffffffu, e0, 0) == INFINITY) continue;  // not split

@@ -577,3 +577,14 @@ def test_two_threads_on_one_stream(P):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+def test_cumulative_lengths_that_pass_the_queries(P, form):
+    """A last sequence that the rows of q cut down to a few tokens, behind chunks whose keys are split."""
+    b = Batch(P, [64, 20], [2000, 1500], form=form, seed=9)
+    c = cfg(P, 128)
+    b.run(c)
+    b.q, b.lq = b.q[:66].contiguous(), [64, 2]
+    out = b.pool.attention(b.q, b.cu, b.table, b.kv_len, 64, 2000, c)
+    b.check(out, c)

@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(PR_WARPS * 32) paged_unpack_kernel(const Unpac
     const uint64_t unit = (uint64_t)blockIdx.x * PR_WARPS + warp, t = unit / p.parts;
     const uint32_t part = (uint32_t)(unit % p.parts);
     const PoolParams &pl = p.pool;
-    if (t >= p.total || t >= p.cu[p.b]) return;
+    if (t >= p.total || t >= p.cu[p.b] || t < p.cu[0]) return;
     const uint32_t seq = pool_seq(p.cu, p.b, t, lane), j = (uint32_t)(t - p.cu[seq]);
     const uint32_t page = pool_div(j, pl.div_mul, pl.div_shr), row = j - page * pl.block_rows;
     const int id = page < p.table_cols ? p.table[seq * p.table_stride + page] : -1;

@@ -276,7 +276,7 @@ class PagedKvPool:
                     status: Optional[torch.Tensor] = None):
         """The rows of sequences, packed one behind the other: contiguous (total, kv_heads, head_dim) keys and values in `dtype` (the
         pool's own, bf16 for MXFP8). `seqlens_k`: cumulative lengths (sequences + 1, on the device, as for the varlen calls); `total`:
-        their last (rows behind it are left as allocated). Page numbers outside the pool read as zeros and set `status` to 3."""
+        their last (rows behind it, and in front of the first, are left as allocated). Page numbers outside the pool read as zeros and set `status` to 3."""
         b = seqlens_k.numel() - 1
         dev = self.device
         table = self._table(block_table, b, "paged keys_values")

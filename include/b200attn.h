@@ -541,8 +541,8 @@ typedef struct B200PagedAppendArgs {
 int b200_paged_append(const B200PagedAppendArgs *args, b200_stream_t stream);
 
 /* The way back: the keys and values of b sequences, packed one behind the other, as contiguous (total, hkv, d) tensors of `dtype`
- * (f32, f16 or bf16; each value rounded once). Sequence i has the rows cu_k[i] .. cu_k[i + 1] - 1; rows of the outputs behind
- * cu_k[b] are left as they were. v = NULL: only keys. Keys beyond table_cols pages read as zeros (status 3). */
+ * (f32, f16 or bf16; each value rounded once). Sequence i has the rows cu_k[i] .. cu_k[i + 1] - 1; rows of the outputs in front of
+ * cu_k[0] and behind cu_k[b] are left as they were. v = NULL: only keys. Keys beyond table_cols pages read as zeros (status 3). */
 typedef struct B200PagedUnpackArgs {
     B200PagedPool pool;
     const int32_t *table; /* device, (b, table_cols) with row stride table_stride */
@@ -562,7 +562,7 @@ int b200_paged_unpack(const B200PagedUnpackArgs *args, b200_stream_t stream);
  * Masks are aligned to the bottom right (token t of lq sits at position kv_len - lq + t) as for b200_tq_attention, and rows
  * without a visible key give zeros; scores scale * q . k, then softcap (> 0) and ALiBi. All lengths are read on the
  * device: nothing synchronises, and a captured call follows them. max_q, max_k and the table's columns bound the lengths (longer
- * ones are cut) and size the launches; total_q bounds cu_q[b], and rows of `out` behind cu_q[b] are left as they were. q and out of q_dtype
+ * ones are cut) and size the launches; total_q bounds cu_q[b], and rows of `out` in front of cu_q[0] and behind cu_q[b] are left as they were. q and out of q_dtype
  * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows; out does not overlap q. An MXFP8
  * pool's values count as q_dtype holds them (f16: an infinity above 65504).
  * A call is up to three launches that hand partial results on in the workspace: calls that may come in between one another, on

@@ -588,3 +588,15 @@ def test_cumulative_lengths_that_pass_the_queries(P, form):
     b.q, b.lq = b.q[:66].contiguous(), [64, 2]
     out = b.pool.attention(b.q, b.cu, b.table, b.kv_len, 64, 2000, c)
     b.check(out, c)
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_rows_in_front_of_the_first_sequence(P, lq):
+    """Some sequences of a longer list of cumulative lengths: the rows of the others stay as they were."""
+    b = Batch(P, [lq, lq], [300, 900], seed=17)
+    c = cfg(P, 128)
+    want = b.run(c).clone()
+    q, out = (torch.full((2 * lq + 8, b.hq, 128), 3.0, device="cuda", dtype=b.q.dtype) for _ in range(2))
+    q[5:5 + 2 * lq] = b.q
+    b.pool.attention(q, b.cu + 5, b.table, b.kv_len, lq, 900, c, out=out)
+    assert torch.equal(out[5:5 + 2 * lq], want) and bool((out[:5] == 3).all()) and bool((out[5 + 2 * lq:] == 3).all())

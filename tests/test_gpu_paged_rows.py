@@ -321,3 +321,24 @@ def test_every_code_reads_as_its_value(P, dt, e):
         want = (plane.float().double() * 2.0 ** (e - 127)).to(DT[dt]).flatten(0, 1)
         assert bool(((x == want) | (x.isnan() & want.isnan())).all())
         assert int(x.isnan().sum()) == 4
+
+
+@pytest.mark.parametrize("form", ["bf16", "mxfp8"])
+def test_rows_in_front_of_the_first_sequence_are_left(P, form):
+    """Cumulative lengths of some sequences out of a longer list: rows of the others, in front and behind, are nobody's."""
+    import ctypes as C
+    A = P._abi
+    pool = P.PagedKvPool(6, 16, 2, 64, form)
+    x = torch.randn((96, 2, 64), generator=gen(3), device="cuda").bfloat16()
+    pool.append(x, x, torch.arange(96, device="cuda"))
+    table = torch.tensor([[4, 1], [3, 0]], device="cuda").int()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 40, 60, 77, 90], device="cuda").int()
+    k, v = (torch.full((90, 2, 64), 7.0, device="cuda") for _ in range(2))
+    u = A.PagedUnpackArgs.from_buffer_copy(pool._packed + P.paged._UNPACK_ARGS.pack(
+        table.data_ptr(), 2, cu[1:].data_ptr(), k.data_ptr(), v.data_ptr(), 90, 2, 2, A.F32, 0, status.data_ptr()))
+    A.check(A.lib().b200_paged_unpack(C.byref(u), torch.cuda.current_stream().cuda_stream))
+    want, _ = pool.keys_values(table, torch.tensor([0, 20, 37], device="cuda").int(), 37, dtype=torch.float32)
+    for t in (k, v):
+        assert bool((t[:40] == 7).all()) and bool((t[77:] == 7).all()) and torch.equal(t[40:77], want)
+    assert int(status) == 0

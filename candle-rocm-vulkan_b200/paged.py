@@ -55,10 +55,14 @@ def _scratch(device, nbytes: int, stream: int) -> torch.Tensor:
 
 
 def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:
-    """Lengths, slots, positions and tables as the kernels read them: `dtype`, on the device, contiguous along the last axis."""
+    """Lengths, slots, positions and tables as the kernels read them: `dtype`, on the device, contiguous along the last axis. Wider numbers that
+    `dtype` does not hold become its nearest ones, so that what was out of range stays so."""
     if t.dtype != dtype or t.device != device:
         if t.dtype.is_floating_point or t.dtype == torch.bool:
             raise ValueError(f"{what} must be whole numbers, got {t.dtype}")
+        if t.element_size() > dtype.itemsize or t.dtype == torch.uint32:
+            top = torch.iinfo(dtype).max
+            t = t.to(torch.int64).clamp(-top - 1, top)
         t = t.to(device=device, dtype=dtype)
     return t if t.stride()[-1] == 1 or t.numel() <= 1 else t.contiguous()
 

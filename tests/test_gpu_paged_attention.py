@@ -600,3 +600,28 @@ def test_rows_in_front_of_the_first_sequence(P, lq):
     q[5:5 + 2 * lq] = b.q
     b.pool.attention(q, b.cu + 5, b.table, b.kv_len, lq, 900, c, out=out)
     assert torch.equal(out[5:5 + 2 * lq], want) and bool((out[:5] == 3).all()) and bool((out[5 + 2 * lq:] == 3).all())
+
+
+def test_wide_page_numbers_and_lengths_stay_out_of_range(P):
+    """64-bit tables and lengths whose low 32 bits would be a page of the pool, or a negative length."""
+    b = Batch(P, [1, 40], [100, 90], seed=5, page=16)
+    c = cfg(P, 128)
+    want = b.run(c).clone()
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    far = torch.tensor([2 ** 31, 2 ** 40], device="cuda")
+    assert torch.equal(b.pool.attention(b.q, b.cu, b.table, far, 40, 100, c, status=status)[:1], want[:1]) and int(status) == 3  # (the second has no such pages)
+    for bad in (2 ** 32, -2 ** 32):
+        table = b.table.long()
+        keep = b.table[1, 2].clone()
+        table[1, 2] += bad
+        status.zero_()
+        got = b.pool.attention(b.q, b.cu, table, b.kv_len, 40, 100, c, status=status).clone()
+        assert int(status) == 3
+        k, _ = b.pool.keys_values(table, torch.tensor([0, 100, 190], device="cuda"), 190)
+        assert bool((k[132:148] == 0).all())
+        hold = [(t, t[keep.long()].clone()) for t in (b.pool.k, b.pool.v)]
+        for t, _ in hold:
+            t[keep.long()] = 0
+        b.check(got, c)
+        for t, x in hold:
+            t[keep.long()] = x

@@ -228,3 +228,15 @@ def test_threads_that_share_a_stream_have_scratch_of_their_own(P):
         t.join()
     places = [x.data_ptr() for x in got]
     assert len(places) == 7 and len(set(places)) == 5  # one thread's calls on one stream share theirs
+
+
+def test_wide_integers_are_not_wrapped(P):
+    """A page number or a length that 32 bits do not hold stays out of range."""
+    from candle_rocm_vulkan_b200 import paged
+    cpu = torch.device("cpu")
+    wide = torch.tensor([2 ** 32 + 5, 2 ** 31, -2 ** 32 + 5, 2 ** 31 - 1, -2 ** 31, 7, -1])
+    got = paged._ints(wide, torch.int32, cpu, "x")
+    assert got.dtype == torch.int32 and got.tolist() == [2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, -2 ** 31, 7, -1]
+    assert paged._ints(torch.tensor([2 ** 31 + 5, 3]).to(torch.uint32), torch.int32, cpu, "x").tolist() == [2 ** 31 - 1, 3]
+    assert paged._ints(torch.tensor([3, 250]).to(torch.uint8), torch.int32, cpu, "x").tolist() == [3, 250]
+    assert paged._ints(wide, torch.int64, cpu, "x") is wide

@@ -67,6 +67,11 @@ def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:
     return t if t.stride()[-1] == 1 or t.numel() <= 1 else t.contiguous()
 
 
+def _lengths(t: torch.Tensor, device, what: str) -> torch.Tensor:
+    """A vector of lengths, or of cumulative ones, out of a tensor of any shape (a column of a matrix, one number), in its order."""
+    return _ints(t if len(t.shape) == 1 else t.reshape(-1), torch.int32, device, what)
+
+
 def _word(status: Optional[torch.Tensor], device) -> int:
     if status is None:
         return 0
@@ -241,9 +246,9 @@ class PagedKvPool:
         v, vsh, vs = _heads(v, "paged append: v", tokens, d)
         if h != self.kv_heads or vsh[1] != h or k.dtype != v.dtype or k.device != dev or v.device != dev:
             raise ValueError(f"paged append: k {tuple(k.shape)} {k.dtype} / v {tuple(v.shape)} {v.dtype} do not match {self.kv_heads} kv heads on {dev}")
-        slots = _ints(slots, torch.int64, dev, "paged append: slots")
         if slots.shape != (tokens,):
             raise ValueError(f"paged append: {tokens} tokens need as many slots, got {tuple(slots.shape)}")
+        slots = _ints(slots, torch.int64, dev, "paged append: slots")
         qo, qp, qop, qs, qos, hq = None, 0, 0, (0, 0), (0, 0), 0
         if rotary is not None:
             if positions is None:
@@ -284,7 +289,7 @@ class PagedKvPool:
         b = seqlens_k.numel() - 1
         dev = self.device
         table = self._table(block_table, b, "paged keys_values")
-        cu = _ints(seqlens_k, torch.int32, dev, "paged keys_values: seqlens_k")
+        cu = _lengths(seqlens_k, dev, "paged keys_values: seqlens_k")
         dtype = dtype or (torch.bfloat16 if self.dtype == A.FP8 else self.k.dtype)
         total, h, d = int(total), self.kv_heads, self.head_dim
         k = torch.empty_strided((total, h, d), (h * d, d, 1), dtype=dtype, device=dev)
@@ -317,8 +322,8 @@ class PagedKvPool:
             raise ValueError(f"paged attention: {seqlens_q.numel()} cumulative lengths do not go with {kv_len.numel()} sequences")
         out, os = _out_like(q, out, "paged attention: out")
         table = self._table(block_table, b, "paged attention")
-        cu = _ints(seqlens_q, torch.int32, dev, "paged attention: seqlens_q")
-        lens = _ints(kv_len, torch.int32, dev, "paged attention: kv_len")
+        cu = _lengths(seqlens_q, dev, "paged attention: seqlens_q")
+        lens = _lengths(kv_len, dev, "paged attention: kv_len")
         alibi, ap, abs_ = None, 0, 0
         if cfg.alibi_slopes is not None:
             alibi = cfg.alibi_slopes.to(device=dev, dtype=torch.float32).contiguous()

@@ -625,3 +625,21 @@ def test_wide_page_numbers_and_lengths_stay_out_of_range(P):
         b.check(got, c)
         for t, x in hold:
             t[keep.long()] = x
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_lengths_that_are_columns_of_a_matrix(P, lq):
+    """Lengths and cumulative lengths as (n, 1) columns of a scheduler's matrix, and a single sequence's as a number."""
+    c = cfg(P, 128)
+    b = Batch(P, [lq, lq, lq], [50, 333, 120], seed=7)
+    want = b.run(c).clone()
+    info = torch.zeros((4, 3), dtype=torch.int32, device="cuda")
+    info[:, 0], info[:3, 2] = b.cu, b.kv_len
+    got = b.pool.attention(b.q, info[:, :1], b.table, info[:3, 2:], lq, 333, c)
+    assert torch.equal(got, want)
+    info[:, 1] = torch.tensor([0, 50, 383, 503])
+    for x, y in zip(b.pool.keys_values(b.table, info[:, 1:2], 503), b.pool.keys_values(b.table, info[:, 1].contiguous(), 503)):
+        assert torch.equal(x, y)
+    got = b.pool.attention(b.q[:lq], b.cu[:2], b.table[:1], b.kv_len[0], lq, 333, c)
+    b.lq, b.lk = [lq], [50]
+    b.check(got, c)

@@ -240,3 +240,14 @@ def test_wide_integers_are_not_wrapped(P):
     assert paged._ints(torch.tensor([2 ** 31 + 5, 3]).to(torch.uint32), torch.int32, cpu, "x").tolist() == [2 ** 31 - 1, 3]
     assert paged._ints(torch.tensor([3, 250]).to(torch.uint8), torch.int32, cpu, "x").tolist() == [3, 250]
     assert paged._ints(wide, torch.int64, cpu, "x") is wide
+
+
+def test_lengths_out_of_any_shape(P):
+    from candle_rocm_vulkan_b200 import paged
+    cpu = torch.device("cpu")
+    info = torch.arange(12, dtype=torch.int32).view(4, 3)
+    for t, want in ((info[:, :1], [0, 3, 6, 9]), (info[:, 2], [2, 5, 8, 11]), (info[2, 1], [7]), (info[:, 1:2].long(), [1, 4, 7, 10]), (info[:0, :1], [])):
+        got = paged._lengths(t, cpu, "x")
+        assert got.tolist() == want and got.dtype == torch.int32 and got.dim() == 1 and got.is_contiguous()
+    one = info[:, 0].contiguous()
+    assert paged._lengths(one, cpu, "x") is one

@@ -1560,7 +1560,7 @@ __device__ __forceinline__ void p3_body(const FaParams &p, const CUtensorMap &tm
                         ks = *reinterpret_cast<const uint32_t *>(pg.pool.ks + at);
                         vs = *reinterpret_cast<const uint32_t *>(pg.pool.vs + at);
                     } else {
-                        ks = vs = 0;
+                        ks = vs = 0x7f7f7f7fu << (8 * nb);  // (bytes that no block has are in every type's range)
                         for (uint32_t i = 0; i < nb; ++i) ks |= (uint32_t)pg.pool.ks[at + i] << (8 * i), vs |= (uint32_t)pg.pool.vs[at + i] << (8 * i);
                     }
                 };

@@ -123,3 +123,14 @@ def test_keys_behind_the_smallest_scale_count(P, lq, d):
     b.q = (b.q.float() * 2.0 ** 100).bfloat16()
     c = P.FlashAttnConfig(2.0 ** 16).causal()
     b.check(b.run(c), c)
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("lo,hi", [(110, 125), (95, 120), (103, 104), (102, 103), (0, 1)])
+def test_f16_chunks_over_small_scales(P, d, lo, hi):
+    """Rows whose scales f16 has, rows whose it has not, and both, in a chunk's tiles, where a row has one to four of them."""
+    b = Apart(P, [60, 300], [333, 500], dt="f16", form="mxfp8", d=d, seed=lo + d)
+    for s in (b.pool.k_scale, b.pool.v_scale):
+        s.copy_(torch.randint(lo, hi, s.shape, generator=b.g, device="cuda"))
+    c = cfg(P, d)
+    b.check(b.run(c), c)

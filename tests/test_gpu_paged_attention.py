@@ -643,3 +643,25 @@ def test_lengths_that_are_columns_of_a_matrix(P, lq):
     got = b.pool.attention(b.q[:lq], b.cu[:2], b.table[:1], b.kv_len[0], lq, 333, c)
     b.lq, b.lk = [lq], [50]
     b.check(got, c)
+
+
+@pytest.mark.parametrize("dt,form", [("bf16", None), ("bf16", "mxfp8"), ("f16", "mxfp8")])
+@pytest.mark.parametrize("page", [5, 16, 32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_pages_outside_the_pool_in_every_form(P, dt, form, page, d):
+    """Steps and chunks, tensor copies and 16-byte chunks, codes and elements: bad pages hold zeros, and no wait runs out."""
+    b = Batch(P, [1, 5, 40], [64, 200, 190], seed=5, page=page, form=form, dt=dt, d=d)
+    c = cfg(P, d)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cols = [64 // page - 1, 100 // page, 70 // page]
+    keep = [b.table[i, j].clone().long() for i, j in enumerate(cols)]
+    table = b.table.clone()
+    for i, bad in enumerate((-3, b.pool.num_blocks, 2 ** 31 - 1)):
+        table[i, cols[i]] = bad
+    got = b.pool.attention(b.q, b.cu, table, b.kv_len, 40, 200, c, status=status).clone()
+    assert int(status) == 3
+    for p in keep:
+        for t in (b.pool.k, b.pool.v):
+            (t if form is None else t.view(torch.uint8))[p] = 0
+    b.check(got, c)
+    assert P._abi.lib().b200_device_wait_status() == 0

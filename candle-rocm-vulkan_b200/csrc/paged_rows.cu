@@ -199,10 +199,13 @@ __global__ void __launch_bounds__(PR_WARPS * 32, 8) paged_rows_kernel(const Rows
     if (TURN) {
         for (uint32_t f = lane; f < half; f += 32) {
             const uint32_t a = p.rot.axis ? min((uint32_t)p.rot.axis[f], p.rot.n_axes - 1) : 0u;
-            // the angle in turns; its whole turns leave before it is rounded to f32
-            const double t = (double)p.rot.pos[a * p.rot.pos_stride + token] * (double)p.rot.freq[f] * 0.15915494309189533577;
-            float s, k;
-            sincospif((float)(2.0 * (t - rint(t))), &s, &k);
+            // the angle in turns; its whole turns leave before it is rounded to f32, and what the rounding leaves (up to 2^-25 of a half turn, as much as
+            // all other roundings of a turned element together) turns sine and cosine a little further
+            const double t = (double)p.rot.pos[a * p.rot.pos_stride + token] * (double)p.rot.freq[f] * 0.15915494309189533577, h = 2.0 * (t - rint(t));
+            const float hi = (float)h, lo = (float)(h - (double)hi) * 3.14159265358979f;
+            float s0, k0;
+            sincospif(hi, &s0, &k0);
+            const float s = fmaf(lo, k0, s0), k = fmaf(-lo, s0, k0);
             s_cs[warp][f] = make_float2(k, s * p.rot.sign);
         }
         __syncwarp();

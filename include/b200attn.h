@@ -430,8 +430,8 @@ int b200_tq_attention_gather(const B200TqAttnArgs *args, const B200PeerGather *g
  * Head dims: every multiple of 8 up to 256 (kernel_supported of candle-core/src/accel/attention.rs:283-290 takes any
  * d <= 256; others return B200_ERR_UNSUPPORTED_SHAPE and the caller's unfused path serves them).
  * A masked key has weight zero in its row, which makes nothing of an infinite or NaN value where the row's tile holds that key:
- * such a value reaches the rows that see it and, at most, those of the same tile of up to 128 packed query rows (256 in the
- * 16-byte chunk tiles), never another tile's, another sequence's or rows past the end of a block. */
+ * such a value reaches the rows that see it and, at most, those of the same tile of up to 256 packed query rows, never another
+ * tile's, another sequence's or rows past the end of a block. */
 typedef struct B200FaArgs {
     const void *q, *k, *v;
     void *o;
@@ -563,8 +563,11 @@ int b200_paged_unpack(const B200PagedUnpackArgs *args, b200_stream_t stream);
  * without a visible key give zeros; scores scale * q . k, then softcap (> 0) and ALiBi. All lengths are read on the
  * device: nothing synchronises, and a captured call follows them. max_q, max_k and the table's columns bound the lengths (longer
  * ones are cut) and size the launches; total_q bounds cu_q[b], and rows of `out` in front of cu_q[0] and behind cu_q[b] are left as they were. q and out of q_dtype
- * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows; out does not overlap q. An MXFP8
- * pool's values count as q_dtype holds them (f16: an infinity above 65504).
+ * (f16 or bf16; a 16-bit pool holds the same type), (token, head) element strides, 16-byte aligned rows; out does not overlap q.
+ * An MXFP8 pool's values count as q_dtype holds code times power of two, rounded once (f16: in steps of 2^-24 below 2^-14, an infinity above
+ * 65504); so do its keys where a sequence has more new tokens than a few, whose scores take the keys as they are. A masked key has weight
+ * zero, which makes nothing of an infinite or NaN value: that reaches, of the same sequence and kv head, the rows that see the key and at most
+ * those of the same up to 256 packed rows.
  * A call is up to three launches that hand partial results on in the workspace: calls that may come in between one another, on
  * different streams or from threads that share one, need different workspaces.
  * The reference gathers the pages on the host (candle-flash-attn/src/lib.rs:341-420). */

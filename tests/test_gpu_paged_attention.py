@@ -665,3 +665,20 @@ def test_pages_outside_the_pool_in_every_form(P, dt, form, page, d):
             (t if form is None else t.view(torch.uint8))[p] = 0
     b.check(got, c)
     assert P._abi.lib().b200_device_wait_status() == 0
+
+
+@pytest.mark.parametrize("form", [None, "mxfp8"])
+@pytest.mark.parametrize("lq,clean", [(4, 0), (8, 4), (300, 256)])
+def test_how_far_a_masked_nan_reaches(P, form, lq, clean):
+    """A NaN among the last token's value: rows that see it have it, and at most those of the same 16 packed rows (steps) or 256 (tiles: a
+    group of 128 that does not see it may share its step of 16 keys)."""
+    b = Batch(P, [lq, lq], [lq + 500, 90 + lq], form=form, seed=18)
+    c = cfg(P, 128)
+    want = b.run(c).clone()
+    last = b.lk[0] - 1
+    b.pool.v.view(torch.uint8 if form else torch.int16)[b.table[0, last // b.page].long(), last % b.page, 1, 7] = 0x7f if form else 0x7fff
+    out = b.run(c)
+    assert bool(out[lq - 1, 4:, 7].isnan().all())
+    assert torch.equal(out[:clean], want[:clean]) and torch.equal(out[lq:], want[lq:]) and torch.equal(out[:, :4], want[:, :4])
+    out[:lq, 4:, 7] = want[:lq, 4:, 7]
+    assert torch.equal(out, want)

@@ -13,9 +13,9 @@
 // across columns too; scores and sums run on mma.sync m16n8k16, and the warps' partial results meet in shared memory at a
 // column's end.
 //
-// Measured (32 / 8 heads of 128; copy bandwidth 6 470 GB/s): 64 sequences of 500 to 8192 keys, bf16, 185 us, 0.95 of the copy; 48 x 4 tokens over
-// 4000 to 30000 keys, MXFP8, 387 us, 0.69: there the loads alone take 281 and the instructions alone 278, on two blocks of four warps per SM, which is
-// what the registers hold. A fifth warp per block for the copies (463: its registers come from the others), E4M3 operands for the scores with q in two parts
+// Measured (32 / 8 heads of 128; copy bandwidth 6 470 GB/s), L2 flushed: 64 sequences of 500 to 8192 keys, bf16, 195 us, 0.90 of the copy (179 to 192 back to
+// back); 48 x 4 tokens over 4000 to 30000 keys, MXFP8, 419 us, 0.64 (384 to 407). There, at 387, the loads alone took 281 and the instructions alone 278, on two
+// blocks of four warps per SM: what 251 registers leave, which 16 rows of accumulators need whatever the column has. A fifth warp per block for the copies (463: its registers come from the others), E4M3 operands for the scores with q in two parts
 // (477) and the code without its rare forms (380) were tried.
 //
 // MXFP8 keys and values stay codes up to the registers. Scores: the codes are exact in f16; q is taken to f16 behind a power of

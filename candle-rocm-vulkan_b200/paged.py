@@ -165,7 +165,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     """`q` (tokens, q_heads, head_dim) and `k` (tokens, kv_heads, head_dim; or None) turned by the angles of `positions` (axes, tokens),
     in one launch: (q_out, k_out), new tensors unless given (`q_out=q`: in place). The angles are formed in 64 bits from whole
     positions; the elements are turned in f32 and rounded once. `inverse=True` turns back: the gradient with respect to q and
-    k of a call's outputs' gradients."""
+    k of a call's outputs' gradients. No graph is recorded: a program that trains makes that call in its own backward pass."""
     _need_cuda(q, "q")
     q, (tokens, hq, d), qs = _heads(q, "rotary: q")
     device = q.device
@@ -307,7 +307,8 @@ class PagedKvPool:
         bottom-right aligned as for `flash_attn_varlen`; rows without a visible key give zeros. The lengths are read on the device;
         `max_seqlen_q` and `max_seqlen_k` bound them (longer ones are cut). Rows of `out` (a new tensor unless given) behind the last
         sequence are left as they were; `out` must not overlap `q`. Page numbers outside the pool hold zeros and set `status` (an int32 device
-        tensor) to 3. MXFP8 values count as q's type holds them (f16: up to 65504, as far as sums of weights with them go)."""
+        tensor) to 3. MXFP8 values count as q's type holds them (f16: in steps of 2^-24 below 2^-14, infinite
+        above 65504), and so do the keys of a chunk; those of a few tokens count as they are."""
         dev = self.device
         q, (total, hq, _), qs = _heads(q, "paged attention: q", None, self.head_dim)
         if q.device != dev:

@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _abi as A
-from .turbo_quant import FlashAttnConfig, _DTYPES, _capturing, _dtype_id, _need_cuda, _stream, _workspace
+from .turbo_quant import FlashAttnConfig, _DTYPES, _WORKSPACE_KEPT, _capturing, _dtype_id, _need_cuda, _stream
 
 _E4M3 = getattr(torch, "float8_e4m3fn", None)
 _POOL_DTYPES = {torch.float16: A.F16, torch.bfloat16: A.BF16, _E4M3: A.FP8}
@@ -45,13 +45,25 @@ def _call(fn, args: bytes, device):
         A.check(rc)
 
 
-_this_thread = threading.get_ident
+class _Kept(threading.local):
+    def __init__(self):
+        self.buffers = {}
+
+
+_KEPT = _Kept()
 
 
 def _scratch(device, nbytes: int, stream: int) -> torch.Tensor:
-    """`_workspace` of this thread on this stream. An attention call is up to three launches that hand partial results on, and threads that share a
-    stream may come in between one another's: each has scratch of its own."""
-    return _workspace(device, nbytes, (stream, _this_thread()))
+    """Scratch for a call on the current stream, of this thread's own: an attention call is up to three launches that hand partial results on, and
+    threads that share a stream may come in between one another's. Up to _WORKSPACE_KEPT bytes it is one growing buffer per stream, as in
+    `_workspace`, but what was outgrown, and all when the thread ends, returns to torch's allocator in the order of the stream: no graph knows it."""
+    ws = _KEPT.buffers.get((device, stream))
+    if ws is None or ws.numel() < nbytes:
+        if nbytes > _WORKSPACE_KEPT:
+            return torch.empty((nbytes + 15) // 16 * 16, dtype=torch.uint8, device=device)
+        ws = torch.empty(max(1 << 20, 1 << (nbytes - 1).bit_length()), dtype=torch.uint8, device=device)
+        _KEPT.buffers[device, stream] = ws
+    return ws
 
 
 def _ints(t: torch.Tensor, dtype, device, what: str) -> torch.Tensor:

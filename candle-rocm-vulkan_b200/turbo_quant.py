@@ -346,9 +346,9 @@ _WORKSPACES_OUTGROWN = []
 _WORKSPACE_KEPT = 32 << 20
 
 
-def _workspace(device, nbytes: int, stream=None) -> torch.Tensor:
-    """Scratch for a call on the current stream (or what else a caller keeps buffers by: `stream`). Up to _WORKSPACE_KEPT bytes it is one growing buffer
-    per (device, stream): calls on one stream are ordered, so they can share it (the reference allocates the split buffers per call, accel.rs:190-199).
+def _workspace(device, nbytes: int, stream: Optional[int] = None) -> torch.Tensor:
+    """Scratch for a call on the current stream. Up to _WORKSPACE_KEPT bytes it is one growing buffer per (device, stream): calls
+    on one stream are ordered, so they can share it (the reference allocates the split buffers per call, accel.rs:190-199).
     A graph may have captured the address of a buffer that has become too small, so these stay; sizes double, which makes
     them one more _WORKSPACE_KEPT in all. Larger requests (16-bit copies of f32 tensors take up to 256 MB) come from torch's
     allocator and return to it after the call, in the order of the stream."""

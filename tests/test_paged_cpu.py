@@ -251,3 +251,26 @@ def test_lengths_out_of_any_shape(P):
         assert got.tolist() == want and got.dtype == torch.int32 and got.dim() == 1 and got.is_contiguous()
     one = info[:, 0].contiguous()
     assert paged._lengths(one, cpu, "x") is one
+
+
+def test_scratch_grows_and_ends_with_its_thread(P):
+    import gc
+    import threading
+    import weakref
+    from candle_rocm_vulkan_b200 import paged
+    cpu, gone = torch.device("cpu"), []
+
+    def work():
+        small = paged._scratch(cpu, 100, 3)
+        assert small.numel() == 1 << 20 and paged._scratch(cpu, 1 << 20, 3) is small
+        large = paged._scratch(cpu, (1 << 20) + 1, 3)
+        assert large.numel() == 2 << 20 and paged._scratch(cpu, 5, 3) is large
+        over = paged._scratch(cpu, paged._WORKSPACE_KEPT + 3, 3)  # not kept
+        assert over.numel() >= paged._WORKSPACE_KEPT + 3 and paged._scratch(cpu, 5, 3) is large
+        gone.extend(weakref.ref(t) for t in (small, large, over))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    gc.collect()
+    assert len(gone) == 3 and all(r() is None for r in gone)
